@@ -13,6 +13,7 @@ Reference call sites these replace: apex/TorchScript fused ops in ``megatron/mod
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -32,6 +33,30 @@ def _k(*ts) -> bool:
 
 def _s():
     return ctypes.c_void_p(native.stream_ptr())
+
+
+_HERE = contextlib.nullcontext()
+
+
+def device_of(t):
+    """Context in which a GPU tensor's device is the current one, so that a launch and its stream belong to it."""
+    return _HERE if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+
+
+class _Once(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, g, x):
+        return g.view_as(g)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("this operator's gradient cannot be differentiated a second time")
+
+
+def once(g, x):
+    """``g``, the gradient a kernel has computed from ``x``.  Under ``create_graph`` it depends on ``x`` in a way that nothing
+    records: differentiating it is then an error instead of a term that is silently missing."""
+    return _Once.apply(g, x) if torch.is_grad_enabled() and x.requires_grad else g
 
 
 _workspaces = {}

@@ -14,16 +14,25 @@ moe_mlp.py`` (grouped expert MLP through MegaBlocks' ``gmm``), ``megatron/model/
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import torch
 import torch.nn.functional as F
 
 from . import flop_count, native
 from . import gemm as G
-from .functional import _DT, dgelu_mul
+from .functional import _DT, device_of, dgelu_mul, once
 from .linear import main_grad_of
 
 PAD = 64
+
+_P, _I, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
+native._ARGTYPES.update({
+    "neox_router_blocks": [_L, _I],
+    "neox_balanced_router": [_P, _L, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P],
+    "neox_balanced_router_grad": [_P, _L, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P],
+})
+native._CountingLib._NOT_LAUNCHES.add("neox_router_blocks")
 
 
 def padded_rows(assignments: int, experts: int) -> int:
@@ -84,6 +93,111 @@ def router(logits, k):
     if router_kernel_ok(logits, k):
         return _RouterFn.apply(logits, k)
     return router_ref(logits, k)
+
+
+# ------------------------------------------------------------------------------------------------ router with its losses
+class RouterOutput(NamedTuple):
+    """``weights`` ``[T, k]`` fp32, ``experts`` ``[T, k]`` int64, ``counts`` ``[E]`` int64 (of all tokens), and the scalar losses
+    ``balance`` and ``z``; weights and losses are differentiable."""
+    weights: torch.Tensor
+    experts: torch.Tensor
+    counts: torch.Tensor
+    balance: torch.Tensor
+    z: torch.Tensor
+
+
+def balanced_router_ref(logits, k, token_mask=None):
+    """:func:`balanced_router` in plain PyTorch."""
+    E = logits.shape[1]
+    wide = logits if logits.dtype == torch.float64 else logits.float()
+    experts = logits.detach().sort(dim=-1, descending=True, stable=True).indices[:, :k].contiguous()
+    p, lse = wide.softmax(-1), wide.logsumexp(-1)
+    w = p.gather(-1, experts)
+    if k > 1:
+        w = w / w.sum(-1, keepdim=True)
+    kept = torch.ones_like(lse, dtype=torch.bool) if token_mask is None else token_mask.bool()
+    counts = torch.bincount(experts.reshape(-1), minlength=E)
+    load = torch.bincount(experts[kept].reshape(-1), minlength=E).to(wide.dtype)
+    n = kept.sum().clamp(min=1).to(wide.dtype)
+    balance = E * (load / (n * k) * (p[kept].sum(0) / n)).sum()
+    z = lse[kept].square().sum() / n
+    return RouterOutput(w, experts, counts, balance, z)
+
+
+def _balanced_values(x, k, kept):
+    T, E = x.shape
+    L, dev = native.lib(), x.device
+    weights = torch.empty(T, k, dtype=torch.float32, device=dev)
+    experts = torch.empty(T, k, dtype=torch.int64, device=dev)
+    row = torch.empty(T, 4, dtype=torch.float32, device=dev)
+    counts = torch.empty(E, dtype=torch.int64, device=dev)
+    load = torch.empty(E + 1, dtype=torch.float32, device=dev)
+    out = torch.empty(2, dtype=torch.float32, device=dev)
+    scratch = torch.empty(L.neox_router_blocks(T, E) * (E * 12 + 8) + 16 * 17 + 16, dtype=torch.uint8, device=dev)
+    rc = L.neox_balanced_router(x.data_ptr(), x.stride(0), None if kept is None else kept.data_ptr(), T, E, k, _DT[x.dtype],
+                                weights.data_ptr(), experts.data_ptr(), row.data_ptr(), counts.data_ptr(), load.data_ptr(),
+                                out.data_ptr(), scratch.data_ptr(), native.stream_ptr())
+    native.check(rc, "neox_balanced_router")
+    balance, z = out.unbind(0)
+    return weights, experts, counts, balance, z, row, load
+
+
+class _BalancedRouterFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, k, kept):
+        with device_of(x):
+            weights, experts, counts, balance, z, row, load = _balanced_values(x, k, kept)
+        # the weights are an output: saved as such, so that changing them in place is noticed
+        ctx.save_for_backward(x, kept, weights, experts, row, load)
+        ctx.k = k
+        ctx.mark_non_differentiable(experts, counts)
+        ctx.set_materialize_grads(False)
+        return weights, experts, counts, balance, z
+
+    @staticmethod
+    def backward(ctx, g_weights, _e, _c, g_balance, g_z):
+        x, kept, weights, experts, row, load = ctx.saved_tensors
+        T, E = x.shape
+        dx = torch.empty(T, E, dtype=x.dtype, device=x.device)
+        gw, gb, gz = (None if g is None else g.float().contiguous() for g in (g_weights, g_balance, g_z))
+        with device_of(x):
+            rc = native.lib().neox_balanced_router_grad(
+                x.data_ptr(), x.stride(0), None if kept is None else kept.data_ptr(), T, E, ctx.k, _DT[x.dtype],
+                weights.data_ptr(), experts.data_ptr(), row.data_ptr(), load.data_ptr(), None if gw is None else gw.data_ptr(),
+                None if gb is None else gb.data_ptr(), None if gz is None else gz.data_ptr(), dx.data_ptr(),
+                native.stream_ptr())
+            native.check(rc, "neox_balanced_router_grad")
+        return once(dx, x), None, None
+
+
+def balanced_router(logits, k, token_mask=None):
+    """Router of ``logits`` ``[T, E]`` together with the losses that train it, gradients from all of them in one pass::
+
+        p = softmax(logits);  experts = the k largest logits (of equal ones the lower index);  weights = p[experts],
+        divided by their sum for k > 1;  counts = tokens per expert
+        balance = E * sum_e f_e * P_e          f: share of the choices that went to an expert (a constant), P: mean of p
+        z = mean(logsumexp(logits) ** 2)
+
+    ``token_mask`` (``[T]``, bool): tokens that count for ``balance`` and ``z``; the others (padding) are routed all the same and
+    are in ``counts``.  No kept token: both losses are zero.  Up to 512 experts and eight choices run as kernels
+    (``csrc/moe_balance.cu``); the gradient can be taken once, not differentiated again."""
+    if logits.dim() != 2 or not logits.is_floating_point():
+        raise ValueError(f"router logits are [tokens, experts] floating-point numbers, got {tuple(logits.shape)} {logits.dtype}")
+    if not 1 <= k <= logits.shape[1]:
+        raise ValueError(f"top-k is between 1 and the number of experts, got {k} of {logits.shape[1]}")
+    if token_mask is not None:
+        if token_mask.shape != logits.shape[:1] or token_mask.dtype != torch.bool:
+            raise ValueError(f"token_mask is bool [{logits.shape[0]}], got {token_mask.dtype} {tuple(token_mask.shape)}")
+        if token_mask.device != logits.device:
+            raise ValueError(f"token_mask is on {token_mask.device}, the logits are on {logits.device}")
+    if not router_kernel_ok(logits, k):
+        return balanced_router_ref(logits, k, token_mask)
+    x = logits if logits.stride(1) == 1 or logits.shape[1] == 1 else logits.contiguous()
+    kept = None if token_mask is None else token_mask.contiguous()
+    if native.plain_call(logits):
+        with device_of(x):
+            return RouterOutput(*_balanced_values(x, k, kept)[:5])
+    return RouterOutput(*_BalancedRouterFn.apply(x, k, kept))
 
 
 # ------------------------------------------------------------------------------------------------ row plan
