@@ -15,8 +15,11 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <float.h>
+#include <limits.h>
 #include <stdint.h>
 
+#include "dynamic_smem.h"
+#include "launch.cuh"
 #include "neox_b200.h"
 
 namespace {
@@ -75,14 +78,81 @@ template <typename T> __device__ __forceinline__ uint4 repack(const float (&v)[E
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
-// Largest element (NaN is passed over: it shows in the sum).
-template <typename T> __device__ __forceinline__ float largest(const uint4& u) {
-    float v[Elem<T>::PER_16];
-    unpack<T>(u, v);
-    float m = v[0];
+// Largest element of one and of many (NaN is passed over: it shows in the sum).
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b, __nv_bfloat16) {
+    const __nv_bfloat162 m = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b, __half) {
+    const __half2 m = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b, float) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+}
+template <typename T> __device__ __forceinline__ uint32_t larger(const uint4& u) {
+    return larger(larger(u.x, u.y, T()), larger(u.z, u.w, T()), T());
+}
+template <typename T> __device__ __forceinline__ float as_max(uint32_t w) {
+    if constexpr (Elem<T>::PER_16 == 4) return __uint_as_float(w);
+    else {
+        const float2 f = two(w, T());
+        return fmaxf(f.x, f.y);
+    }
+}
+
+// Two 32-bit floats in one instruction.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 parts(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f32x2 add(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+constexpr float LOG2E = 1.4426950408889634f;
+__device__ __forceinline__ float exp2_fast(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+// exp(x + shift).  The sum first: a row's largest and lowest numbers may be as large as the type has them, and the difference of
+// two 16-bit numbers near each other is exact.
+__device__ __forceinline__ f32x2 exp_of(f32x2 x, f32x2 shift) {
+    const float2 t = parts(mul(add(x, shift), pair(LOG2E, LOG2E)));
+    return pair(exp2_fast(t.x), exp2_fast(t.y));
+}
+// The elements of 16 bytes as pairs.
+template <typename T> __device__ __forceinline__ void pairs_of(const uint4& u, f32x2 (&v)[Elem<T>::PER_16 / 2]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    if constexpr (Elem<T>::PER_16 == 4) {
+        v[0] = pair(__uint_as_float(w[0]), __uint_as_float(w[1]));
+        v[1] = pair(__uint_as_float(w[2]), __uint_as_float(w[3]));
+    } else {
 #pragma unroll
-    for (int i = 1; i < Elem<T>::PER_16; ++i) m = fmaxf(m, v[i]);
-    return m;
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = two(w[i], T());
+            v[i] = pair(f.x, f.y);
+        }
+    }
 }
 
 // Logits are read once a pass: they stay out of L1.
@@ -92,6 +162,14 @@ __device__ __forceinline__ uint4 load_16(const void* p) {
                  : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
+
+// Asynchronous copies of 16 bytes to shared memory, in groups: `copies_here<K>` waits until all but the last K groups of this thread
+// have arrived.  Each thread reads only what it copied itself.
+__device__ __forceinline__ void copy_16(void* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_sent() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int K> __device__ __forceinline__ void copies_here() { asm volatile("cp.async.wait_group %0;" ::"n"(K) : "memory"); }
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -129,18 +207,40 @@ struct Rows {
     }
 };
 
+// ---------------------------------------------------------------------------------------------- statistics of the kept rows
+// One block an SM: its warps, a lane's 16-byte vectors a step, and steps in shared memory, the one being worked on among them.
+template <bool FULL> struct Shape {
+    static constexpr int WARPS = FULL ? 16 : 24, STAGES = FULL ? 3 : 2, VECTORS = 6;
+};
+constexpr int MOST_ROWS = 1024;                                 // rows a block keeps at a time
+constexpr int SCAN = 8;                                         // mask words a lane has in flight
+
 struct StatsArgs {
     Rows x, y;                     // policy and reference
     const long long* labels;       // [n, s]
     const float* mask;             // [n, s]
-    float* part;                   // planes of [rows, splits]: max, sum (policy), max, sum (reference), sum p (x - y)
-    float* target;                 // planes of [rows]: the label's logit where this share of the vocabulary has it, else 0
-    int* ticket;
+    float2* part;                  // [streams][rows, most]: (max, sum) of a chunk of a row
+    float* cross;                  // [rows, most]: sum of p (x - y)
+    float* target;                 // [streams][rows]: the label's logit where this share of the vocabulary has it, else 0
+    int* ticket;                   // zero for the next kernel, then the number of chunks
     long long v0;
-    int rows, s, vocab, splits, chunk;
+    int rows, s, vocab;
+    int streams;                   // 2: the reference's rows are further rows; 1 for the KL over the vocabulary, which reads both at once
+    int chunks, most;              // of a row: as many as suit a batch that keeps everything, and the most there is room for
 };
 
-// A row's sums over one chunk, joined over the G threads that share it.  (m, t): maximum and sum of exponentials.
+// Into how many chunks each of `rows` rows is cut.  A chunk's end costs a warp about what PER_CHUNK further elements do; a warp
+// that is left alone with its last chunk works about four times as fast as one among many.
+constexpr int PER_CHUNK = 1280;
+__host__ __device__ __forceinline__ float cut_cost(long long rows, int vocab, int chunks, int blocks, int warps) {
+    const long long block = (rows * chunks + blocks - 1) / blocks;
+    const float size = (float)((vocab + chunks - 1) / chunks), each = (float)block / (float)warps;
+    return fmaxf(each, 0.25f) * (size + PER_CHUNK) + 0.25f * size;
+}
+// Elements of a chunk; the count that goes with it is at most `chunks`.
+__host__ __device__ __forceinline__ int chunk_size(int vocab, int chunks) { return ((vocab + chunks - 1) / chunks + 7) / 8 * 8; }
+
+// (m, t): maximum and sum of exponentials against it.
 struct Sums {
     float m, t;
     __device__ __forceinline__ void join_warp() {
@@ -150,213 +250,344 @@ struct Sums {
     }
 };
 
-// G threads a chunk of a row, U 16-byte loads a thread, all of them in flight before the first is used.  A thread takes the
-// maximum of what it holds and the exponentials against that, so nothing is rescaled inside the loop.
-template <typename T, int G, int U>
-__global__ void __launch_bounds__(THREADS) stats_kernel(const StatsArgs a) {
-    constexpr int N = Elem<T>::PER_16;
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.ticket = 0;
-    const unsigned item = blockIdx.x * (THREADS / G) + threadIdx.x / G;
-    const int lane = threadIdx.x % G, which = blockIdx.y;
-    const int row = (int)(item / (unsigned)a.splits), part = (int)(item % (unsigned)a.splits);
-    if (row >= a.rows) return;
-    const long long cells = (long long)a.rows * a.splits;
-    float* out_m = a.part + 2 * which * cells + item;
-    float* out_t = out_m + cells;
-    if (a.mask[row] == 0.f) {
-        if (lane == 0) {
-            *out_m = -FLT_MAX;
-            *out_t = 0.f;
-            if (part == 0) a.target[(long long)which * a.rows + row] = 0.f;
-        }
-        return;
-    }
-    const T* x = (which ? a.y : a.x).at<T>(row / a.s, row % a.s);
-    if (part == 0 && lane == G - 1) {
-        const long long y = a.labels[row] - a.v0;
-        a.target[(long long)which * a.rows + row] = y >= 0 && y < a.vocab ? Elem<T>::get(x[y]) : 0.f;
-    }
-    const int c0 = part * a.chunk, count = min(a.chunk, a.vocab - c0);
-    x += c0;
-    const Cut<T> cut(x, count);
-    const uint4* xv = reinterpret_cast<const uint4*>(x + cut.head);
-    uint4 raw[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-        if (lane + u * G < cut.vectors) raw[u] = load_16(xv + lane + u * G);
-    Sums r{-FLT_MAX, 0.f};
-    float edge = -INFINITY;                                     // head and tail: at most one element a thread
-    if (lane < cut.head) edge = Elem<T>::get(x[lane]);
-    else if (lane - N < cut.tail && lane >= N) edge = Elem<T>::get(x[cut.head + cut.vectors * N + lane - N]);
-    r.m = fmaxf(r.m, edge);
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-        if (lane + u * G < cut.vectors) r.m = fmaxf(r.m, largest<T>(raw[u]));
-    r.t = __expf(edge - r.m);
-    float t1 = 0.f;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-        if (lane + u * G < cut.vectors) {
-            float v[N];
-            unpack<T>(raw[u], v);
-#pragma unroll
-            for (int i = 0; i < N; i += 2) {
-                r.t += __expf(v[i] - r.m);
-                t1 += __expf(v[i + 1] - r.m);
-            }
-        }
-    r.t += t1;
-    r.join_warp();
-    if constexpr (G > 32) {
-        __shared__ Sums warps[THREADS / 32];
-        if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = r;
-        __syncthreads();
-        if (threadIdx.x >= 32) return;
-        r = lane < G / 32 ? warps[lane] : Sums{-FLT_MAX, 0.f};
-        r.join_warp();
-    }
-    if (lane == 0) {
-        *out_m = r.m;
-        *out_t = r.t;
-    }
-}
+struct Kept {                      // a kept row of this block
+    const void* x;
+    const void* y;
+    int row, stream;
+};
 
-// The same over policy and reference side by side, with the sum of p (x - y) that the KL over the vocabulary needs.  An entry of
-// probability zero adds nothing, also where both logits are -inf.
-template <typename T, int G, int U>
-__global__ void __launch_bounds__(THREADS) stats_full_kernel(const StatsArgs a) {
-    constexpr int N = Elem<T>::PER_16;
-    if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0;
-    const unsigned item = blockIdx.x * (THREADS / G) + threadIdx.x / G;
-    const int lane = threadIdx.x % G;
-    const int row = (int)(item / (unsigned)a.splits), part = (int)(item % (unsigned)a.splits);
-    if (row >= a.rows) return;
-    const long long cells = (long long)a.rows * a.splits;
-    float* out = a.part + item;
-    if (a.mask[row] == 0.f) {
-        if (lane == 0) {
-            out[0] = out[2 * cells] = -FLT_MAX;
-            out[cells] = out[3 * cells] = out[4 * cells] = 0.f;
-            if (part == 0) a.target[row] = 0.f;
-        }
-        return;
-    }
-    const T* x = a.x.at<T>(row / a.s, row % a.s);
-    const T* y = a.y.at<T>(row / a.s, row % a.s);
-    if (part == 0 && lane == G - 1) {
-        const long long l = a.labels[row] - a.v0;
-        a.target[row] = l >= 0 && l < a.vocab ? Elem<T>::get(x[l]) : 0.f;
-    }
-    const int c0 = part * a.chunk, count = min(a.chunk, a.vocab - c0);
-    x += c0;
-    y += c0;
-    Sums p{-FLT_MAX, 0.f}, q{-FLT_MAX, 0.f};
-    float w = 0.f;
-    if ((((uintptr_t)x ^ (uintptr_t)y) & 15) == 0) {
+template <bool FULL> struct StatsSmem {
+    using S = Shape<FULL>;
+    uint4 ring[S::STAGES][S::WARPS][S::VECTORS][32];
+    Kept list[MOST_ROWS];
+    int counts[S::WARPS];
+    int queue[S::WARPS][4];        // chunks a warp has taken and not yet begun to sum
+    int next;
+};
+
+// A warp's walk over its chunks, one step of at most 32 * U vectors at a time.
+template <typename T, bool FULL> struct Walk {
+    static constexpr int N = Elem<T>::PER_16, U = Shape<FULL>::VECTORS / (FULL ? 2 : 1), STEP = 32 * U;
+    const T* x;
+    const T* y;
+    int item, entry, part;         // (kept row, chunk) of this warp: number, row in the list, chunk
+    int count, vectors, head, done;
+    bool apart;                    // policy and reference rows that no common shift aligns
+
+    __device__ __forceinline__ void enter(const StatsArgs& a, const Kept* list, int first, int chunks, int chunk) {
+        const int kept = item / chunks;
+        part = item - kept * chunks;
+        entry = kept - first;
+        const int c0 = part * chunk;
+        count = min(chunk, a.vocab - c0);
+        x = static_cast<const T*>(list[entry].x) + c0;
+        if constexpr (FULL) y = static_cast<const T*>(list[entry].y) + c0;
         const Cut<T> cut(x, count);
-        const uint4* xv = reinterpret_cast<const uint4*>(x + cut.head);
-        const uint4* yv = reinterpret_cast<const uint4*>(y + cut.head);
-        uint4 xr[U], yr[U];
+        head = cut.head;
+        apart = FULL && (((uintptr_t)x ^ (uintptr_t)y) & 15) != 0;
+        vectors = apart ? 0 : cut.vectors;
+        done = 0;
+    }
+    __device__ __forceinline__ void request(uint4 (*slot)[32], int lane) const {
+        const uint4* xv = reinterpret_cast<const uint4*>(x + head) + done + lane;
+        const uint4* yv = FULL ? reinterpret_cast<const uint4*>(y + head) + done + lane : nullptr;
+        const int left = vectors - done - lane;
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (lane + u * G < cut.vectors) {
-                xr[u] = load_16(xv + lane + u * G);
-                yr[u] = load_16(yv + lane + u * G);
+            if (u * 32 < left) {
+                copy_16(&slot[u][lane], xv + u * 32);
+                if constexpr (FULL) copy_16(&slot[U + u][lane], yv + u * 32);
             }
-        float ex = -INFINITY, ey = -INFINITY;
-        int at = -1;
-        if (lane < cut.head) at = lane;
-        else if (lane - N < cut.tail && lane >= N) at = cut.head + cut.vectors * N + lane - N;
-        if (at >= 0) {
-            ex = Elem<T>::get(x[at]);
-            ey = Elem<T>::get(y[at]);
+    }
+    __device__ __forceinline__ bool ends() const { return done + STEP >= vectors; }
+};
+
+// What a lane has of a chunk so far: the largest logit and the sums against it.
+template <typename T, bool FULL> struct Running {
+    static constexpr int N = Elem<T>::PER_16, U = Shape<FULL>::VECTORS / (FULL ? 2 : 1);
+    float m, n;                    // policy, reference
+    f32x2 t, r, w;                 // sum of exponentials (policy, reference), sum of p (x - y)
+
+    __device__ __forceinline__ void clear() {
+        m = n = -FLT_MAX;
+        t = r = w = pair(0.f, 0.f);
+    }
+    // A new maximum: what was summed against the old one is scaled.
+    __device__ __forceinline__ void raise(float px, float qx) {
+        const float k = __expf(m - px);
+        m = px;
+        t = mul(t, pair(k, k));
+        if constexpr (FULL) {
+            const float kr = __expf(n - qx);
+            n = qx;
+            r = mul(r, pair(kr, kr));
+            w = mul(w, pair(k, k));
         }
-        p.m = fmaxf(p.m, ex);
-        q.m = fmaxf(q.m, ey);
+    }
+    __device__ __forceinline__ void add_vectors(const uint4 (&xr)[U], const uint4 (&yr)[FULL ? U : 1], int left, bool whole) {
+        uint32_t p = larger<T>(xr[0]), q = 0;
+        if constexpr (FULL) q = larger<T>(yr[0]);
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (lane + u * G < cut.vectors) {
-                p.m = fmaxf(p.m, largest<T>(xr[u]));
-                q.m = fmaxf(q.m, largest<T>(yr[u]));
+        for (int u = 1; u < U; ++u)
+            if (whole || u * 32 < left) {
+                p = larger(p, larger<T>(xr[u]), T());
+                if constexpr (FULL) q = larger(q, larger<T>(yr[u]), T());
             }
-        p.t = __expf(ex - p.m);
-        q.t = __expf(ey - q.m);
-        w = p.t > 0.f ? p.t * (ex - ey) : 0.f;
+        raise(fmaxf(m, as_max<T>(p)), FULL ? fmaxf(n, as_max<T>(q)) : 0.f);
+        const f32x2 xs = pair(-m, -m), ys = pair(-n, -n), minus = pair(-1.f, -1.f);
+        f32x2 gap = pair(0.f, 0.f);
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (lane + u * G < cut.vectors) {
-                float v[N], r[N];
-                unpack<T>(xr[u], v);
-                unpack<T>(yr[u], r);
+            if (whole || u * 32 < left) {
+                f32x2 v[N / 2], q2[N / 2];
+                pairs_of<T>(xr[u], v);
+                if constexpr (FULL) pairs_of<T>(yr[u], q2);
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const float e = __expf(v[i] - p.m);
-                    p.t += e;
-                    w += e > 0.f ? e * (v[i] - r[i]) : 0.f;
-                    q.t += __expf(r[i] - q.m);
+                for (int i = 0; i < N / 2; ++i) {
+                    const f32x2 e = exp_of(v[i], xs);
+                    t = add(t, e);
+                    if constexpr (FULL) {
+                        gap = fma(e, fma(q2[i], minus, v[i]), gap);
+                        r = add(r, exp_of(q2[i], ys));
+                    }
                 }
             }
-    } else {                                                    // rows that no common shift aligns: element by element
-        for (int c = lane; c < count; c += G) {
-            p.m = fmaxf(p.m, Elem<T>::get(x[c]));
-            q.m = fmaxf(q.m, Elem<T>::get(y[c]));
-        }
-        for (int c = lane; c < count; c += G) {
-            const float xe = Elem<T>::get(x[c]), ye = Elem<T>::get(y[c]), e = __expf(xe - p.m);
-            p.t += e;
-            w += e > 0.f ? e * (xe - ye) : 0.f;
-            q.t += __expf(ye - q.m);
+        if constexpr (FULL) {
+            const float2 g = parts(gap);
+            if (g.x + g.y != g.x + g.y) {                       // 0 times infinity somewhere: what is impossible adds nothing
+                float again = 0.f;
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (u * 32 < left) {
+                        float v[N], q1[N];
+                        unpack<T>(xr[u], v);
+                        unpack<T>(yr[u], q1);
+#pragma unroll
+                        for (int i = 0; i < N; ++i) {
+                            const float e = __expf(v[i] - m);
+                            again += e > 0.f ? e * (v[i] - q1[i]) : 0.f;
+                        }
+                    }
+                gap = pair(again, 0.f);
+            }
+            w = add(w, gap);
         }
     }
-    const float own = p.m;
-    p.join_warp();
-    w = warp_sum(w * __expf(own - p.m));
-    q.join_warp();
-    if constexpr (G > 32) {
-        __shared__ Sums ps[THREADS / 32], qs[THREADS / 32];
-        __shared__ float ws[THREADS / 32];
-        if ((threadIdx.x & 31) == 0) {
-            ps[threadIdx.x >> 5] = p;
-            qs[threadIdx.x >> 5] = q;
-            ws[threadIdx.x >> 5] = w;
+    __device__ __forceinline__ void add_one(float ex, float ey) {
+        raise(fmaxf(m, ex), FULL ? fmaxf(n, ey) : 0.f);
+        const float e = __expf(ex - m);
+        t = add(t, pair(e, 0.f));
+        if constexpr (FULL) {
+            w = add(w, pair(e > 0.f ? e * (ex - ey) : 0.f, 0.f));
+            r = add(r, pair(__expf(ey - n), 0.f));
         }
+    }
+};
+
+// One block an SM.  It counts the mask, so that every block gets the same number of chunks of kept rows; its warps then walk over
+// them.  A lane copies its own 16-byte vectors to shared memory ahead of the step it works on and reads back what it copied itself, so nothing waits for another lane until a chunk ends in one
+// (max, sum) that the next kernel joins.
+template <typename T, bool FULL>
+__global__ void __launch_bounds__(Shape<FULL>::WARPS * 32, 1) stats_kernel(const StatsArgs a) {
+    using W = Walk<T, FULL>;
+    constexpr int N = W::N, U = W::U, WARPS = Shape<FULL>::WARPS, STAGES = Shape<FULL>::STAGES;
+    extern __shared__ __align__(16) unsigned char raw_smem[];
+    StatsSmem<FULL>& sm = *reinterpret_cast<StatsSmem<FULL>*>(raw_smem);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    // each round: so many rows that this block's part fits its list
+    const int round = (int)min((long long)a.rows, (long long)gridDim.x * (MOST_ROWS - 2) / a.streams);
+    for (int base = 0; base < a.rows; base += round) {
+        const int rows = min(round, a.rows - base);
+        const int segment = ((rows + WARPS - 1) / WARPS + 31) / 32 * 32;
+        const int from = base + warp * segment, to = min(base + rows, from + segment);
+        int mine = 0;
+        for (int r = from; r < to; r += 32 * SCAN) {
+            float w[SCAN];
+#pragma unroll
+            for (int k = 0; k < SCAN; ++k) w[k] = r + k * 32 + lane < to ? a.mask[r + k * 32 + lane] : 0.f;
+#pragma unroll
+            for (int k = 0; k < SCAN; ++k) mine += __popc(__ballot_sync(0xffffffffu, w[k] != 0.f));
+        }
+        __syncthreads();                                        // the list of the round before is no longer read
+        if (lane == 0) sm.counts[warp] = mine;
         __syncthreads();
-        if (threadIdx.x >= 32) return;
-        p = lane < G / 32 ? ps[lane] : Sums{-FLT_MAX, 0.f};
-        q = lane < G / 32 ? qs[lane] : Sums{-FLT_MAX, 0.f};
-        w = lane < G / 32 ? ws[lane] : 0.f;
-        const float mine = p.m;
-        p.join_warp();
-        w = warp_sum(w * __expf(mine - p.m));
-        q.join_warp();
+        int before = 0, kept = 0;
+        for (int w = 0; w < WARPS; ++w) {
+            before += w < warp ? sm.counts[w] : 0;
+            kept += sm.counts[w];
+        }
+        int chunks = a.chunks;
+        if (round == a.rows) {                                  // all rows are known here: every block finds the same best cut
+            float best = INFINITY;
+            chunks = 1;
+            for (int c = 1 + lane; c <= a.most; c += 32) {
+                const float cost = cut_cost((long long)kept * a.streams, a.vocab, c, gridDim.x, WARPS);
+                if (cost < best) {
+                    best = cost;
+                    chunks = c;
+                }
+            }
+            const float least = -warp_max(-best);
+            chunks = __reduce_min_sync(0xffffffffu, best == least ? chunks : INT_MAX);
+        }
+        const int chunk = chunk_size(a.vocab, chunks);
+        chunks = (a.vocab + chunk - 1) / chunk;
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
+            a.ticket[0] = 0;
+            a.ticket[1] = chunks;
+        }
+        const long long items = (long long)kept * a.streams * chunks;
+        const int lo = (int)(items * blockIdx.x / gridDim.x), hi = (int)(items * (blockIdx.x + 1) / gridDim.x);
+        const int first = lo / chunks, end = (hi + chunks - 1) / chunks;
+        for (int k = 0; k < a.streams; ++k) {                   // the second stream's rows follow the first's
+            int rank = before + k * kept;
+            if (rank >= end || rank + mine <= first) continue;
+            for (int r = from; r < to; r += 32 * SCAN) {
+                float w[SCAN];
+#pragma unroll
+                for (int q = 0; q < SCAN; ++q) w[q] = r + q * 32 + lane < to ? a.mask[r + q * 32 + lane] : 0.f;
+#pragma unroll
+                for (int q = 0; q < SCAN; ++q) {
+                    const unsigned all = __ballot_sync(0xffffffffu, w[q] != 0.f);
+                    const int at = rank + __popc(all & ((1u << lane) - 1));
+                    if (w[q] != 0.f && at >= first && at < end) {
+                        const int row = r + q * 32 + lane, i = row / a.s, j = row - i * a.s;
+                        sm.list[at - first] = Kept{(k ? a.y : a.x).template at<T>(i, j), FULL ? a.y.template at<T>(i, j) : nullptr, row, k};
+                    }
+                    rank += __popc(all);
+                }
+            }
+        }
+        if (threadIdx.x == 0) sm.next = lo + WARPS;
+        __syncthreads();
+        W ahead, now;                                           // the walk of the copies and that of the sums
+        ahead.item = now.item = lo + warp;
+        unsigned taken = 0, begun = 0;
+        Running<T, FULL> run;
+        run.clear();
+        if (now.item < hi) {
+            ahead.enter(a, sm.list, first, chunks, chunk);
+            now.enter(a, sm.list, first, chunks, chunk);
+        }
+        int slot = 0;
+        auto request = [&](int at) {
+            if (ahead.item < hi) {
+                ahead.request(sm.ring[at][warp], lane);
+                if (!ahead.ends()) {
+                    ahead.done += W::STEP;
+                } else {                                        // the next chunk of the block, whoever comes first
+                    int item = 0;
+                    if (lane == 0) sm.queue[warp][taken & 3] = item = atomicAdd(&sm.next, 1);
+                    ahead.item = __shfl_sync(0xffffffffu, item, 0);
+                    ++taken;
+                    if (ahead.item < hi) ahead.enter(a, sm.list, first, chunks, chunk);
+                }
+            }
+            copies_sent();
+        };
+#pragma unroll
+        for (int d = 0; d < STAGES - 1; ++d) request(d);
+        while (now.item < hi) {
+            request(slot == 0 ? STAGES - 1 : slot - 1);         // the slot that was read last
+            if (now.done == 0) {                                // head and tail of the chunk: at most one element a lane
+                const int tail = now.count - now.head - now.vectors * N;
+                if (FULL && now.apart) {
+                    for (int c = lane; c < now.count; c += 32) run.add_one(Elem<T>::get(now.x[c]), Elem<T>::get(now.y[c]));
+                } else if (now.head + tail > 0) {
+                    int at = -1;
+                    if (lane < now.head) at = lane;
+                    else if (lane >= N && lane - N < tail) at = now.head + now.vectors * N + lane - N;
+                    if (at >= 0) run.add_one(Elem<T>::get(now.x[at]), FULL ? Elem<T>::get(now.y[at]) : 0.f);
+                }
+            }
+            copies_here<STAGES - 1>();
+            const int left = now.vectors - now.done - lane;
+            const uint4(*from_ring)[32] = sm.ring[slot][warp];
+            uint4 xr[U], yr[FULL ? U : 1];
+            if (now.vectors - now.done >= W::STEP) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    xr[u] = from_ring[u][lane];
+                    if constexpr (FULL) yr[u] = from_ring[U + u][lane];
+                }
+                run.add_vectors(xr, yr, left, true);
+            } else if (left > 0) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (u * 32 < left) {
+                        xr[u] = from_ring[u][lane];
+                        if constexpr (FULL) yr[u] = from_ring[U + u][lane];
+                    }
+                run.add_vectors(xr, yr, left, false);
+            }
+            slot = slot == STAGES - 1 ? 0 : slot + 1;
+            if (!now.ends()) {
+                now.done += W::STEP;
+                continue;
+            }
+            const int row = sm.list[now.entry].row, stream = sm.list[now.entry].stream;
+            const long long cells = (long long)a.rows * a.most, at = (long long)row * a.most + now.part;
+            Sums p{run.m, parts(run.t).x + parts(run.t).y};
+            const float own = p.m;
+            p.join_warp();
+            if (lane == 0) a.part[stream * cells + at] = make_float2(p.m, p.t);
+            if constexpr (FULL) {
+                Sums q{run.n, parts(run.r).x + parts(run.r).y};
+                const float w = warp_sum((parts(run.w).x + parts(run.w).y) * __expf(own - p.m));
+                q.join_warp();
+                if (lane == 0) {
+                    a.part[cells + at] = make_float2(q.m, q.t);
+                    a.cross[at] = w;
+                }
+            }
+            if (now.part == 0 && lane == 0) {                   // x is the row's first element here
+                const long long label = a.labels[row] - a.v0;
+                a.target[(long long)stream * a.rows + row] = label >= 0 && label < a.vocab ? Elem<T>::get(now.x[label]) : 0.f;
+            }
+            run.clear();
+            __syncwarp();
+            now.item = sm.queue[warp][begun++ & 3];
+            if (now.item < hi) now.enter(a, sm.list, first, chunks, chunk);
+        }
+        copies_here<0>();
     }
-    if (lane == 0) {
-        out[0] = p.m;
-        out[cells] = p.t;
-        out[2 * cells] = q.m;
-        out[3 * cells] = q.t;
-        out[4 * cells] = w;
-    }
+    if (a.rows == 0 && blockIdx.x == 0 && threadIdx.x == 0) a.ticket[0] = a.ticket[1] = 0;
+    __syncthreads();
+    launch::let_successor_start();
 }
 
 // ---------------------------------------------------------------------------------------------- from rows to the loss
+constexpr int LANES = 8;                                        // lanes that join a row's chunks
+constexpr int ROWS = THREADS / LANES;                           // rows of a block
+
 struct RowSums {
-    const float* part;
+    const float2* part;
+    const float* cross;
     const float* target;
     const long long* labels;
+    const int* ticket;             // [1]: chunks of a row, where `chunks` does not say
     long long vocab;               // of all ranks: a label outside makes its row NaN
-    int rows, splits;
+    int rows, most, chunks;
 };
 
-// Joins a row's chunks: maximum and sum, in 64 bits.
-__device__ __forceinline__ void join(const RowSums& r, int plane, int row, float& m, double& t) {
-    const long long cells = (long long)r.rows * r.splits;
-    const float* pm = r.part + plane * cells + (long long)row * r.splits;
-    const float* pt = pm + cells;
-    m = pm[0];
-    for (int k = 1; k < r.splits; ++k) m = fmaxf(m, pm[k]);
+template <typename V> __device__ __forceinline__ V lanes_sum(V v) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// Joins a row's chunks: maximum and sum, in 64 bits.  All lanes of a warp come here, each with its row.
+__device__ __forceinline__ void join(const RowSums& r, int chunks, int stream, int row, bool on, float& m, double& t) {
+    const int lane = threadIdx.x % LANES;
+    const float2* p = r.part + ((long long)stream * r.rows + row) * r.most;
+    m = -FLT_MAX;
+    if (on)
+        for (int k = lane; k < chunks; k += LANES) m = fmaxf(m, p[k].x);
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     t = 0.0;
-    for (int k = 0; k < r.splits; ++k) t += (double)pt[k] * (double)__expf(pm[k] - m);
+    if (on)
+        for (int k = lane; k < chunks; k += LANES) t += (double)p[k].y * (double)__expf(p[k].x - m);
+    t = lanes_sum(t);
 }
 __device__ __forceinline__ double label_logp(const RowSums& r, int which, int row, float m, double t) {
     const long long y = r.labels[row];
@@ -407,30 +638,27 @@ struct PreferenceArgs {
     float* coef;                   // [n]: d loss / d logp
 };
 
-// Each block joins THREADS rows of one sequence and leaves their sums; the last block adds those up in order, a warp a
+// Each block joins ROWS rows of one sequence and leaves their sums; the last block adds those up in order, a warp a
 // sequence, and forms, pair by pair,  z = beta ((P_c - P_r) - (R_c - R_r)),
 // loss = -(1 - e) log sigma(z) - e log sigma(-z),  d loss / d P_c = -beta ((1 - e) sigma(-z) - e sigma(z)) / pairs = -d/d P_r.
 __global__ void __launch_bounds__(THREADS) preference_kernel(const PreferenceArgs a) {
-    const int seq = blockIdx.x / a.pieces, j = (blockIdx.x % a.pieces) * THREADS + threadIdx.x;
+    const int seq = blockIdx.x / a.pieces, j = (blockIdx.x % a.pieces) * ROWS + threadIdx.x / LANES;
+    const int row = seq * a.s + j;
+    const float w = j < a.s ? a.mask[row] : 0.f;
+    launch::wait_for_predecessor();
+    const int chunks = a.sums.chunks ? a.sums.chunks : a.sums.ticket[1];
     double v[2] = {0.0, 0.0};
-    if (j < a.s) {
-        const int row = seq * a.s + j;
-        const float w = a.mask[row];
-        float2 keep = make_float2(0.f, 0.f);
+    float m, mr = 0.f;
+    double t, tr = 0.0;
+    join(a.sums, chunks, 0, row, w != 0.f, m, t);
+    if (a.has_ref_logits) join(a.sums, chunks, 1, row, w != 0.f, mr, tr);
+    if (j < a.s && threadIdx.x % LANES == 0) {
+        a.row[row] = w != 0.f ? make_float2(m, (float)(1.0 / t)) : make_float2(0.f, 0.f);
         if (w != 0.f) {
-            float m;
-            double t;
-            join(a.sums, 0, row, m, t);
-            keep = make_float2(m, (float)(1.0 / t));
             v[0] = w * label_logp(a.sums, 0, row, m, t);
-            if (a.has_ref_logits) {
-                join(a.sums, 2, row, m, t);
-                v[1] = w * label_logp(a.sums, 1, row, m, t);
-            } else if (a.ref_logp) {
-                v[1] = (double)w * a.ref_logp[row];
-            }
+            if (a.has_ref_logits) v[1] = w * label_logp(a.sums, 1, row, mr, tr);
+            else if (a.ref_logp) v[1] = (double)w * a.ref_logp[row];
         }
-        a.row[row] = keep;
     }
     block_sum(v);
     if (threadIdx.x == 0) {
@@ -500,17 +728,27 @@ struct PolicyArgs {
 // Row by row: r = exp(l - old), term = -min(r A, clip(r) A) + kl_beta KL and its slope in l; sums of mask, mask * term,
 // mask * KL and mask * [clipped] by sequence, then the means.
 __global__ void __launch_bounds__(THREADS) policy_kernel(const PolicyArgs a) {
-    const int seq = blockIdx.x / a.pieces, j = (blockIdx.x % a.pieces) * THREADS + threadIdx.x;
+    const int seq = blockIdx.x / a.pieces, j = (blockIdx.x % a.pieces) * ROWS + threadIdx.x / LANES;
+    const int row = seq * a.s + j;
+    const float w = j < a.s ? a.mask[row] : 0.f;
+    launch::wait_for_predecessor();
+    const int chunks = a.sums.chunks ? a.sums.chunks : a.sums.ticket[1];
     double v[4] = {0.0, 0.0, 0.0, 0.0};
-    if (j < a.s) {
-        const int row = seq * a.s + j;
-        const float w = a.mask[row];
+    float m, mq = 0.f;
+    double t, tq = 0.0, cross = 0.0;
+    join(a.sums, chunks, 0, row, w != 0.f, m, t);
+    if (a.has_ref_logits) join(a.sums, chunks, 1, row, w != 0.f, mq, tq);
+    if (a.kl == KL_FULL) {
+        const long long at = (long long)row * a.sums.most;
+        if (w != 0.f)
+            for (int k = threadIdx.x % LANES; k < chunks; k += LANES)
+                cross += (double)a.sums.cross[at + k] * (double)__expf(a.sums.part[at + k].x - m);
+        cross = lanes_sum(cross);
+    }
+    if (j < a.s && threadIdx.x % LANES == 0) {
         float2 keep = make_float2(0.f, 0.f);
         float slope = 0.f, shift = 0.f, logp = 0.f;
         if (w != 0.f) {
-            float m;
-            double t;
-            join(a.sums, 0, row, m, t);
             keep = make_float2(m, (float)(1.0 / t));
             const double l = label_logp(a.sums, 0, row, m, t);
             logp = (float)l;
@@ -521,26 +759,13 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(const PolicyArgs a) {
             const bool clipped = free > held;
             double term = clipped ? -held : -free, d = clipped ? 0.0 : -free, kl = 0.0;
             if (a.kl == KL_FULL) {
-                const long long cells = (long long)a.sums.rows * a.sums.splits, at = (long long)row * a.sums.splits;
-                double w_sum = 0.0;
-                for (int k = 0; k < a.sums.splits; ++k)
-                    w_sum += (double)a.sums.part[4 * cells + at + k] * (double)__expf(a.sums.part[at + k] - m);
-                float mq;
-                double tq;
-                join(a.sums, 2, row, mq, tq);
                 const double gap = ((double)m - (double)mq) + (log(t) - log(tq));
-                kl = w_sum / t - gap;
+                kl = cross / t - gap;
                 shift = (float)(gap + kl);
             } else if (a.kl != KL_NONE) {
                 double ref;
-                if (a.has_ref_logits) {
-                    float mq;
-                    double tq;
-                    join(a.sums, 2, row, mq, tq);
-                    ref = label_logp(a.sums, 1, row, mq, tq);
-                } else {
-                    ref = a.ref_logp[row];
-                }
+                if (a.has_ref_logits) ref = label_logp(a.sums, 1, row, mq, tq);
+                else ref = a.ref_logp[row];
                 const double x = l - ref;
                 double more;
                 if (a.kl == KL_PLAIN) {
@@ -717,19 +942,35 @@ __global__ void __launch_bounds__(THREADS) grad_kernel(const GradArgs a) {
     }
 }
 
-// Chunks of a row: what G threads with U loads each hold.  The chunks of a row are of one size, up to rounding to 8 elements.
-struct Plan {
-    bool warp;                     // a warp a row, else a block a chunk
-    int splits, chunk;
+// How the gradient cuts a row: G threads with U loads each, for narrow vocabularies fewer of them, so that all have something to do.
+struct GradPlan {
+    int threads, splits, chunk;
+    GradPlan(int vocab, int dtype, int u) {
+        const int n = dtype == 1 ? 4 : 8;
+        threads = 32;
+        while (threads < THREADS && threads * u * n < vocab) threads *= 2;
+        const int most = threads * u * n;
+        splits = (vocab + most - 1) / most;
+        chunk = splits == 1 ? vocab : ((vocab + splits - 1) / splits + 7) / 8 * 8;
+    }
     bool fits(long long rows, int vocab) const { return rows * splits < (1ll << 31) && (splits - 1ll) * chunk < vocab; }
 };
-Plan plan(int vocab, int dtype, int u) {
-    const int n = dtype == 1 ? 4 : 8;
-    if (vocab <= 32 * u * n) return {true, 1, vocab};
-    const int most = THREADS * u * n;
-    const int splits = (vocab + most - 1) / most;
-    return {false, splits, ((vocab + splits - 1) / splits + 7) / 8 * 8};
-}
+
+// Chunks of a row that there is room for: down to a vector a lane, 64 at most; and those for a batch that keeps all its rows, where
+// the kernel cannot count them.
+struct StatsPlan {
+    int chunks = 1, most;
+    StatsPlan(long long rows, int vocab, int dtype, int full) {
+        const int least = 32 * (dtype == 1 ? 4 : 8), warps = full ? Shape<true>::WARPS : Shape<false>::WARPS;
+        most = (vocab + least - 1) / least;
+        // a row of its own for every warp of the machine: no more than the chunks of a long row
+        const long long busy = (long long)warps * neox_sm_count(), usual = (vocab + 4095) / 4096;
+        if (rows > 2 * busy && most > usual) most = (int)usual;
+        if (most > 64) most = 64;
+        for (int c = 1; c <= most; ++c)
+            if (cut_cost(rows, vocab, c, neox_sm_count(), warps) < cut_cost(rows, vocab, chunks, neox_sm_count(), warps)) chunks = c;
+    }
+};
 
 #define FOR_TYPE(dtype, CALL)                                  \
     do {                                                       \
@@ -737,6 +978,18 @@ Plan plan(int vocab, int dtype, int u) {
         else if (dtype == 1) { using T = float; CALL; }        \
         else { using T = __half; CALL; }                       \
     } while (0)
+
+#define FOR_THREADS(threads, CALL)                                 \
+    do {                                                           \
+        if (threads == 32) { constexpr int G = 32; CALL; }         \
+        else if (threads == 64) { constexpr int G = 64; CALL; }    \
+        else if (threads == 128) { constexpr int G = 128; CALL; }  \
+        else { constexpr int G = 256; CALL; }                      \
+    } while (0)
+
+#define LAUNCH_STATS(T, FULL)                                                                             \
+    if (!allow_dynamic_smem<stats_kernel<T, FULL>>(sizeof(StatsSmem<FULL>))) return NEOX_ERR_LAUNCH;      \
+    stats_kernel<T, FULL><<<blocks, Shape<FULL>::WARPS * 32, sizeof(StatsSmem<FULL>), st>>>(a)
 
 constexpr int U_ONE = 8, U_FULL = 4;
 
@@ -746,46 +999,44 @@ int launched() { return cudaGetLastError() == cudaSuccess ? 0 : NEOX_ERR_LAUNCH;
 
 extern "C" {
 
-// Chunks a row is read in: the planes that neox_vocab_stats writes are [n * s, this].
-int neox_vocab_splits(int vocab, int dtype, int full) { return plan(vocab, dtype, full ? U_FULL : U_ONE).splits; }
+// Chunks of a row that neox_vocab_stats has room for: `part` is [streams][n * s, this] pairs, `cross` [n * s, this].
+int neox_vocab_splits(long long rows, int vocab, int dtype, int full) {
+    const StatsPlan p(rows, vocab, dtype, full);
+    return p.most;
+}
 
 int neox_vocab_stats(const void* x, long long xn, long long xs, const void* y, long long yn, long long ys,
                      const long long* labels, const float* mask, int n, int s, int vocab, long long v0, int dtype, int full,
-                     float* part, float* target, int* ticket, void* stream) {
+                     void* part, float* cross, float* target, int* ticket, void* stream) {
     if (n < 0 || s < 0 || vocab < 1 || (full && !y)) return NEOX_ERR_SHAPE;
-    const Plan p = plan(vocab, dtype, full ? U_FULL : U_ONE);
     const long long rows = (long long)n * s;
-    if (!p.fits(rows, vocab)) return NEOX_ERR_TOO_LARGE;
-    StatsArgs a = {{x, xn, xs}, {y, yn, ys}, labels, mask, part, target, ticket, v0, (int)rows, s, vocab, p.splits, p.chunk};
-    const long long per = p.warp ? THREADS / 32 : 1;
-    const dim3 grid((unsigned)((rows * p.splits + per) / per), !full && y ? 2 : 1);        // one block at least: it sets the ticket
+    const StatsPlan p(rows, vocab, dtype, full);
+    const int streams = !full && y ? 2 : 1;
+    if (rows * streams * p.most >= (1ll << 31)) return NEOX_ERR_TOO_LARGE;
+    const StatsArgs a = {{x, xn, xs}, {y, yn, ys}, labels, mask, (float2*)part, cross, target, ticket, v0, (int)rows, s, vocab,
+                         streams, p.chunks, p.most};
+    const int blocks = neox_sm_count();
     cudaStream_t st = (cudaStream_t)stream;
-    if (full) {
-        if (p.warp) FOR_TYPE(dtype, (stats_full_kernel<T, 32, U_FULL><<<grid, THREADS, 0, st>>>(a)));
-        else FOR_TYPE(dtype, (stats_full_kernel<T, THREADS, U_FULL><<<grid, THREADS, 0, st>>>(a)));
-    } else {
-        if (p.warp) FOR_TYPE(dtype, (stats_kernel<T, 32, U_ONE><<<grid, THREADS, 0, st>>>(a)));
-        else FOR_TYPE(dtype, (stats_kernel<T, THREADS, U_ONE><<<grid, THREADS, 0, st>>>(a)));
-    }
+    if (full) FOR_TYPE(dtype, LAUNCH_STATS(T, true));
+    else FOR_TYPE(dtype, LAUNCH_STATS(T, false));
     return launched();
 }
 
 // Blocks that join a sequence's rows; `partial` of the two calls below holds (n * this + n) * 2 or * 4 doubles.
-int neox_loss_pieces(int s) { return s > 0 ? (s + THREADS - 1) / THREADS : 1; }
+int neox_loss_pieces(int s) { return s > 0 ? (s + ROWS - 1) / ROWS : 1; }
 
-int neox_preference_loss(const float* part, const float* target, int splits, const long long* labels, const float* mask,
+int neox_preference_loss(const void* part, const float* target, int most, int chunks, const long long* labels, const float* mask,
                          const float* ref_logp, int has_ref_logits, int n, int s, long long vocab, double beta, double smoothing,
                          void* row, double* partial, int* ticket, float* loss, float* logp, float* ref, float* coef, void* stream) {
     if (n < 2 || n % 2 || s < 0) return NEOX_ERR_SHAPE;
     const int pieces = neox_loss_pieces(s);
     if ((long long)n * pieces >= (1ll << 31)) return NEOX_ERR_TOO_LARGE;
-    const PreferenceArgs a = {{part, target, labels, vocab, n * s, splits}, mask, ref_logp, has_ref_logits, n, s, pieces, beta,
+    const PreferenceArgs a = {{(const float2*)part, nullptr, target, labels, ticket, vocab, n * s, most, chunks}, mask, ref_logp, has_ref_logits, n, s, pieces, beta,
                               smoothing, (float2*)row, partial, ticket, loss, logp, ref, coef};
-    preference_kernel<<<n * pieces, THREADS, 0, (cudaStream_t)stream>>>(a);
-    return launched();
+    return launch::overlapped(preference_kernel, dim3(n * pieces), dim3(THREADS), 1, (cudaStream_t)stream, a);
 }
 
-int neox_policy_loss(const float* part, const float* target, int splits, const long long* labels, const float* mask,
+int neox_policy_loss(const void* part, const float* cross, const float* target, int most, int chunks, const long long* labels, const float* mask,
                      const float* advantages, long long adv_n, long long adv_s, const float* old_logp, const float* ref_logp,
                      int has_ref_logits, int n, int s, long long vocab, int kl, int by_sequence, double low, double high,
                      double kl_beta, void* row, float* slope, float* shift, double* partial, int* ticket, float* out, float* logp,
@@ -793,11 +1044,10 @@ int neox_policy_loss(const float* part, const float* target, int splits, const l
     if (n < 1 || s < 0) return NEOX_ERR_SHAPE;
     const int pieces = neox_loss_pieces(s);
     if ((long long)n * pieces >= (1ll << 31)) return NEOX_ERR_TOO_LARGE;
-    const PolicyArgs a = {{part, target, labels, vocab, n * s, splits}, mask, advantages, adv_n, adv_s, old_logp, ref_logp,
+    const PolicyArgs a = {{(const float2*)part, cross, target, labels, ticket, vocab, n * s, most, chunks}, mask, advantages, adv_n, adv_s, old_logp, ref_logp,
                           has_ref_logits, n, s, pieces, kl, by_sequence, low, high, kl_beta, (float2*)row, slope, shift, partial,
                           ticket, out, logp, coef};
-    policy_kernel<<<n * pieces, THREADS, 0, (cudaStream_t)stream>>>(a);
-    return launched();
+    return launch::overlapped(policy_kernel, dim3(n * pieces), dim3(THREADS), 1, (cudaStream_t)stream, a);
 }
 
 int neox_vocab_grad(const void* x, long long xn, long long xs, const void* y, long long yn, long long ys, void* g, long long gn,
@@ -806,22 +1056,17 @@ int neox_vocab_grad(const void* x, long long xn, long long xs, const void* y, lo
                     int vocab, long long v0, int dtype, void* stream) {
     if (n < 0 || s < 0 || vocab < 1) return NEOX_ERR_SHAPE;
     const int full = shift != nullptr;
-    const Plan p = plan(vocab, dtype, full ? U_FULL : U_ONE);
+    const GradPlan p(vocab, dtype, full ? U_FULL : U_ONE);
     const long long rows = (long long)n * s;
     if (rows == 0) return 0;
     if (!p.fits(rows, vocab)) return NEOX_ERR_TOO_LARGE;
     const GradArgs a = {{x, xn, xs}, {y, yn, ys}, g, gn, gs, labels, slope, mask, shift, (const float2*)row, coef, g_loss, g_logp,
                         v0, kl_beta, (int)rows, s, vocab, p.splits, p.chunk};
-    const long long per = p.warp ? THREADS / 32 : 1;
+    const long long per = THREADS / p.threads;
     const unsigned grid = (unsigned)((rows * p.splits + per - 1) / per);
     cudaStream_t st = (cudaStream_t)stream;
-    if (full) {
-        if (p.warp) FOR_TYPE(dtype, (grad_kernel<T, 32, U_FULL, true><<<grid, THREADS, 0, st>>>(a)));
-        else FOR_TYPE(dtype, (grad_kernel<T, THREADS, U_FULL, true><<<grid, THREADS, 0, st>>>(a)));
-    } else {
-        if (p.warp) FOR_TYPE(dtype, (grad_kernel<T, 32, U_ONE, false><<<grid, THREADS, 0, st>>>(a)));
-        else FOR_TYPE(dtype, (grad_kernel<T, THREADS, U_ONE, false><<<grid, THREADS, 0, st>>>(a)));
-    }
+    if (full) FOR_TYPE(dtype, FOR_THREADS(p.threads, (grad_kernel<T, G, U_FULL, true><<<grid, THREADS, 0, st>>>(a))));
+    else FOR_TYPE(dtype, FOR_THREADS(p.threads, (grad_kernel<T, G, U_ONE, false><<<grid, THREADS, 0, st>>>(a))));
     return launched();
 }
 

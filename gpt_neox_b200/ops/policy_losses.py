@@ -25,11 +25,11 @@ KL_KINDS = {"kl": 1, "abs": 2, "mse": 3, "k3": 4, "full": 5}
 
 _P, _I, _L, _D, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_double, ctypes.c_float
 native._ARGTYPES.update({
-    "neox_vocab_splits": [_I, _I, _I],
+    "neox_vocab_splits": [_L, _I, _I, _I],
     "neox_loss_pieces": [_I],
-    "neox_vocab_stats": [_P, _L, _L, _P, _L, _L, _P, _P, _I, _I, _I, _L, _I, _I, _P, _P, _P, _P],
-    "neox_preference_loss": [_P, _P, _I, _P, _P, _P, _I, _I, _I, _L, _D, _D, _P, _P, _P, _P, _P, _P, _P, _P],
-    "neox_policy_loss": [_P, _P, _I, _P, _P, _P, _L, _L, _P, _P, _I, _I, _I, _L, _I, _I, _D, _D, _D, _P, _P, _P, _P, _P, _P, _P,
+    "neox_vocab_stats": [_P, _L, _L, _P, _L, _L, _P, _P, _I, _I, _I, _L, _I, _I, _P, _P, _P, _P, _P],
+    "neox_preference_loss": [_P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _L, _D, _D, _P, _P, _P, _P, _P, _P, _P, _P],
+    "neox_policy_loss": [_P, _P, _P, _I, _I, _P, _P, _P, _L, _L, _P, _P, _I, _I, _I, _L, _I, _I, _D, _D, _D, _P, _P, _P, _P, _P, _P, _P,
                          _P, _P],
     "neox_vocab_grad": [_P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P, _F, _I, _I, _I, _L, _I, _P],
 })
@@ -95,82 +95,102 @@ def _rows(t):
     return t if t is None or t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
 
 
-def _addr(t):
-    return None if t is None else t.data_ptr()
-
-
 def _tensor_parallel():
     from ..parallel import mpu
     return mpu.get_model_parallel_world_size(), mpu.get_model_parallel_rank(), mpu.get_model_parallel_group
 
 
 # ---------------------------------------------------------------------------------------------- kernels
-class _Stats(NamedTuple):
-    part: torch.Tensor       # [planes, rows, splits]
-    target: torch.Tensor     # [1 or 2, rows]
-    ticket: torch.Tensor
-    splits: int
-    first: int               # first word of this rank's share of the vocabulary
-    vocab: int               # words of all ranks
+class _Stats:
+    """One pass over the kept rows of policy (and reference) logits, and the scratch memory of a forward, in one piece::
 
+        sums    [n * (pieces + 1), width] fp64    what the joining kernel's blocks leave
+        part    [streams, rows, most, 2]          maximum and sum of every chunk of a row, policy and reference
+        cross   [rows, most]                      sum of p (x - y), for the KL over the vocabulary
+        target  [streams, rows]                   the labels' logits
+        ticket  [2] int32
 
-def _row_stats(x, y, labels, mask, full):
-    """One pass over the kept rows of policy (and reference) logits.  With the vocabulary split over ranks the chunks are joined
-    here and two all-reduces -- maxima, then sums and label logits -- make the statistics those of whole rows."""
-    n, s, v = x.shape
-    rows = n * s
-    tp, rank, group = _tensor_parallel()
-    L, dt = native.lib(), _DT[x.dtype]
-    splits = L.neox_vocab_splits(v, dt, int(full))
-    planes = 5 if full else 2 if y is None else 4
-    part = torch.empty(planes, rows, splits, dtype=torch.float32, device=x.device)
-    target = torch.empty(1 if full or y is None else 2, rows, dtype=torch.float32, device=x.device)
-    ticket = torch.empty(1, dtype=torch.int32, device=x.device)
-    rc = L.neox_vocab_stats(_addr(x), x.stride(0), x.stride(1), _addr(y), 0 if y is None else y.stride(0),
-                            0 if y is None else y.stride(1), _addr(labels), _addr(mask), n, s, v, rank * v, dt, int(full),
-                            _addr(part), _addr(target), _addr(ticket), native.stream_ptr())
-    native.check(rc, "neox_vocab_stats")
-    if tp > 1:
+    With the vocabulary split over ranks the chunks are joined here and two all-reduces -- maxima, then sums and label logits --
+    make the statistics those of whole rows.  What stands in rows of mask zero is never read."""
+
+    def __init__(self, x, y, labels, mask, full, width):
+        n, s, v = x.shape
+        rows = n * s
+        streams = 1 if y is None else 2
+        tp, rank, group = _tensor_parallel()
+        L, dt = native.lib(), _DT[x.dtype]
+        most = L.neox_vocab_splits(rows, v, dt, full)
+        sums = 2 * width * n * (L.neox_loss_pieces(s) + 1)
+        parts = streams * rows * most * 2
+        crosses = rows * most if full else 0
+        self.buf = buf = torch.empty(sums + parts + crosses + streams * rows + 2, dtype=torch.float32, device=x.device)
+        self.sums = buf.data_ptr()
+        self.part = self.sums + 4 * sums
+        self.cross = self.part + 4 * parts
+        self.target = self.cross + 4 * crosses
+        self.ticket = self.target + 4 * streams * rows
+        self.most, self.chunks, self.first, self.vocab = most, 0, rank * v, tp * v
+        y_ = x if y is None else y
+        rc = L.neox_vocab_stats(x.data_ptr(), x.stride(0), x.stride(1), None if y is None else y.data_ptr(), y_.stride(0),
+                                y_.stride(1), labels.data_ptr(), mask.data_ptr(), n, s, v, self.first, dt, full, self.part,
+                                self.cross, self.target, self.ticket, native.stream_ptr())
+        native.check(rc, "neox_vocab_stats")
+        if tp > 1:
+            self._reduce(sums, parts, crosses, streams, rows, group())
+
+    def _reduce(self, sums, parts, crosses, streams, rows, group):
         import torch.distributed as dist
-        top = part[0:4:2].amax(-1)
-        dist.all_reduce(top, op=dist.ReduceOp.MAX, group=group())
-        sums = (part[1:4:2] * (part[0:4:2] - top[..., None]).exp()).sum(-1)
-        if full:
-            sums = torch.cat([sums, (part[4] * (part[0] - top[0, :, None]).exp()).sum(-1)[None]])
-        both = torch.cat([sums, target])
-        dist.all_reduce(both, group=group())
-        joined = [t for k in range(top.shape[0]) for t in (top[k], both[k])] + ([both[2]] if full else [])
-        part, target, splits = torch.stack(joined), both[sums.shape[0]:].contiguous(), 1
-    return _Stats(part, target, ticket, splits, rank * v, tp * v)
+        _, part, cross, target, ticket = self.buf.split([sums, parts, crosses, streams * rows, 2])
+        part, target = part.view(streams, rows, self.most, 2), target.view(streams, rows)
+        there = torch.arange(self.most, device=part.device) < ticket.view(torch.int32)[1]
+        local = torch.where(there, part[..., 0], torch.finfo(torch.float32).min)
+        top = local.amax(-1)
+        dist.all_reduce(top, op=dist.ReduceOp.MAX, group=group)
+        scale = (local - top[..., None]).exp()
+        terms = [torch.where(there, part[..., 1] * scale, 0.0).sum(-1), target]
+        if crosses:
+            terms.append(torch.where(there, cross.view(rows, self.most) * scale[0], 0.0).sum(-1)[None])
+        both = torch.cat(terms)
+        dist.all_reduce(both, group=group)
+        joined = torch.stack([top, both[:streams]], -1)
+        self.keep = (joined, both)
+        self.part, self.target = joined.data_ptr(), both[streams].data_ptr()
+        self.cross = both[-1].data_ptr() if crosses else 0
+        self.most = self.chunks = 1
 
 
 def _logits_grad(x, y, labels, slope, mask, shift, row, coef, g_loss, g_logp, kl_beta, first):
-    """Gradient of the logits in their own memory order where that is dense."""
+    """Gradient of the logits in their own memory order where that is dense.  ``slope`` to ``coef`` are addresses."""
     n, s, v = x.shape
     g = torch.empty_like(x)
     if g.stride(2) != 1:
         g = torch.empty(n, s, v, dtype=x.dtype, device=x.device)
+    y_ = x if y is None else y
     rc = native.lib().neox_vocab_grad(
-        _addr(x), x.stride(0), x.stride(1), _addr(y), 0 if y is None else y.stride(0), 0 if y is None else y.stride(1), _addr(g),
-        g.stride(0), g.stride(1), _addr(labels), _addr(slope), _addr(mask), _addr(shift), _addr(row), _addr(coef),
-        _addr(g_loss), _addr(g_logp), kl_beta, n, s, v, first, _DT[x.dtype], native.stream_ptr())
+        x.data_ptr(), x.stride(0), x.stride(1), y_.data_ptr(), y_.stride(0), y_.stride(1), g.data_ptr(), g.stride(0), g.stride(1),
+        labels.data_ptr(), slope, mask.data_ptr(), shift, row, coef, None if g_loss is None else g_loss.data_ptr(),
+        None if g_logp is None else g_logp.data_ptr(), kl_beta, n, s, v, first, _DT[x.dtype], native.stream_ptr())
     native.check(rc, "neox_vocab_grad")
     return g
 
 
 def _preference_values(x, labels, mask, ref_logits, ref_logp, beta, smoothing):
+    """Loss, log-probabilities, what the backward needs (``[rows, 2]`` maximum and 1 / sum, then ``[n]`` coefficients), and the
+    first word of this rank's vocabulary."""
     n, s, _ = x.shape
-    st = _row_stats(x, ref_logits, labels, mask, False)
-    L, dev = native.lib(), x.device
-    row = torch.empty(n * s, 2, dtype=torch.float32, device=dev)
-    sums = torch.empty(2 * n * (L.neox_loss_pieces(s) + 1), dtype=torch.float64, device=dev)
+    st = _Stats(x, ref_logits, labels, mask, 0, 2)
+    dev = x.device
+    kept = torch.empty(2 * n * s + n, dtype=torch.float32, device=dev)
     loss = torch.empty((), dtype=torch.float32, device=dev)
-    logp, ref, coef = (torch.empty(n, dtype=torch.float32, device=dev) for _ in range(3))
-    rc = L.neox_preference_loss(_addr(st.part), _addr(st.target), st.splits, _addr(labels), _addr(mask), _addr(ref_logp),
-                                int(ref_logits is not None), n, s, st.vocab, beta, smoothing, _addr(row), _addr(sums),
-                                _addr(st.ticket), _addr(loss), _addr(logp), _addr(ref), _addr(coef), native.stream_ptr())
+    logp = torch.empty(n, dtype=torch.float32, device=dev)
+    ref = torch.empty(n, dtype=torch.float32, device=dev)
+    row = kept.data_ptr()
+    rc = native.lib().neox_preference_loss(
+        st.part, st.target, st.most, st.chunks, labels.data_ptr(), mask.data_ptr(), None if ref_logp is None else ref_logp.data_ptr(),
+        ref_logits is not None, n, s, st.vocab, beta, smoothing, row, st.sums, st.ticket, loss.data_ptr(), logp.data_ptr(),
+        ref.data_ptr(), row + 8 * n * s, native.stream_ptr())
     native.check(rc, "neox_preference_loss")
-    return loss, logp, ref, row, coef, st.first
+    return loss, logp, ref, kept, st.first
 
 
 def _grad_f32(g):
@@ -181,62 +201,69 @@ class _PreferenceFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, labels, mask, ref_logits, ref_logp, beta, smoothing):
         with device_of(x):
-            loss, logp, ref, row, coef, first = _preference_values(x, labels, mask, ref_logits, ref_logp, beta, smoothing)
-        ctx.save_for_backward(x, labels, mask, row, coef)
-        ctx.first = first
+            loss, logp, ref, kept, ctx.first = _preference_values(x, labels, mask, ref_logits, ref_logp, beta, smoothing)
+        ctx.save_for_backward(x, labels, mask, kept)
         ctx.mark_non_differentiable(ref)
         ctx.set_materialize_grads(False)
         return loss, logp, ref
 
     @staticmethod
     def backward(ctx, g_loss, g_logp, _):
-        x, labels, mask, row, coef = ctx.saved_tensors
+        x, labels, mask, kept = ctx.saved_tensors
         if g_loss is None and g_logp is None:
             return (None,) * 7
+        row = kept.data_ptr()
         with device_of(x):
-            g = _logits_grad(x, None, labels, mask, mask, None, row, coef, _grad_f32(g_loss), _grad_f32(g_logp), 0.0, ctx.first)
+            g = _logits_grad(x, None, labels, mask.data_ptr(), mask, None, row, row + 8 * mask.numel(), _grad_f32(g_loss),
+                             _grad_f32(g_logp), 0.0, ctx.first)
         return (once(g, x),) + (None,) * 6
 
 
 def _policy_values(x, labels, mask, adv, old_logp, ref_logits, ref_logp, low, high, kl, kl_beta, by_sequence):
+    """Loss, means, log-probabilities, what the backward needs (``[rows, 2]`` maximum and 1 / sum, ``[n]`` coefficients, ``[rows]``
+    slopes and, for the KL over the vocabulary, ``[rows]`` shifts), and the first word of this rank's vocabulary."""
     n, s, _ = x.shape
-    full = kl == KL_KINDS["full"]
-    st = _row_stats(x, ref_logits, labels, mask, full)
-    L, dev = native.lib(), x.device
-    row = torch.empty(n * s, 2, dtype=torch.float32, device=dev)
-    slope = torch.empty(n * s, dtype=torch.float32, device=dev)
-    shift = torch.empty(n * s, dtype=torch.float32, device=dev) if full else None
-    sums = torch.empty(4 * n * (L.neox_loss_pieces(s) + 1), dtype=torch.float64, device=dev)
+    rows, full = n * s, kl == KL_KINDS["full"]
+    st = _Stats(x, ref_logits, labels, mask, int(full), 4)
+    dev = x.device
+    kept = torch.empty((4 if full else 3) * rows + n, dtype=torch.float32, device=dev)
     out = torch.empty(3, dtype=torch.float32, device=dev)
     logp = torch.empty(n, s, dtype=torch.float32, device=dev)
-    coef = torch.empty(n, dtype=torch.float32, device=dev)
-    rc = L.neox_policy_loss(_addr(st.part), _addr(st.target), st.splits, _addr(labels), _addr(mask), _addr(adv), adv.stride(0),
-                            adv.stride(1), _addr(old_logp), _addr(ref_logp), int(ref_logits is not None), n, s, st.vocab, kl,
-                            int(by_sequence), low, high, kl_beta, _addr(row), _addr(slope), _addr(shift), _addr(sums),
-                            _addr(st.ticket), _addr(out), _addr(logp), _addr(coef), native.stream_ptr())
+    row = kept.data_ptr()
+    coef = row + 8 * rows
+    slope = coef + 4 * n
+    rc = native.lib().neox_policy_loss(
+        st.part, st.cross, st.target, st.most, st.chunks, labels.data_ptr(), mask.data_ptr(), adv.data_ptr(), adv.stride(0),
+        adv.stride(1), None if old_logp is None else old_logp.data_ptr(), None if ref_logp is None else ref_logp.data_ptr(),
+        ref_logits is not None, n, s, st.vocab, kl, by_sequence, low, high, kl_beta, row, slope, slope + 4 * rows if full else None,
+        st.sums, st.ticket, out.data_ptr(), logp.data_ptr(), coef, native.stream_ptr())
     native.check(rc, "neox_policy_loss")
-    return (*out.unbind(0), logp, row, slope, shift, coef, st.first)
+    return (*out.unbind(0), logp, kept, st.first)
 
 
 class _PolicyFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, labels, mask, adv, old_logp, ref_logits, ref_logp, low, high, kl, kl_beta, by_sequence):
         with device_of(x):
-            loss, mean_kl, clipped, logp, row, slope, shift, coef, first = _policy_values(
-                x, labels, mask, adv, old_logp, ref_logits, ref_logp, low, high, kl, kl_beta, by_sequence)
-        ctx.save_for_backward(x, labels, mask, row, slope, coef, shift, ref_logits if shift is not None else None)
-        ctx.first, ctx.kl_beta = first, kl_beta
+            loss, mean_kl, clipped, logp, kept, ctx.first = _policy_values(x, labels, mask, adv, old_logp, ref_logits, ref_logp, low,
+                                                                           high, kl, kl_beta, by_sequence)
+        ctx.full, ctx.kl_beta = kl == KL_KINDS["full"], kl_beta
+        ctx.save_for_backward(x, labels, mask, kept, ref_logits if ctx.full else None)
         ctx.mark_non_differentiable(mean_kl, clipped, logp)
         ctx.set_materialize_grads(False)
         return loss, mean_kl, clipped, logp
 
     @staticmethod
     def backward(ctx, g_loss, *_):
-        x, labels, mask, row, slope, coef, shift, ref_logits = ctx.saved_tensors
+        x, labels, mask, kept, ref_logits = ctx.saved_tensors
         if g_loss is None:
             return (None,) * 12
+        rows, row = mask.numel(), kept.data_ptr()
+        coef = row + 8 * rows
+        slope = coef + 4 * mask.shape[0]
         with device_of(x):
-            g = _logits_grad(x, ref_logits, labels, slope, mask, shift, row, coef, _grad_f32(g_loss), None, ctx.kl_beta, ctx.first)
+            g = _logits_grad(x, ref_logits, labels, slope, mask, slope + 4 * rows if ctx.full else None, row, coef,
+                             _grad_f32(g_loss), None, ctx.kl_beta, ctx.first)
         return (once(g, x),) + (None,) * 11
 
 
