@@ -15,6 +15,7 @@
 #include <float.h>
 #include <stdint.h>
 
+#include "launch.cuh"
 #include "neox_b200.h"
 
 namespace {
@@ -236,6 +237,7 @@ __global__ void __launch_bounds__(THREADS) router_kernel(const ForwardArgs a) {
         for (int w = 0; w < WARPS; ++w) s += zs[w];
         a.z[blockIdx.x] = s;
     }
+    launch::let_successor_start();
 }
 
 struct LossArgs {
@@ -246,7 +248,8 @@ struct LossArgs {
     double* part;                  // [gridDim, 2]: sum of count * column sum, sum of counts
     long long* counts;
     float* load;                   // [E + 1]: choices of the kept tokens; then 1 / kept tokens
-    float* out;                    // balance, z
+    float* balance;
+    float* z_loss;
     int blocks, E, k;
 };
 
@@ -255,6 +258,7 @@ __global__ void __launch_bounds__(1024) router_loss_kernel(const LossArgs a) {
     __shared__ double p[32][33];
     __shared__ int n_all[32][33], n_kept[32][33];
     __shared__ int last;
+    launch::wait_for_predecessor();
     const int x = threadIdx.x & 31, y = threadIdx.x >> 5, e = blockIdx.x * 32 + x;
     double s = 0.0;
     int all = 0, kept = 0;
@@ -308,8 +312,8 @@ __global__ void __launch_bounds__(1024) router_loss_kernel(const LossArgs a) {
     }
     if (x == 0) {
         const double tokens = n / a.k;
-        a.out[0] = n > 0.0 ? (float)(a.E * dot / (n * tokens)) : 0.f;
-        a.out[1] = n > 0.0 ? (float)(z / tokens) : 0.f;
+        *a.balance = n > 0.0 ? (float)(a.E * dot / (n * tokens)) : 0.f;
+        *a.z_loss = n > 0.0 ? (float)(z / tokens) : 0.f;
         a.load[a.E] = n > 0.0 ? (float)(1.0 / tokens) : 0.f;
     }
 }
@@ -445,7 +449,8 @@ extern "C" {
 int neox_router_blocks(long long tokens, int E) { return router_blocks(tokens, E); }
 
 int neox_balanced_router(const void* x, long long stride, const void* kept, int tokens, int E, int k, int dtype, float* weights,
-                         long long* experts, void* row, long long* counts, float* load, float* out, void* scratch, void* stream) {
+                         long long* experts, void* row, long long* counts, float* load, float* balance, float* z_loss, void* scratch,
+                         void* stream) {
     if (tokens < 0 || E < 1 || E > 512 || k < 1 || k > MAX_K || k > E) return NEOX_ERR_SHAPE;
     const int blocks = router_blocks(tokens, E);
     double* z = (double*)scratch;
@@ -455,11 +460,11 @@ int neox_balanced_router(const void* x, long long stride, const void* kept, int 
     int* chosen = (int*)(sums + (long long)blocks * E);
     const ForwardArgs f = {x, stride, (const uint8_t*)kept, weights, experts, (float4*)row, sums, chosen, z, ticket, tokens, E, k,
                            rows_aligned(x, stride, E, dtype)};
-    const LossArgs l = {sums, chosen, z, ticket, part, counts, load, out, blocks, E, k};
+    const LossArgs l = {sums, chosen, z, ticket, part, counts, load, balance, z_loss, blocks, E, k};
     cudaStream_t st = (cudaStream_t)stream;
     FOR_TYPE(dtype, FOR_LANES(E, (router_kernel<T, L, C><<<blocks, THREADS, 0, st>>>(f))));
-    router_loss_kernel<<<(E + 31) / 32, 1024, 0, st>>>(l);
-    return launched();
+    if (launched() != 0) return NEOX_ERR_LAUNCH;
+    return launch::overlapped(router_loss_kernel, dim3((E + 31) / 32), dim3(1024), 1, st, l);
 }
 
 int neox_balanced_router_grad(const void* x, long long stride, const void* kept, int tokens, int E, int k, int dtype,

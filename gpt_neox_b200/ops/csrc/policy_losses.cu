@@ -720,7 +720,9 @@ struct PolicyArgs {
     float* shift;                  // per row: lse(x) - lse(y) + KL, for the KL over the vocabulary
     double* partial;               // [n * pieces, 4], then [n, 4]
     int* ticket;
-    float* out;                    // loss, mean KL, share of clipped tokens
+    float* loss;
+    float* kl_mean;
+    float* share;                  // of clipped tokens
     float* logp;                   // [n, s]
     float* coef;                   // [n]: what a row's slope is multiplied by
 };
@@ -831,9 +833,9 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(const PolicyArgs a) {
         total = sum[0];
         filled = sum[4];
         const bool any = sum[0] != 0.0;                        // nothing kept: no loss, no gradient
-        a.out[0] = !any ? 0.f : (float)(a.by_sequence ? sum[5] / sum[4] : sum[1] / sum[0]);
-        a.out[1] = any ? (float)(sum[2] / sum[0]) : 0.f;
-        a.out[2] = any ? (float)(sum[3] / sum[0]) : 0.f;
+        *a.loss = !any ? 0.f : (float)(a.by_sequence ? sum[5] / sum[4] : sum[1] / sum[0]);
+        *a.kl_mean = any ? (float)(sum[2] / sum[0]) : 0.f;
+        *a.share = any ? (float)(sum[3] / sum[0]) : 0.f;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < a.n; i += THREADS) {
@@ -995,78 +997,106 @@ constexpr int U_ONE = 8, U_FULL = 4;
 
 int launched() { return cudaGetLastError() == cudaSuccess ? 0 : NEOX_ERR_LAUNCH; }
 
+// One forward or backward call.  Some forty arguments, so they come packed (the caller's side is a struct format of the same
+// order: 64-bit words, doubles, ints); addresses are null where an operator has no such tensor.
+struct LossCall {
+    const void* x;                 // logits [n, s, vocab], element strides of the first two
+    long long xn, xs;
+    const void* y;                 // reference logits, or null
+    long long yn, ys;
+    const long long* labels;
+    const float* mask;
+    float2* part;                  // scratch: [streams][n * s, most]
+    float* cross;                  // scratch: [n * s, most], for the KL over the vocabulary
+    float* target;                 // scratch: [streams][n * s]
+    int* ticket;                   // scratch: 2
+    double* sums;                  // scratch: [n * pieces + n, 2 or 4]
+    float2* row;                   // kept for the backward: [n * s], [n], [n * s], [n * s]
+    float* coef;
+    float* slope;
+    float* shift;                  // the KL over the vocabulary has one
+    float* loss;
+    float* kl_mean;
+    float* clipped;
+    float* logp;                   // [n] preference, [n, s] policy
+    float* ref;                    // [n]
+    const float* old_logp;
+    const float* ref_logp;
+    const float* advantages;       // element (i, j) at i * adv_n + j * adv_s
+    long long adv_n, adv_s;
+    void* g;                       // backward: gradient of the logits
+    long long gn, gs;
+    const float* g_loss;
+    const float* g_logp;
+    long long v0, whole;           // first word of this share of the vocabulary; words of all shares
+    void* stream;
+    double beta, smoothing, low, high;       // beta: of the preference, or the KL's weight
+    int n, s, vocab, dtype;
+    int kl, by_sequence;
+    int most, chunks;              // 0 chunks: as the statistics found
+    int policy, first, second;     // which loss; whether to run the statistics and what joins them
+};
+
 }  // namespace
 
 extern "C" {
 
-// Chunks of a row that neox_vocab_stats has room for: `part` is [streams][n * s, this] pairs, `cross` [n * s, this].
-int neox_vocab_splits(long long rows, int vocab, int dtype, int full) {
+// Chunks of a row that the statistics have room for.
+int neox_vocab_chunks(long long rows, int vocab, int dtype, int full) {
     const StatsPlan p(rows, vocab, dtype, full);
     return p.most;
 }
 
-int neox_vocab_stats(const void* x, long long xn, long long xs, const void* y, long long yn, long long ys,
-                     const long long* labels, const float* mask, int n, int s, int vocab, long long v0, int dtype, int full,
-                     void* part, float* cross, float* target, int* ticket, void* stream) {
-    if (n < 0 || s < 0 || vocab < 1 || (full && !y)) return NEOX_ERR_SHAPE;
-    const long long rows = (long long)n * s;
-    const StatsPlan p(rows, vocab, dtype, full);
-    const int streams = !full && y ? 2 : 1;
-    if (rows * streams * p.most >= (1ll << 31)) return NEOX_ERR_TOO_LARGE;
-    const StatsArgs a = {{x, xn, xs}, {y, yn, ys}, labels, mask, (float2*)part, cross, target, ticket, v0, (int)rows, s, vocab,
-                         streams, p.chunks, p.most};
-    const int blocks = neox_sm_count();
-    cudaStream_t st = (cudaStream_t)stream;
-    if (full) FOR_TYPE(dtype, LAUNCH_STATS(T, true));
-    else FOR_TYPE(dtype, LAUNCH_STATS(T, false));
-    return launched();
-}
-
-// Blocks that join a sequence's rows; `partial` of the two calls below holds (n * this + n) * 2 or * 4 doubles.
+// Blocks that join a sequence's rows.
 int neox_loss_pieces(int s) { return s > 0 ? (s + ROWS - 1) / ROWS : 1; }
 
-int neox_preference_loss(const void* part, const float* target, int most, int chunks, const long long* labels, const float* mask,
-                         const float* ref_logp, int has_ref_logits, int n, int s, long long vocab, double beta, double smoothing,
-                         void* row, double* partial, int* ticket, float* loss, float* logp, float* ref, float* coef, void* stream) {
-    if (n < 2 || n % 2 || s < 0) return NEOX_ERR_SHAPE;
-    const int pieces = neox_loss_pieces(s);
-    if ((long long)n * pieces >= (1ll << 31)) return NEOX_ERR_TOO_LARGE;
-    const PreferenceArgs a = {{(const float2*)part, nullptr, target, labels, ticket, vocab, n * s, most, chunks}, mask, ref_logp, has_ref_logits, n, s, pieces, beta,
-                              smoothing, (float2*)row, partial, ticket, loss, logp, ref, coef};
-    return launch::overlapped(preference_kernel, dim3(n * pieces), dim3(THREADS), 1, (cudaStream_t)stream, a);
+int neox_loss_forward(const void* packed) {
+    const LossCall& c = *(const LossCall*)packed;
+    const bool full = c.shift != nullptr;
+    const long long rows = (long long)c.n * c.s, pieces = neox_loss_pieces(c.s);
+    const int streams = !full && c.y ? 2 : 1;
+    if (c.n < (c.policy ? 1 : 2) || (!c.policy && c.n % 2) || c.s < 0 || c.vocab < 1 || (full && !c.y)) return NEOX_ERR_SHAPE;
+    if (rows * streams * c.most >= (1ll << 31) || c.n * pieces >= (1ll << 31)) return NEOX_ERR_TOO_LARGE;
+    cudaStream_t st = (cudaStream_t)c.stream;
+    if (c.first) {
+        const StatsPlan p(rows, c.vocab, c.dtype, full);
+        if (p.most != c.most) return NEOX_ERR_SHAPE;
+        const StatsArgs a = {{c.x, c.xn, c.xs}, {c.y, c.yn, c.ys}, c.labels, c.mask, c.part, c.cross, c.target, c.ticket, c.v0,
+                             (int)rows, c.s, c.vocab, streams, p.chunks, p.most};
+        const int blocks = neox_sm_count();
+        if (full) FOR_TYPE(c.dtype, LAUNCH_STATS(T, true));
+        else FOR_TYPE(c.dtype, LAUNCH_STATS(T, false));
+        if (launched() != 0) return NEOX_ERR_LAUNCH;
+    }
+    if (!c.second) return 0;
+    const RowSums sums = {c.part, c.cross, c.target, c.labels, c.ticket, c.whole, (int)rows, c.most, c.chunks};
+    const dim3 grid((unsigned)(c.n * pieces));
+    if (c.policy) {
+        const PolicyArgs a = {sums, c.mask, c.advantages, c.adv_n, c.adv_s, c.old_logp, c.ref_logp, c.y != nullptr, c.n, c.s,
+                              (int)pieces, c.kl, c.by_sequence, c.low, c.high, c.beta, c.row, c.slope, c.shift, c.sums, c.ticket,
+                              c.loss, c.kl_mean, c.clipped, c.logp, c.coef};
+        return launch::overlapped(policy_kernel, grid, dim3(THREADS), 1, st, a);
+    }
+    const PreferenceArgs a = {sums, c.mask, c.ref_logp, c.y != nullptr, c.n, c.s, (int)pieces, c.beta, c.smoothing, c.row, c.sums,
+                              c.ticket, c.loss, c.logp, c.ref, c.coef};
+    return launch::overlapped(preference_kernel, grid, dim3(THREADS), 1, st, a);
 }
 
-int neox_policy_loss(const void* part, const float* cross, const float* target, int most, int chunks, const long long* labels, const float* mask,
-                     const float* advantages, long long adv_n, long long adv_s, const float* old_logp, const float* ref_logp,
-                     int has_ref_logits, int n, int s, long long vocab, int kl, int by_sequence, double low, double high,
-                     double kl_beta, void* row, float* slope, float* shift, double* partial, int* ticket, float* out, float* logp,
-                     float* coef, void* stream) {
-    if (n < 1 || s < 0) return NEOX_ERR_SHAPE;
-    const int pieces = neox_loss_pieces(s);
-    if ((long long)n * pieces >= (1ll << 31)) return NEOX_ERR_TOO_LARGE;
-    const PolicyArgs a = {{(const float2*)part, cross, target, labels, ticket, vocab, n * s, most, chunks}, mask, advantages, adv_n, adv_s, old_logp, ref_logp,
-                          has_ref_logits, n, s, pieces, kl, by_sequence, low, high, kl_beta, (float2*)row, slope, shift, partial,
-                          ticket, out, logp, coef};
-    return launch::overlapped(policy_kernel, dim3(n * pieces), dim3(THREADS), 1, (cudaStream_t)stream, a);
-}
-
-int neox_vocab_grad(const void* x, long long xn, long long xs, const void* y, long long yn, long long ys, void* g, long long gn,
-                    long long gs, const long long* labels, const float* slope, const float* mask, const float* shift,
-                    const void* row, const float* coef, const float* g_loss, const float* g_logp, float kl_beta, int n, int s,
-                    int vocab, long long v0, int dtype, void* stream) {
-    if (n < 0 || s < 0 || vocab < 1) return NEOX_ERR_SHAPE;
-    const int full = shift != nullptr;
-    const GradPlan p(vocab, dtype, full ? U_FULL : U_ONE);
-    const long long rows = (long long)n * s;
+int neox_loss_backward(const void* packed) {
+    const LossCall& c = *(const LossCall*)packed;
+    const bool full = c.shift != nullptr;
+    if (c.n < 0 || c.s < 0 || c.vocab < 1) return NEOX_ERR_SHAPE;
+    const GradPlan p(c.vocab, c.dtype, full ? U_FULL : U_ONE);
+    const long long rows = (long long)c.n * c.s;
     if (rows == 0) return 0;
-    if (!p.fits(rows, vocab)) return NEOX_ERR_TOO_LARGE;
-    const GradArgs a = {{x, xn, xs}, {y, yn, ys}, g, gn, gs, labels, slope, mask, shift, (const float2*)row, coef, g_loss, g_logp,
-                        v0, kl_beta, (int)rows, s, vocab, p.splits, p.chunk};
+    if (!p.fits(rows, c.vocab)) return NEOX_ERR_TOO_LARGE;
+    const GradArgs a = {{c.x, c.xn, c.xs}, {c.y, c.yn, c.ys}, c.g, c.gn, c.gs, c.labels, c.slope, c.mask, c.shift, c.row, c.coef,
+                        c.g_loss, c.g_logp, c.v0, (float)c.beta, (int)rows, c.s, c.vocab, p.splits, p.chunk};
     const long long per = THREADS / p.threads;
     const unsigned grid = (unsigned)((rows * p.splits + per - 1) / per);
-    cudaStream_t st = (cudaStream_t)stream;
-    if (full) FOR_TYPE(dtype, FOR_THREADS(p.threads, (grad_kernel<T, G, U_FULL, true><<<grid, THREADS, 0, st>>>(a))));
-    else FOR_TYPE(dtype, FOR_THREADS(p.threads, (grad_kernel<T, G, U_ONE, false><<<grid, THREADS, 0, st>>>(a))));
+    cudaStream_t st = (cudaStream_t)c.stream;
+    if (full) FOR_TYPE(c.dtype, FOR_THREADS(p.threads, (grad_kernel<T, G, U_FULL, true><<<grid, THREADS, 0, st>>>(a))));
+    else FOR_TYPE(c.dtype, FOR_THREADS(p.threads, (grad_kernel<T, G, U_ONE, false><<<grid, THREADS, 0, st>>>(a))));
     return launched();
 }
 

@@ -14,6 +14,7 @@ moe_mlp.py`` (grouped expert MLP through MegaBlocks' ``gmm``), ``megatron/model/
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import NamedTuple
 
 import torch
@@ -29,7 +30,7 @@ PAD = 64
 _P, _I, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
 native._ARGTYPES.update({
     "neox_router_blocks": [_L, _I],
-    "neox_balanced_router": [_P, _L, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P],
+    "neox_balanced_router": [_P, _L, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P],
     "neox_balanced_router_grad": [_P, _L, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P],
 })
 native._CountingLib._NOT_LAUNCHES.add("neox_router_blocks")
@@ -124,31 +125,41 @@ def balanced_router_ref(logits, k, token_mask=None):
     return RouterOutput(w, experts, counts, balance, z)
 
 
+@functools.lru_cache(maxsize=256)
+def _router_layout(tokens, experts, device):
+    """Floats of one forward's buffer: ``[E + 1]`` loads (an even number), ``[T, 4]`` row statistics -- kept for the backward -- and
+    the scratch that the kernels' blocks leave their sums in."""
+    load, row = (experts + 4) // 4 * 4, 4 * tokens
+    blocks = native.lib().neox_router_blocks(tokens, experts)
+    return load, load + row, load + row + (blocks * (experts * 12 + 8) + 16 * 17 + 16 + 3) // 4
+
+
 def _balanced_values(x, k, kept):
     T, E = x.shape
-    L, dev = native.lib(), x.device
+    dev = x.device
     weights = torch.empty(T, k, dtype=torch.float32, device=dev)
     experts = torch.empty(T, k, dtype=torch.int64, device=dev)
-    row = torch.empty(T, 4, dtype=torch.float32, device=dev)
     counts = torch.empty(E, dtype=torch.int64, device=dev)
-    load = torch.empty(E + 1, dtype=torch.float32, device=dev)
-    out = torch.empty(2, dtype=torch.float32, device=dev)
-    scratch = torch.empty(L.neox_router_blocks(T, E) * (E * 12 + 8) + 16 * 17 + 16, dtype=torch.uint8, device=dev)
-    rc = L.neox_balanced_router(x.data_ptr(), x.stride(0), None if kept is None else kept.data_ptr(), T, E, k, _DT[x.dtype],
-                                weights.data_ptr(), experts.data_ptr(), row.data_ptr(), counts.data_ptr(), load.data_ptr(),
-                                out.data_ptr(), scratch.data_ptr(), native.stream_ptr())
+    balance = torch.empty((), dtype=torch.float32, device=dev)
+    z = torch.empty((), dtype=torch.float32, device=dev)
+    row, scratch, total = _router_layout(T, E, x.get_device())
+    buf = torch.empty(total, dtype=torch.float32, device=dev)
+    load = buf.data_ptr()
+    rc = native.lib().neox_balanced_router(x.data_ptr(), x.stride(0), None if kept is None else kept.data_ptr(), T, E, k,
+                                           _DT[x.dtype], weights.data_ptr(), experts.data_ptr(), load + 4 * row,
+                                           counts.data_ptr(), load, balance.data_ptr(), z.data_ptr(), load + 4 * scratch,
+                                           native.stream_ptr())
     native.check(rc, "neox_balanced_router")
-    balance, z = out.unbind(0)
-    return weights, experts, counts, balance, z, row, load
+    return weights, experts, counts, balance, z, buf
 
 
 class _BalancedRouterFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, k, kept):
         with device_of(x):
-            weights, experts, counts, balance, z, row, load = _balanced_values(x, k, kept)
+            weights, experts, counts, balance, z, buf = _balanced_values(x, k, kept)
         # the weights are an output: saved as such, so that changing them in place is noticed
-        ctx.save_for_backward(x, kept, weights, experts, row, load)
+        ctx.save_for_backward(x, kept, weights, experts, buf)
         ctx.k = k
         ctx.mark_non_differentiable(experts, counts)
         ctx.set_materialize_grads(False)
@@ -156,17 +167,19 @@ class _BalancedRouterFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g_weights, _e, _c, g_balance, g_z):
-        x, kept, weights, experts, row, load = ctx.saved_tensors
+        x, kept, weights, experts, buf = ctx.saved_tensors
         T, E = x.shape
         dx = torch.empty(T, E, dtype=x.dtype, device=x.device)
-        gw, gb, gz = (None if g is None else g.float().contiguous() for g in (g_weights, g_balance, g_z))
+        gw, gb, gz = (g if g is None or g.dtype == torch.float32 and g.is_contiguous() else g.float().contiguous()
+                      for g in (g_weights, g_balance, g_z))
+        load = buf.data_ptr()
         with device_of(x):
             rc = native.lib().neox_balanced_router_grad(
                 x.data_ptr(), x.stride(0), None if kept is None else kept.data_ptr(), T, E, ctx.k, _DT[x.dtype],
-                weights.data_ptr(), experts.data_ptr(), row.data_ptr(), load.data_ptr(), None if gw is None else gw.data_ptr(),
-                None if gb is None else gb.data_ptr(), None if gz is None else gz.data_ptr(), dx.data_ptr(),
-                native.stream_ptr())
-            native.check(rc, "neox_balanced_router_grad")
+                weights.data_ptr(), experts.data_ptr(), load + 4 * _router_layout(T, E, x.get_device())[0], load,
+                None if gw is None else gw.data_ptr(), None if gb is None else gb.data_ptr(),
+                None if gz is None else gz.data_ptr(), dx.data_ptr(), native.stream_ptr())
+        native.check(rc, "neox_balanced_router_grad")
         return once(dx, x), None, None
 
 

@@ -13,6 +13,8 @@ log-probabilities in fp32.
 from __future__ import annotations
 
 import ctypes
+import functools
+import struct
 from typing import NamedTuple, Optional
 
 import torch
@@ -23,17 +25,16 @@ from .functional import _DT, _k, device_of, once
 
 KL_KINDS = {"kl": 1, "abs": 2, "mse": 3, "k3": 4, "full": 5}
 
-_P, _I, _L, _D, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_double, ctypes.c_float
 native._ARGTYPES.update({
-    "neox_vocab_splits": [_L, _I, _I, _I],
-    "neox_loss_pieces": [_I],
-    "neox_vocab_stats": [_P, _L, _L, _P, _L, _L, _P, _P, _I, _I, _I, _L, _I, _I, _P, _P, _P, _P, _P],
-    "neox_preference_loss": [_P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _L, _D, _D, _P, _P, _P, _P, _P, _P, _P, _P],
-    "neox_policy_loss": [_P, _P, _P, _I, _I, _P, _P, _P, _L, _L, _P, _P, _I, _I, _I, _L, _I, _I, _D, _D, _D, _P, _P, _P, _P, _P, _P, _P,
-                         _P, _P],
-    "neox_vocab_grad": [_P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P, _F, _I, _I, _I, _L, _I, _P],
+    "neox_vocab_chunks": [ctypes.c_longlong, ctypes.c_int, ctypes.c_int, ctypes.c_int],
+    "neox_loss_pieces": [ctypes.c_int],
+    "neox_loss_forward": [ctypes.c_char_p],
+    "neox_loss_backward": [ctypes.c_char_p],
 })
-native._CountingLib._NOT_LAUNCHES.update({"neox_vocab_splits", "neox_loss_pieces"})
+native._CountingLib._NOT_LAUNCHES.update({"neox_vocab_chunks", "neox_loss_pieces"})
+
+# The kernels' arguments in the order of LossCall (csrc/policy_losses.cu): addresses and 64-bit words, doubles, ints.
+_CALL = struct.Struct("@35q4d11i4x")
 
 
 class PreferenceLoss(NamedTuple):
@@ -101,169 +102,168 @@ def _tensor_parallel():
 
 
 # ---------------------------------------------------------------------------------------------- kernels
-class _Stats:
-    """One pass over the kept rows of policy (and reference) logits, and the scratch memory of a forward, in one piece::
+@functools.lru_cache(maxsize=256)
+def _layout(n, s, v, dtype, streams, width, full, device):
+    """Chunks of a row, and where the parts of a forward's one buffer begin, in bytes, with its size in floats at the end::
 
         sums    [n * (pieces + 1), width] fp64    what the joining kernel's blocks leave
         part    [streams, rows, most, 2]          maximum and sum of every chunk of a row, policy and reference
         cross   [rows, most]                      sum of p (x - y), for the KL over the vocabulary
         target  [streams, rows]                   the labels' logits
         ticket  [2] int32
-
-    With the vocabulary split over ranks the chunks are joined here and two all-reduces -- maxima, then sums and label logits --
-    make the statistics those of whole rows.  What stands in rows of mask zero is never read."""
-
-    def __init__(self, x, y, labels, mask, full, width):
-        n, s, v = x.shape
-        rows = n * s
-        streams = 1 if y is None else 2
-        tp, rank, group = _tensor_parallel()
-        L, dt = native.lib(), _DT[x.dtype]
-        most = L.neox_vocab_splits(rows, v, dt, full)
-        sums = 2 * width * n * (L.neox_loss_pieces(s) + 1)
-        parts = streams * rows * most * 2
-        crosses = rows * most if full else 0
-        self.buf = buf = torch.empty(sums + parts + crosses + streams * rows + 2, dtype=torch.float32, device=x.device)
-        self.sums = buf.data_ptr()
-        self.part = self.sums + 4 * sums
-        self.cross = self.part + 4 * parts
-        self.target = self.cross + 4 * crosses
-        self.ticket = self.target + 4 * streams * rows
-        self.most, self.chunks, self.first, self.vocab = most, 0, rank * v, tp * v
-        y_ = x if y is None else y
-        rc = L.neox_vocab_stats(x.data_ptr(), x.stride(0), x.stride(1), None if y is None else y.data_ptr(), y_.stride(0),
-                                y_.stride(1), labels.data_ptr(), mask.data_ptr(), n, s, v, self.first, dt, full, self.part,
-                                self.cross, self.target, self.ticket, native.stream_ptr())
-        native.check(rc, "neox_vocab_stats")
-        if tp > 1:
-            self._reduce(sums, parts, crosses, streams, rows, group())
-
-    def _reduce(self, sums, parts, crosses, streams, rows, group):
-        import torch.distributed as dist
-        _, part, cross, target, ticket = self.buf.split([sums, parts, crosses, streams * rows, 2])
-        part, target = part.view(streams, rows, self.most, 2), target.view(streams, rows)
-        there = torch.arange(self.most, device=part.device) < ticket.view(torch.int32)[1]
-        local = torch.where(there, part[..., 0], torch.finfo(torch.float32).min)
-        top = local.amax(-1)
-        dist.all_reduce(top, op=dist.ReduceOp.MAX, group=group)
-        scale = (local - top[..., None]).exp()
-        terms = [torch.where(there, part[..., 1] * scale, 0.0).sum(-1), target]
-        if crosses:
-            terms.append(torch.where(there, cross.view(rows, self.most) * scale[0], 0.0).sum(-1)[None])
-        both = torch.cat(terms)
-        dist.all_reduce(both, group=group)
-        joined = torch.stack([top, both[:streams]], -1)
-        self.keep = (joined, both)
-        self.part, self.target = joined.data_ptr(), both[streams].data_ptr()
-        self.cross = both[-1].data_ptr() if crosses else 0
-        self.most = self.chunks = 1
+        row     [rows, 2]                         maximum and 1 / sum, from here on kept for the backward
+        coef    [n]
+        slope   [rows]                            of the policy loss
+        shift   [rows]                            for the KL over the vocabulary
+    """
+    L, rows = native.lib(), n * s
+    most = L.neox_vocab_chunks(rows, v, dtype, full)
+    sizes = (2 * width * n * (L.neox_loss_pieces(s) + 1), 2 * streams * rows * most, rows * most * full, streams * rows, 2,
+             2 * rows, n, rows * (width == 4), rows * full)
+    at, offsets = 0, []
+    for size in sizes:
+        offsets.append(4 * at)
+        at += size + size % 2                   # pairs of floats and doubles are read in one piece
+    return (most, *offsets, at)
 
 
-def _logits_grad(x, y, labels, slope, mask, shift, row, coef, g_loss, g_logp, kl_beta, first):
-    """Gradient of the logits in their own memory order where that is dense.  ``slope`` to ``coef`` are addresses."""
+def _reduced(buf, at, streams, rows, most, full, group):
+    """Statistics of whole rows from those of every rank's share of the vocabulary: the chunks are joined here and two all-reduces
+    follow, maxima, then sums and label logits.  What stands in rows of mask zero is never read."""
+    import torch.distributed as dist
+    _, part, cross, target, ticket = (o // 4 for o in at[:5])
+    part = buf[part:part + 2 * streams * rows * most].view(streams, rows, most, 2)
+    there = torch.arange(most, device=buf.device) < buf[ticket:ticket + 2].view(torch.int32)[1]
+    local = torch.where(there, part[..., 0], torch.finfo(torch.float32).min)
+    top = local.amax(-1)
+    dist.all_reduce(top, op=dist.ReduceOp.MAX, group=group)
+    scale = (local - top[..., None]).exp()
+    terms = [torch.where(there, part[..., 1] * scale, 0.0).sum(-1),
+             buf[target:target + (1 if full else streams) * rows].view(-1, rows)]
+    if full:
+        terms.append(torch.where(there, buf[cross:cross + rows * most].view(rows, most) * scale[0], 0.0).sum(-1)[None])
+    both = torch.cat(terms)
+    dist.all_reduce(both, group=group)
+    return torch.stack([top, both[:streams]], -1), both[streams:], both[-1]
+
+
+def _forward(x, y, labels, mask, width, loss, kl_mean, clipped, logp, ref, old_logp, ref_logp, adv, kl, by_sequence, beta, smoothing,
+             low, high):
+    """Runs a forward into the given outputs; the buffer whose end the backward needs, and the first word of this rank's share of
+    the vocabulary."""
     n, s, v = x.shape
+    dt, streams, full = _DT[x.dtype], 1 if y is None else 2, int(kl == KL_KINDS["full"])
+    tp, rank, group = _tensor_parallel()
+    most, *at, total = _layout(n, s, v, dt, streams, width, full, x.get_device())
+    buf = torch.empty(total, dtype=torch.float32, device=x.device)
+    base = buf.data_ptr()
+    sums, part, cross, target, ticket, row, coef, slope, shift = [base + o for o in at]
+    y_ = x if y is None else y
+    head = (x.data_ptr(), x.stride(0), x.stride(1), 0 if y is None else y.data_ptr(), y_.stride(0), y_.stride(1),
+            labels.data_ptr(), mask.data_ptr())
+    tail = (ticket, sums, row, coef, slope, shift if full else 0, loss.data_ptr(), 0 if kl_mean is None else kl_mean.data_ptr(),
+            0 if clipped is None else clipped.data_ptr(), logp.data_ptr(), 0 if ref is None else ref.data_ptr(),
+            0 if old_logp is None else old_logp.data_ptr(), 0 if ref_logp is None else ref_logp.data_ptr(),
+            0 if adv is None else adv.data_ptr(), 0 if adv is None else adv.stride(0), 0 if adv is None else adv.stride(1),
+            0, 0, 0, 0, 0, rank * v, tp * v, native.stream_ptr(), beta, smoothing, low, high, n, s, v, dt, kl, by_sequence)
+    run = native.lib().neox_loss_forward
+    policy = width == 4
+    if tp == 1:
+        native.check(run(_CALL.pack(*head, part, cross, target, *tail, most, 0, policy, 1, 1)), "neox_loss_forward")
+    else:
+        native.check(run(_CALL.pack(*head, part, cross, target, *tail, most, 0, policy, 1, 0)), "neox_loss_forward")
+        pairs, targets, crosses = _reduced(buf, at, streams, n * s, most, full, group())
+        native.check(run(_CALL.pack(*head, pairs.data_ptr(), crosses.data_ptr(), targets.data_ptr(), *tail, 1, 1, policy, 0, 1)),
+                     "neox_loss_forward")
+    return buf, rank * v
+
+
+def _backward(x, y, labels, mask, buf, first, width, streams, g_loss, g_logp, beta):
+    """Gradient of the logits, in their own memory order where that is dense.  ``y``: the reference, for the KL over the
+    vocabulary."""
+    n, s, v = x.shape
+    dt, full = _DT[x.dtype], int(y is not None)
+    _, *at, _ = _layout(n, s, v, dt, streams, width, full, x.get_device())
+    base = buf.data_ptr()
+    row, coef, slope, shift = [base + o for o in at[5:]]
     g = torch.empty_like(x)
     if g.stride(2) != 1:
         g = torch.empty(n, s, v, dtype=x.dtype, device=x.device)
     y_ = x if y is None else y
-    rc = native.lib().neox_vocab_grad(
-        x.data_ptr(), x.stride(0), x.stride(1), y_.data_ptr(), y_.stride(0), y_.stride(1), g.data_ptr(), g.stride(0), g.stride(1),
-        labels.data_ptr(), slope, mask.data_ptr(), shift, row, coef, None if g_loss is None else g_loss.data_ptr(),
-        None if g_logp is None else g_logp.data_ptr(), kl_beta, n, s, v, first, _DT[x.dtype], native.stream_ptr())
-    native.check(rc, "neox_vocab_grad")
+    weight = mask.data_ptr()
+    call = _CALL.pack(x.data_ptr(), x.stride(0), x.stride(1), y_.data_ptr(), y_.stride(0), y_.stride(1), labels.data_ptr(), weight,
+                      0, 0, 0, 0, 0, row, coef, slope if width == 4 else weight, shift if full else 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
+                      g.data_ptr(), g.stride(0), g.stride(1), 0 if g_loss is None else g_loss.data_ptr(),
+                      0 if g_logp is None else g_logp.data_ptr(), first, 0, native.stream_ptr(), beta, 0.0, 0.0, 0.0, n, s, v, dt,
+                      0, 0, 0, 0, 0, 0, 0)
+    native.check(native.lib().neox_loss_backward(call), "neox_loss_backward")
     return g
 
 
 def _preference_values(x, labels, mask, ref_logits, ref_logp, beta, smoothing):
-    """Loss, log-probabilities, what the backward needs (``[rows, 2]`` maximum and 1 / sum, then ``[n]`` coefficients), and the
-    first word of this rank's vocabulary."""
-    n, s, _ = x.shape
-    st = _Stats(x, ref_logits, labels, mask, 0, 2)
-    dev = x.device
-    kept = torch.empty(2 * n * s + n, dtype=torch.float32, device=dev)
+    n, dev = x.shape[0], x.device
     loss = torch.empty((), dtype=torch.float32, device=dev)
     logp = torch.empty(n, dtype=torch.float32, device=dev)
     ref = torch.empty(n, dtype=torch.float32, device=dev)
-    row = kept.data_ptr()
-    rc = native.lib().neox_preference_loss(
-        st.part, st.target, st.most, st.chunks, labels.data_ptr(), mask.data_ptr(), None if ref_logp is None else ref_logp.data_ptr(),
-        ref_logits is not None, n, s, st.vocab, beta, smoothing, row, st.sums, st.ticket, loss.data_ptr(), logp.data_ptr(),
-        ref.data_ptr(), row + 8 * n * s, native.stream_ptr())
-    native.check(rc, "neox_preference_loss")
-    return loss, logp, ref, kept, st.first
+    kept = _forward(x, ref_logits, labels, mask, 2, loss, None, None, logp, ref, None, ref_logp, None, 0, 0, beta, smoothing, 0.0, 0.0)
+    return loss, logp, ref, kept
 
 
 def _grad_f32(g):
-    return None if g is None else _as(g, torch.float32)
+    return g if g is None or (g.dtype == torch.float32 and g.is_contiguous()) else g.float().contiguous()
 
 
 class _PreferenceFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, labels, mask, ref_logits, ref_logp, beta, smoothing):
         with device_of(x):
-            loss, logp, ref, kept, ctx.first = _preference_values(x, labels, mask, ref_logits, ref_logp, beta, smoothing)
-        ctx.save_for_backward(x, labels, mask, kept)
+            loss, logp, ref, (buf, ctx.first) = _preference_values(x, labels, mask, ref_logits, ref_logp, beta, smoothing)
+        ctx.streams = 1 if ref_logits is None else 2
+        ctx.save_for_backward(x, labels, mask, buf)
         ctx.mark_non_differentiable(ref)
         ctx.set_materialize_grads(False)
         return loss, logp, ref
 
     @staticmethod
     def backward(ctx, g_loss, g_logp, _):
-        x, labels, mask, kept = ctx.saved_tensors
         if g_loss is None and g_logp is None:
             return (None,) * 7
-        row = kept.data_ptr()
+        x, labels, mask, buf = ctx.saved_tensors
         with device_of(x):
-            g = _logits_grad(x, None, labels, mask.data_ptr(), mask, None, row, row + 8 * mask.numel(), _grad_f32(g_loss),
-                             _grad_f32(g_logp), 0.0, ctx.first)
-        return (once(g, x),) + (None,) * 6
+            g = _backward(x, None, labels, mask, buf, ctx.first, 2, ctx.streams, _grad_f32(g_loss), _grad_f32(g_logp), 0.0)
+        return once(g, x), None, None, None, None, None, None
 
 
 def _policy_values(x, labels, mask, adv, old_logp, ref_logits, ref_logp, low, high, kl, kl_beta, by_sequence):
-    """Loss, means, log-probabilities, what the backward needs (``[rows, 2]`` maximum and 1 / sum, ``[n]`` coefficients, ``[rows]``
-    slopes and, for the KL over the vocabulary, ``[rows]`` shifts), and the first word of this rank's vocabulary."""
-    n, s, _ = x.shape
-    rows, full = n * s, kl == KL_KINDS["full"]
-    st = _Stats(x, ref_logits, labels, mask, int(full), 4)
     dev = x.device
-    kept = torch.empty((4 if full else 3) * rows + n, dtype=torch.float32, device=dev)
-    out = torch.empty(3, dtype=torch.float32, device=dev)
-    logp = torch.empty(n, s, dtype=torch.float32, device=dev)
-    row = kept.data_ptr()
-    coef = row + 8 * rows
-    slope = coef + 4 * n
-    rc = native.lib().neox_policy_loss(
-        st.part, st.cross, st.target, st.most, st.chunks, labels.data_ptr(), mask.data_ptr(), adv.data_ptr(), adv.stride(0),
-        adv.stride(1), None if old_logp is None else old_logp.data_ptr(), None if ref_logp is None else ref_logp.data_ptr(),
-        ref_logits is not None, n, s, st.vocab, kl, by_sequence, low, high, kl_beta, row, slope, slope + 4 * rows if full else None,
-        st.sums, st.ticket, out.data_ptr(), logp.data_ptr(), coef, native.stream_ptr())
-    native.check(rc, "neox_policy_loss")
-    return (*out.unbind(0), logp, kept, st.first)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    kl_mean = torch.empty((), dtype=torch.float32, device=dev)
+    clipped = torch.empty((), dtype=torch.float32, device=dev)
+    logp = torch.empty(x.shape[:2], dtype=torch.float32, device=dev)
+    kept = _forward(x, ref_logits, labels, mask, 4, loss, kl_mean, clipped, logp, None, old_logp, ref_logp, adv, kl, by_sequence, kl_beta,
+                    0.0, low, high)
+    return loss, kl_mean, clipped, logp, kept
 
 
 class _PolicyFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, labels, mask, adv, old_logp, ref_logits, ref_logp, low, high, kl, kl_beta, by_sequence):
         with device_of(x):
-            loss, mean_kl, clipped, logp, kept, ctx.first = _policy_values(x, labels, mask, adv, old_logp, ref_logits, ref_logp, low,
-                                                                           high, kl, kl_beta, by_sequence)
-        ctx.full, ctx.kl_beta = kl == KL_KINDS["full"], kl_beta
-        ctx.save_for_backward(x, labels, mask, kept, ref_logits if ctx.full else None)
-        ctx.mark_non_differentiable(mean_kl, clipped, logp)
+            loss, kl_mean, clipped, logp, (buf, ctx.first) = _policy_values(x, labels, mask, adv, old_logp, ref_logits, ref_logp, low,
+                                                                            high, kl, kl_beta, by_sequence)
+        ctx.streams, ctx.kl_beta = 1 if ref_logits is None else 2, kl_beta
+        ctx.save_for_backward(x, labels, mask, buf, ref_logits if kl == KL_KINDS["full"] else None)
+        ctx.mark_non_differentiable(kl_mean, clipped, logp)
         ctx.set_materialize_grads(False)
-        return loss, mean_kl, clipped, logp
+        return loss, kl_mean, clipped, logp
 
     @staticmethod
     def backward(ctx, g_loss, *_):
-        x, labels, mask, kept, ref_logits = ctx.saved_tensors
         if g_loss is None:
             return (None,) * 12
-        rows, row = mask.numel(), kept.data_ptr()
-        coef = row + 8 * rows
-        slope = coef + 4 * mask.shape[0]
+        x, labels, mask, buf, y = ctx.saved_tensors
         with device_of(x):
-            g = _logits_grad(x, ref_logits, labels, slope, mask, slope + 4 * rows if ctx.full else None, row, coef,
-                             _grad_f32(g_loss), None, ctx.kl_beta, ctx.first)
+            g = _backward(x, y, labels, mask, buf, ctx.first, 4, ctx.streams, _grad_f32(g_loss), None, ctx.kl_beta)
         return (once(g, x),) + (None,) * 11
 
 
