@@ -30,8 +30,8 @@ PAD = 64
 _P, _I, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
 native._ARGTYPES.update({
     "neox_router_blocks": [_L, _I],
-    "neox_balanced_router": [_P, _L, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P],
-    "neox_balanced_router_grad": [_P, _L, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P],
+    "neox_balanced_router": [_P, _L, _P, _I, _I, _I, _I, *[_P] * 9],
+    "neox_balanced_router_grad": [_P, _L, _P, _I, _I, _I, _I, *[_P] * 9],
 })
 native._CountingLib._NOT_LAUNCHES.add("neox_router_blocks")
 
