@@ -225,9 +225,12 @@ kto_undesirable_weight : float = 1.0
 z_loss : float = 0.0
 kto_beta : float = 0.1
 fp32_reinforce : bool = True
-kl_impl : lit[abs|mse|kl|full] = 'mse'
+kl_impl : lit[abs|mse|kl|full|k3] = 'mse'
 kl_div_beta : float = 0.1
 reinforce_leave_one_out : bool = False
+reinforce_clip : float = None
+reinforce_clip_high : float = None
+reinforce_sequence_mean : bool = False
 allow_chopped : bool = True
 mmap_warmup : bool = False
 save : str = None
@@ -315,6 +318,7 @@ moe_type : str = 'megablocks'
 moe_glu : bool = False
 moe_lbl_in_fp32 : bool = False
 moe_jitter_eps : float = None
+moe_z_loss_coeff : float = 0.0
 enable_expert_tensor_parallelism : bool = False
 
 [engine]

@@ -2,7 +2,8 @@
 ``megatron/data/online_dataset.py:29-128``): each request returns a pickled
 ``{"prefix": [...], "completions": [[...], ...], "rewards": [...]}`` batch; rewards are centred with a
 leave-one-out baseline or a moving average, and every completion becomes one sample with the prompt positions
-labelled -100."""
+labelled -100.  An optional ``"logprobs": [[...], ...]`` (of every completion's tokens under the policy that sampled them) becomes
+``old_logp``, which ``reinforce_clip`` needs."""
 from __future__ import annotations
 
 import pickle
@@ -56,15 +57,24 @@ class OnlineDataset(torch.utils.data.Dataset):
             baseline = np.full_like(rewards, float(np.mean(self.reward_window)))
         centred = rewards - baseline
         prefix = list(batch["prefix"])
-        for comp, rw, raw in zip(batch["completions"], centred, rewards):
+        # log-probabilities of the completions' tokens under the policy that sampled them, for the clipped loss
+        logps = batch.get("logprobs") or [None] * len(batch["completions"])
+        for comp, rw, raw, logp in zip(batch["completions"], centred, rewards, logps):
             toks = (prefix + list(comp))[: self.seq_length + 1]
             n = len(toks)
             text = np.zeros(self.seq_length + 1, dtype=np.int64)
             text[:n] = toks
             label = np.full(self.seq_length + 1, -100, dtype=np.int64)
             label[len(prefix):n] = toks[len(prefix):n]
-            self.queue.append({"text": text, "label": label, "reward": np.full(self.seq_length + 1, rw, np.float32),
-                               "raw_reward": np.float32(raw)})
+            sample = {"text": text, "label": label, "reward": np.full(self.seq_length + 1, rw, np.float32),
+                      "raw_reward": np.float32(raw)}
+            if logp is not None:
+                if len(logp) != len(comp):
+                    raise ValueError(f"the data server sent {len(logp)} log-probabilities for {len(comp)} tokens")
+                old = np.zeros(self.seq_length + 1, dtype=np.float32)
+                old[len(prefix):n] = np.asarray(logp, dtype=np.float32)[: max(n - len(prefix), 0)]
+                sample["old_logp"] = old
+            self.queue.append(sample)
 
     def __getitem__(self, idx):
         while not self.queue:

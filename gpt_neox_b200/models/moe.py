@@ -10,14 +10,15 @@ Data flow for T local tokens, E experts, top-k::
 
     probs = softmax(router(x))                       [T, E]
     (w, e) = topk(probs)                             [T, k]      (weights renormalised when k > 1)
+    auxiliary loss of the layer from probs and e     (fused with the router on a GPU)
     sort the T*k assignments by expert -> contiguous per-expert segments (capacity applied here)
     all-to-all over the expert-parallel group: every rank receives the segments of ITS experts
     per local expert: h = act(seg W1^T) W2^T         tcgen05 GEMMs on the variable-length segments
     all-to-all back, un-sort, y[token] += w * out
 
 The auxiliary load-balancing loss returned with the output is ``E * sum_e f_e * P_e`` (``f_e`` fraction of
-assignments routed to expert e, ``P_e`` mean router probability); ``training.py`` scales it by
-``moe_loss_coeff``.  Expert weights are tagged ``expert_parallel`` so the optimizer reduces their gradients
+assignments routed to expert e, ``P_e`` mean router probability), plus the mean of ``logsumexp(router(x))^2`` where
+``moe_z_loss_coeff`` asks for it; ``training.py`` scales it by ``moe_loss_coeff``.  Expert weights are tagged ``expert_parallel`` so the optimizer reduces their gradients
 over the expert-data-parallel group only.
 """
 from __future__ import annotations
@@ -121,15 +122,28 @@ class Router(nn.Module):
         self.top_k = neox_args.moe_top_k
         self.jitter_eps = neox_args.moe_jitter_eps
         self.fp32 = neox_args.moe_lbl_in_fp32
+        if neox_args.moe_z_loss_coeff and not neox_args.moe_loss_coeff:
+            raise ValueError("moe_z_loss_coeff needs a moe_loss_coeff that is not zero: both losses travel as one")
+        self.z_share = neox_args.moe_z_loss_coeff / neox_args.moe_loss_coeff if neox_args.moe_z_loss_coeff else 0.0
 
     def forward(self, x):
         if self.training and self.jitter_eps:
             noise = torch.empty_like(x).uniform_(1.0 - self.jitter_eps, 1.0 + self.jitter_eps)
             x = x * noise
         logits = self.layer(x)
-        # router probabilities always in fp32 (``moe_lbl_in_fp32`` only matters for the statistics built from them);
-        # softmax, top-k, renormalisation and the expert histogram are one kernel on a GPU
-        return MO.router(logits, self.top_k)
+        # router probabilities always in fp32 (``moe_lbl_in_fp32`` only matters for the statistics built from them)
+        if MO.router_kernel_ok(logits, self.top_k):
+            # softmax, top-k, renormalisation, the expert histogram and both losses: two launches, one more for the gradient
+            out = MO.balanced_router(logits, self.top_k)
+            return out.weights, out.experts, out.counts, self._loss(out.balance, lambda: out.z)
+        probs, w, idx, counts = MO.router(logits, self.top_k)
+        f = counts.float() / float(idx.numel())
+        lbl = logits.shape[-1] * torch.sum(f.detach() * probs.mean(dim=0))
+        return w, idx, counts, self._loss(lbl, lambda: logits.float().logsumexp(-1).square().mean())
+
+    def _loss(self, balance, z):
+        """The layer's auxiliary loss: what ``moe_loss_coeff`` multiplies later, so the z loss enters in its units."""
+        return balance + self.z_share * z() if self.z_share else balance
 
 
 class ParallelMoE(nn.Module):
@@ -310,17 +324,13 @@ class ParallelMoE(nn.Module):
         shape = hidden_states.shape
         x = hidden_states.reshape(-1, shape[-1])
         T, E, k = x.shape[0], self.num_experts, self.top_k
-        probs, w, idx, counts = self.router(x)
+        w, idx, counts, lbl = self.router(x)
         if self.expert_tp:
             # the router runs replicated on the unsplit input; what enters the sharded experts is marked so that the
             # partial gradients of the expert input and of the gates are summed over the tensor-parallel group
             x = M.copy_to_model_parallel_region(x)
             w = M.copy_to_model_parallel_region(w)
-        # ---- load-balancing statistics
         flat_e = idx.reshape(-1)
-        f = counts.float() / float(T * k)
-        P = probs.mean(dim=0)
-        lbl = E * torch.sum(f.detach() * P)
         if self.ep == 1 and self._use_grouped(x):
             y = self._forward_grouped(x, w, idx, counts)
             return y.reshape(shape), lbl.to(hidden_states.dtype)

@@ -1,5 +1,5 @@
 """Training objectives beyond the plain LM loss: MoE load-balancing auxiliary loss, pairwise reward
-model, DPO, KTO and REINFORCE with KL variants.
+model, DPO, KTO, REINFORCE with KL variants and its clipped form for completions of an older policy.
 
 Definitions follow ``megatron/training.py:533-939`` of the reference; each objective is a function
 of (sharded) logits so it can be unit-tested against a dense restatement.
@@ -9,6 +9,8 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 
+from .ops.policy_losses import policy_loss, preference_loss
+from .ops.functional import _k
 from .parallel import mappings as M
 from .parallel.cross_entropy import vocab_parallel_cross_entropy
 
@@ -40,8 +42,37 @@ def reward_model_loss(values, loss_mask, z_loss=0.0):
     return loss, metrics
 
 
+def _dpo_kernels(policy_logits, labels, loss_mask, beta, ref_logits, ref_logp, reference_free):
+    """The same loss and metrics from the fused kernels, which read the logits in their own type (statistics in fp32, sums in fp64)
+    and skip masked positions; ``None`` where they do not take the arguments."""
+    x, n = policy_logits, policy_logits.shape[0]
+    if not _k(x) or x.dim() != 3 or n % 2 or n == 0 or labels.shape != x.shape[:2] or loss_mask.shape != x.shape[:2]:
+        return None
+    if reference_free:
+        ref_logits = ref_logp = None
+    elif ref_logp is not None:
+        ref_logits = None
+        if ref_logp.shape != labels.shape:
+            return None
+    elif ref_logits is None or ref_logits.shape != x.shape or ref_logits.dtype != x.dtype:
+        return None
+    const = lambda t: None if t is None else t.detach()                 # noqa: E731
+    out = preference_loss(x, labels, loss_mask.detach(), beta, ref_logits=const(ref_logits), ref_logp=const(ref_logp))
+    chosen_pos, chosen_neg = out.logp.detach().chunk(2)
+    metrics = {"chosen_neg": chosen_neg.mean(), "chosen_pos": chosen_pos.mean()}
+    if not reference_free:
+        ref_pos, ref_neg = out.ref_logp.chunk(2)
+        cr, rr = beta * (chosen_pos - ref_pos), beta * (chosen_neg - ref_neg)
+        metrics.update({"ref_neg": ref_neg.mean(), "ref_pos": ref_pos.mean(), "chosen_rewards": cr.mean(),
+                        "rejected_rewards": rr.mean(), "reward_acc": (cr > rr).float().mean(), "margins": (cr - rr).mean()})
+    return out.loss, metrics
+
+
 def dpo_loss(policy_logits, labels, loss_mask, beta, ref_logits=None, ref_logp=None, reference_free=False,
              fp32=True):
+    fused = _dpo_kernels(policy_logits, labels, loss_mask, beta, ref_logits, ref_logp, reference_free)
+    if fused is not None:
+        return fused
     pos_mask, neg_mask = torch.chunk(loss_mask, 2, 0)
     with torch.no_grad():
         if reference_free:
@@ -127,9 +158,27 @@ def reinforce_loss(policy_logits, labels, loss_mask, rewards, raw_rewards, kl_im
             kl = F.kl_div(ref_full, logp_full, log_target=True, reduction="none").sum(-1)
         else:
             kl = tok - ref_tok
-            kl = kl.abs() if kl_impl == "abs" else 0.5 * kl.square() if kl_impl == "mse" else kl
+            kl = kl.abs() if kl_impl == "abs" else 0.5 * kl.square() if kl_impl == "mse" \
+                else torch.expm1(-kl) + kl if kl_impl == "k3" else kl
         metrics["kl"] = kl.detach().mean()
         loss = -tok * rewards + kl_beta * kl
     else:
         loss = -(rewards * tok)
     return ((loss * loss_mask).sum(-1) / denom).mean(), metrics
+
+
+def clipped_reinforce_loss(policy_logits, labels, loss_mask, rewards, raw_rewards, old_logp, clip, clip_high=None, kl_impl="mse",
+                           kl_beta=0.1, ref_logits=None, sequence_mean=False):
+    """REINFORCE on completions that an older policy sampled: the ratio to the sampler's log-probabilities ``old_logp`` is clipped
+    to ``[1 - clip, 1 + clip_high]`` (``clip_high`` defaults to ``clip``).  ``kl_impl`` as in :func:`reinforce_loss`, and ``k3``:
+    ``exp(-d) - 1 + d`` with ``d`` the difference of the log-probabilities."""
+    out = policy_loss(policy_logits, labels, loss_mask, rewards, old_logp=old_logp,
+                      ref_logits=None if ref_logits is None else ref_logits.detach(), clip_low=clip, clip_high=clip_high,
+                      kl=kl_impl if ref_logits is not None else "k3", kl_beta=kl_beta,
+                      reduce="sequence" if sequence_mean else "token")
+    kept = loss_mask.sum().clamp(min=1)
+    metrics = {"logp": (out.logp * loss_mask).sum() / kept, "reward": raw_rewards.detach().mean(),
+               "reward_std": raw_rewards.detach().std(), "clipped": out.clipped}
+    if ref_logits is not None:
+        metrics["kl"] = out.kl
+    return out.loss, metrics

@@ -132,10 +132,16 @@ def get_batch(neox_args, data_iterator):
             ref_logp = broadcast_data(["ref"], data, torch.float)["ref"][:, :-1].contiguous()
         return tup + (rw, ref_logp)
     if impl == "reinforce":
-        tup = _get_batch(neox_args, neox_args.tokenizer, ["text"], data, dt, label_mask_zero=True)
+        clipped = neox_args.reinforce_clip is not None
+        # the clipped loss compares with the sampler's log-probabilities, which only the completion's tokens have
+        tup = _get_batch(neox_args, neox_args.tokenizer, ["text", "label"] if clipped else ["text"], data, dt,
+                         label_mask_zero=True)
         rws = broadcast_data(["reward", "raw_reward"], data, torch.float)
         rw = rws["reward"].unsqueeze(-1).expand(-1, tup[0].shape[1]) if rws["reward"].dim() == 1 \
             else rws["reward"][:, :-1].contiguous()
+        if clipped:
+            old = broadcast_data(["old_logp"], data, torch.float)["old_logp"][:, 1:].contiguous()
+            return tup + (rw, rws["raw_reward"], old)
         return tup + (rw, rws["raw_reward"])
     if impl in ("dpo", "rm"):
         pos_keys = ["pos", "pos_label"] if neox_args.pos_train_label_data_paths else ["pos"]
@@ -257,9 +263,15 @@ def forward_step(data_iterator, model, neox_args, timers, return_logits=False, i
                 with torch.no_grad():
                     ref_out, _ = _outputs(reference_model(fwd_in, neox_args=neox_args))
             outputs, _ = _outputs(model(fwd_in, neox_args=neox_args))
-            loss, metrics = OBJ.reinforce_loss(outputs, labels, loss_mask, rewards, raw_rewards, neox_args.kl_impl,
-                                               neox_args.kl_div_beta, ref_logits=ref_out,
-                                               fp32=neox_args.fp32_reinforce)
+            if neox_args.reinforce_clip is not None:
+                loss, metrics = OBJ.clipped_reinforce_loss(
+                    outputs, labels, loss_mask, rewards, raw_rewards, batch[7], neox_args.reinforce_clip,
+                    neox_args.reinforce_clip_high, neox_args.kl_impl, neox_args.kl_div_beta, ref_logits=ref_out,
+                    sequence_mean=neox_args.reinforce_sequence_mean)
+            else:
+                loss, metrics = OBJ.reinforce_loss(outputs, labels, loss_mask, rewards, raw_rewards, neox_args.kl_impl,
+                                                   neox_args.kl_div_beta, ref_logits=ref_out,
+                                                   fp32=neox_args.fp32_reinforce)
         else:
             raise ValueError(f"unknown train_impl {impl}")
     if return_logits:

@@ -7,6 +7,8 @@ sends the split name (``train`` / ``valid`` / ``test``) and reads until EOF one 
 
     {"prefix": [token ids], "completions": [[token ids], ...], "rewards": [float, ...]}
 
+(with ``--logprobs`` also ``"logprobs": [[float, ...], ...]``, which the trainer's ``reinforce_clip`` compares with),
+
 with ``--num-completions`` sampled continuations of one prompt.  The sampler keeps its weights current by asking the
 trainer's weight server (``gpt_neox_b200.weight_server``, port ``--weight-port`` + rank) for the CUDA IPC handles of
 the live parameters and re-binding them before every batch, so no checkpoint ever touches disk.
@@ -65,6 +67,17 @@ class Sampler:
                                       max_new_tokens=max_new_tokens, pad_token_id=self.tok.eos_token_id)
         return [o[len(prompt_ids):].tolist() for o in out]
 
+    def logprobs(self, prompt_ids, completions):
+        """Log-probability of every token of the completions under the current weights."""
+        import torch
+        got = []
+        for comp in completions:
+            ids = torch.tensor([list(prompt_ids) + list(comp)], device="cuda")
+            with torch.no_grad():
+                logp = self.model(ids).logits[0, len(prompt_ids) - 1:-1].float().log_softmax(-1)
+            got.append(logp.gather(1, ids[0, len(prompt_ids):, None])[:, 0].tolist())
+        return got
+
 
 def reward_fn(tok, completion):
     ends = len(completion) > 0 and completion[-1] == tok.eos_token_id
@@ -88,6 +101,8 @@ def serve(args):
             prefix = sampler.tok.apply_chat_template([{"role": "user", "content": text}], add_generation_prompt=True)
             comps = sampler.generate(prefix, args.num_completions, args.max_new_tokens)
             payload = {"prefix": prefix, "completions": comps, "rewards": [reward_fn(sampler.tok, c) for c in comps]}
+            if args.logprobs:
+                payload["logprobs"] = sampler.logprobs(prefix, comps)
             conn.sendall(pickle.dumps(payload))
         finally:
             conn.close()
@@ -101,4 +116,5 @@ if __name__ == "__main__":
     ap.add_argument("--prompts", default=None, help="text file with one prompt per line")
     ap.add_argument("--num-completions", type=int, default=4)
     ap.add_argument("--max-new-tokens", type=int, default=256)
+    ap.add_argument("--logprobs", action="store_true", help="send the tokens' log-probabilities (reinforce_clip)")
     serve(ap.parse_args())

@@ -456,3 +456,53 @@ def test_balanced_router_of_extreme_logits():
     assert bool(torch.isfinite(out.balance))
     none = MO.balanced_router(x, 4, token_mask=torch.zeros_like(keep))
     assert float(none.balance) == 0.0 and float(none.z) == 0.0 and torch.equal(none.counts, out.counts)
+
+
+# ---------------------------------------------------------------------------------------------- together, as they are used
+def test_expert_model_trains_on_preferences_with_its_router_losses():
+    """Router, experts and head, and on their logits the preference loss, a clipped policy loss, balance and z loss, as one objective:
+    loss and all gradients against the same model of plain statements in 64 bits.  Everything is in 32 bits; products of up to 64
+    terms, four in a row, stay within 2^-13 of the largest gradient."""
+    torch.manual_seed(0)
+    n, s, h, experts, v = 4, 33, 64, 8, 1003
+    hidden = torch.randn(n * s, h, device=DEV)
+    params = [torch.randn(experts, h, device=DEV) * 0.3, torch.randn(experts, h, h, device=DEV) / 8, torch.randn(v, h, device=DEV) / 8]
+    labels, mask = torch.randint(0, v, (n, s), device=DEV), _mask(n, s, 3)
+    old, adv = -torch.rand(n, s, device=DEV) - 6, torch.randn(n, device=DEV)
+    tokens = mask.reshape(-1) != 0
+
+    def objective(wr, we, wv, x, mask, old, adv, kernels):
+        logits = x @ wr.t()
+        route = MO.balanced_router(logits, 2, token_mask=tokens) if kernels else MO.balanced_router_ref(logits, 2, tokens)
+        picked = torch.einsum("th,tkgh->tkg", x, we[route.experts]).tanh()
+        out = (picked * route.weights.to(x.dtype)[..., None]).sum(1)
+        words = (out @ wv.t()).view(n, s, v)
+        prefer, policy = (PL.preference_loss, PL.policy_loss) if kernels else (PL.preference_loss_ref, PL.policy_loss_ref)
+        a = prefer(words, labels, mask, 0.1)
+        b = policy(words, labels, mask, adv, old_logp=old, ref_logits=words.detach() * 0.9, kl="full", kl_beta=0.1)
+        return a.loss - 0.01 * a.logp.mean() + b.loss + 0.01 * route.balance + 1e-3 * route.z
+
+    def run(dtype, kernels):
+        w = [p.to(dtype).requires_grad_() for p in params]
+        loss = objective(*w, *(t.to(dtype) for t in (hidden, mask, old, adv)), kernels)
+        return [loss.detach()] + list(torch.autograd.grad(loss, w))
+    tf32 = torch.backends.cuda.matmul.allow_tf32
+    torch.backends.cuda.matmul.allow_tf32 = False
+    try:
+        got, want = run(torch.float32, True), run(torch.float64, False)
+    finally:
+        torch.backends.cuda.matmul.allow_tf32 = tf32
+    for a, b in zip(got, want):
+        _near(a, b, 2.0 ** -13 * b.abs().max(), "loss and gradients")
+
+
+@pytest.mark.parametrize("kind", ["dpo", "clipped", "moe"])
+def test_post_training_steps_on_a_gpu(kind):
+    import os
+    import subprocess
+    import sys
+    from common import ROOT, free_port
+    env = dict(os.environ, MASTER_ADDR="127.0.0.1", MASTER_PORT=str(free_port()), WORLD_SIZE="1", RANK="0", LOCAL_RANK="0")
+    r = subprocess.run([sys.executable, os.path.join(ROOT, "tests", "workers", "post_training_worker.py"), kind], env=env,
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "POST_TRAINING_OK" in r.stdout, (r.stdout + r.stderr)[-4000:]
