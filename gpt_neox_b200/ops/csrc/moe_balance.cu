@@ -31,26 +31,34 @@ __device__ __forceinline__ void put(float& d, float v) { d = v; }
 __device__ __forceinline__ void put(__nv_bfloat16& d, float v) { d = __float2bfloat16(v); }
 __device__ __forceinline__ void put(__half& d, float v) { d = __float2half(v); }
 
-// Eight neighbouring elements of a row; `aligned`: rows start on 16 bytes and have no part of eight left over.
-template <typename T> __device__ __forceinline__ void load_8(const T* p, int left, bool aligned, float (&v)[8]) {
-    if (aligned) {
-        __align__(16) T t[8];
-        const uint4* q = reinterpret_cast<const uint4*>(p);
-        uint4* d = reinterpret_cast<uint4*>(t);
-        if (left > 0) {
-            d[0] = __ldg(q);
-            if constexpr (sizeof(T) == 4) d[1] = __ldg(q + 1);
+// Eight neighbouring elements of a row as they lie in memory, -inf where the row has ended; `aligned`: rows start on 16 bytes and
+// have no part of eight left over.
+template <typename T> struct Eight {
+    static constexpr int WORDS = sizeof(T) / 2;                 // of 16 bytes
+    uint4 w[WORDS];
+    __device__ __forceinline__ void load(const T* p, int left, bool aligned) {
+        if (aligned && left > 0) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = to_f(t[i]);
+            for (int i = 0; i < WORDS; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
         } else {
+            __align__(16) T t[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = -INFINITY;
+            for (int i = 0; i < 8; ++i) {
+                put(t[i], -INFINITY);
+                if (i < left) t[i] = p[i];
+            }
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) w[i] = reinterpret_cast<const uint4*>(t)[i];
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < left ? to_f(p[i]) : -INFINITY;
     }
-}
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        __align__(16) T t[8];
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) reinterpret_cast<uint4*>(t)[i] = w[i];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_f(t[i]);
+    }
+};
 template <typename T> __device__ __forceinline__ void store_8(T* p, int left, bool aligned, const float (&v)[8]) {
     if (aligned) {
         __align__(16) T t[8];
@@ -74,41 +82,53 @@ template <int LANES> __device__ __forceinline__ float group_sum(float v) {
     return v;
 }
 
-// Order of the choice in one number: the value's bits in an order that grows with the value, -0 as 0 and NaN above all, then
-// the lower index.  Sixteen-bit values leave room for both in 32 bits.
+// Order of the choice in one number: the bits of the value as a 32-bit float, turned so that they grow with it, -0 as 0 and NaN
+// above all, then the lower index.  A 16-bit value leaves at least 13 of its 32 bits free for the index.
+__device__ __forceinline__ uint32_t rising(float v) {
+    float w;
+    asm("add.rn.f32 %0, %1, 0f00000000;" : "=f"(w) : "f"(v));   // -0 becomes 0, NaN the one of sign 0; subnormal numbers stay
+    const uint32_t u = __float_as_uint(w);
+    return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float unrisen(uint32_t t) {
+    return __uint_as_float(t & 0x80000000u ? t ^ 0x80000000u : ~t);
+}
 template <typename T> struct Key {
     using type = uint32_t;
-    static __device__ __forceinline__ uint32_t of(float v, int e) {
-        T t;
-        put(t, v);                                              // exact: v was one
-        uint32_t b = *reinterpret_cast<const uint16_t*>(&t);
-        if (b == 0x8000u) b = 0;
-        if (v != v) b = 0x7fffu;
-        b = b & 0x8000u ? 0xffffu - b : b | 0x8000u;
-        return b << 16 | (uint32_t)(0xffff - e);
-    }
-    static __device__ __forceinline__ int expert(uint32_t k) { return 0xffff - (int)(k & 0xffffu); }
-    static __device__ __forceinline__ float value(uint32_t k) {
-        uint32_t b = k >> 16;
-        const uint16_t s = (uint16_t)(b & 0x8000u ? b & 0x7fffu : 0xffffu - b);
-        return to_f(*reinterpret_cast<const T*>(&s));
-    }
+    static constexpr uint32_t FREE = 0x1fff;
+    static __device__ __forceinline__ uint32_t of(float v, int e) { return (rising(v) & ~FREE) | (FREE - e); }
+    static __device__ __forceinline__ int expert(uint32_t k) { return (int)(FREE - (k & FREE)); }
+    // of a negative value the turned bits are ones where the value's are zeros
+    static __device__ __forceinline__ float value(uint32_t k) { return unrisen(k & 0x80000000u ? k & ~FREE : k | FREE); }
 };
 template <> struct Key<float> {
     using type = unsigned long long;
     static __device__ __forceinline__ unsigned long long of(float v, int e) {
-        uint32_t b = __float_as_uint(v);
-        if (b == 0x80000000u) b = 0;
-        if (v != v) b = 0x7fffffffu;
-        b = b & 0x80000000u ? ~b : b | 0x80000000u;
-        return (unsigned long long)b << 32 | (uint32_t)(0xffff - e);
+        return (unsigned long long)rising(v) << 32 | (uint32_t)(0xffff - e);
     }
     static __device__ __forceinline__ int expert(unsigned long long k) { return 0xffff - (int)(k & 0xffffu); }
-    static __device__ __forceinline__ float value(unsigned long long k) {
-        const uint32_t b = (uint32_t)(k >> 32);
-        return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
-    }
+    static __device__ __forceinline__ float value(unsigned long long k) { return unrisen((uint32_t)(k >> 32)); }
 };
+
+// Eight numbers in falling order: Batcher's odd-even merge of sorted halves, and the merge of a bitonic sequence.
+template <typename K> __device__ __forceinline__ void order(K& a, K& b) {
+    const K low = min(a, b);
+    a = max(a, b);
+    b = low;
+}
+template <typename K> __device__ __forceinline__ void sort_8(K (&v)[8]) {
+    order(v[0], v[1]); order(v[2], v[3]); order(v[4], v[5]); order(v[6], v[7]);
+    order(v[0], v[2]); order(v[1], v[3]); order(v[4], v[6]); order(v[5], v[7]);
+    order(v[1], v[2]); order(v[5], v[6]);
+    order(v[0], v[4]); order(v[1], v[5]); order(v[2], v[6]); order(v[3], v[7]);
+    order(v[2], v[4]); order(v[3], v[5]);
+    order(v[1], v[2]); order(v[3], v[4]); order(v[5], v[6]);
+}
+template <typename K> __device__ __forceinline__ void merge_8(K (&v)[8]) {
+    order(v[0], v[4]); order(v[1], v[5]); order(v[2], v[6]); order(v[3], v[7]);
+    order(v[0], v[2]); order(v[1], v[3]); order(v[4], v[6]); order(v[5], v[7]);
+    order(v[0], v[1]); order(v[2], v[3]); order(v[4], v[5]); order(v[6], v[7]);
+}
 
 struct ForwardArgs {
     const void* x;
@@ -124,7 +144,12 @@ struct ForwardArgs {
     int tokens, E, k, aligned;
 };
 
-template <typename T, int LANES, int C>
+// Many tokens: one block an SM, as large as registers allow, since few threads read again what the blocks leave (32768 tokens of
+// 128 experts, both kernels: 24.6 us with four blocks of 256 threads an SM, 18.3 us so).  Few: small blocks (16 tokens of 64
+// experts: 6.4 against 8.1 us).
+template <typename T, int C> constexpr int LARGE = sizeof(T) == 2 && C == 1 ? 1024 : 512;
+
+template <typename T, int LANES, int C, int THREADS>
 __global__ void __launch_bounds__(THREADS) router_kernel(const ForwardArgs a) {
     constexpr int GROUPS = THREADS / LANES, WARPS = THREADS / 32, SLOTS = LANES * C * 8;
     using K = Key<T>;
@@ -136,45 +161,57 @@ __global__ void __launch_bounds__(THREADS) router_kernel(const ForwardArgs a) {
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0;
     for (int e = threadIdx.x; e < SLOTS; e += THREADS) hits[0][e] = hits[1][e] = 0;
     __syncthreads();
+    constexpr int MINE = (MAX_K + LANES - 1) / LANES;           // choices a lane writes: every LANES-th
     float col[C][8] = {};
-    double z = 0.0;
-    // whole warps walk together: a group past the last token does the last one's work again and leaves nothing
-    for (int first = blockIdx.x * GROUPS; first < a.tokens; first += gridDim.x * GROUPS) {
-        const bool here = first + group < a.tokens;
-        const int t = here ? first + group : a.tokens - 1;
+    float z = 0.f;
+    Eight<T> next[C];
+    bool next_kept = false;
+    auto fetch = [&](int first) {
+        const int t = min(first + group, a.tokens - 1);
         const T* x = reinterpret_cast<const T*>(a.x) + (long long)t * a.stride;
+#pragma unroll
+        for (int c = 0; c < C; ++c) next[c].load(x + (c * LANES + lane) * 8, a.E - (c * LANES + lane) * 8, a.aligned);
+        next_kept = first + group < a.tokens && (!a.kept || a.kept[t]);
+    };
+    // whole warps walk together: a group past the last token does the last one's work again and leaves nothing
+    if (blockIdx.x * GROUPS < a.tokens) fetch(blockIdx.x * GROUPS);
+    for (int first = blockIdx.x * GROUPS; first < a.tokens; first += gridDim.x * GROUPS) {
+        const bool here = first + group < a.tokens, kept = next_kept;
+        const int t = here ? first + group : a.tokens - 1;
         float v[C][8];
         KeyT key[C][8];
 #pragma unroll
+        for (int c = 0; c < C; ++c) next[c].get(v[c]);
+        if (first + (int)gridDim.x * GROUPS < a.tokens) fetch(first + gridDim.x * GROUPS);
+#pragma unroll
         for (int c = 0; c < C; ++c) {
             const int e0 = (c * LANES + lane) * 8;
-            load_8(x + e0, a.E - e0, a.aligned, v[c]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) key[c][i] = e0 + i < a.E ? K::of(v[c][i], e0 + i) : 0;
+            sort_8(key[c]);
         }
-        const bool kept = here && (!a.kept || a.kept[t]);
-        KeyT picked[MAX_K];
+        if constexpr (C == 2) {                                 // the eight largest of both
+#pragma unroll
+            for (int i = 0; i < 8; ++i) key[0][i] = max(key[0][i], key[1][7 - i]);
+            merge_8(key[0]);
+        }
+        KeyT mine[MINE] = {}, top = 0;
 #pragma unroll
         for (int j = 0; j < MAX_K; ++j) {
             if (j >= a.k) break;
-            KeyT best = 0;
-#pragma unroll
-            for (int c = 0; c < C; ++c)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) best = key[c][i] > best ? key[c][i] : best;
+            KeyT best = key[0][0];                              // the lanes' lists are in order: only their heads compete
 #pragma unroll
             for (int o = LANES / 2; o > 0; o >>= 1) {
                 const KeyT other = __shfl_xor_sync(ALL, best, o);
-                best = other > best ? other : best;
+                best = max(best, other);
             }
-            picked[j] = best;
+            if (j == 0) top = best;
+            if (j % LANES == lane) mine[j / LANES] = best;
+            const bool won = key[0][0] == best;
 #pragma unroll
-            for (int c = 0; c < C; ++c)
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (key[c][i] == best) key[c][i] = 0;
+            for (int i = 0; i + 1 < MAX_K - j; ++i) key[0][i] = won ? key[0][i + 1] : key[0][i];
         }
-        const float m = fmaxf(K::value(picked[0]), -FLT_MAX);
+        const float m = fmaxf(K::value(top), -FLT_MAX);
         float sum = 0.f;
 #pragma unroll
         for (int c = 0; c < C; ++c)
@@ -183,30 +220,35 @@ __global__ void __launch_bounds__(THREADS) router_kernel(const ForwardArgs a) {
                 v[c][i] = __expf(v[c][i] - m);
                 sum += v[c][i];
             }
+        float picked[MINE], mass = 0.f;
+#pragma unroll
+        for (int q = 0; q < MINE; ++q) {
+            picked[q] = q * LANES + lane < a.k ? __expf(K::value(mine[q]) - m) : 0.f;
+            mass += picked[q];
+        }
         sum = group_sum<LANES>(sum);
+        mass = group_sum<LANES>(mass);
         const float inv = __frcp_rn(sum);
         if (kept)
 #pragma unroll
             for (int c = 0; c < C; ++c)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) col[c][i] += v[c][i] * inv;
-        float mass = 0.f;
-#pragma unroll
-        for (int j = 0; j < MAX_K; ++j)
-            if (j < a.k) mass += __expf(K::value(picked[j]) - m);
         const float norm = a.k > 1 ? __frcp_rn(mass) : inv;
 #pragma unroll
-        for (int j = 0; j < MAX_K; ++j)
-            if (here && j < a.k && j % LANES == lane) {
-                const int e = K::expert(picked[j]);
-                a.weights[(long long)t * a.k + j] = __expf(K::value(picked[j]) - m) * norm;
+        for (int q = 0; q < MINE; ++q) {
+            const int j = q * LANES + lane;
+            if (here && j < a.k) {
+                const int e = K::expert(mine[q]);
+                a.weights[(long long)t * a.k + j] = picked[q] * norm;
                 a.experts[(long long)t * a.k + j] = e;
                 atomicAdd(&hits[0][e], 1);
                 if (kept) atomicAdd(&hits[1][e], 1);
             }
+        }
         if (here && lane == 0) {
-            const double lse = (double)m + log((double)sum);
-            a.row[t] = make_float4(m, inv, mass * inv, (float)lse);
+            const float lse = m + __logf(sum);
+            a.row[t] = make_float4(m, inv, mass * inv, lse);
             if (kept) z += lse * lse;
         }
     }
@@ -220,9 +262,10 @@ __global__ void __launch_bounds__(THREADS) router_kernel(const ForwardArgs a) {
             for (int o = 16; o >= LANES; o >>= 1) s += __shfl_xor_sync(ALL, s, o);
             if ((threadIdx.x & 31) < LANES) cols[warp][(c * LANES + lane) * 8 + i] = s;
         }
+    double zw = z;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(ALL, z, o);
-    if ((threadIdx.x & 31) == 0) zs[warp] = z;
+    for (int o = 16; o > 0; o >>= 1) zw += __shfl_xor_sync(ALL, zw, o);
+    if ((threadIdx.x & 31) == 0) zs[warp] = zw;
     __syncthreads();
     for (int e = threadIdx.x; e < a.E; e += THREADS) {
         float s = 0.f;
@@ -257,12 +300,15 @@ struct LossArgs {
 __global__ void __launch_bounds__(1024) router_loss_kernel(const LossArgs a) {
     __shared__ double p[32][33];
     __shared__ int n_all[32][33], n_kept[32][33];
+    __shared__ double dots[32];
+    __shared__ int n_sum[32];
     __shared__ int last;
     launch::wait_for_predecessor();
     const int x = threadIdx.x & 31, y = threadIdx.x >> 5, e = blockIdx.x * 32 + x;
     double s = 0.0;
     int all = 0, kept = 0;
     if (e < a.E)
+#pragma unroll 5
         for (int b = y; b < a.blocks; b += 32) {
             s += a.sums[(long long)b * a.E + e];
             all += a.chosen[(2ll * b) * a.E + e];
@@ -272,17 +318,23 @@ __global__ void __launch_bounds__(1024) router_loss_kernel(const LossArgs a) {
     n_all[x][y] = all;
     n_kept[x][y] = kept;
     __syncthreads();
+    s = p[y][x];                                                // a warp an expert now
+    all = __reduce_add_sync(ALL, n_all[y][x]);
+    kept = __reduce_add_sync(ALL, n_kept[y][x]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(ALL, s, o);
+    const int mine = blockIdx.x * 32 + y;
+    if (x == 0) {
+        if (mine < a.E) {
+            a.counts[mine] = all;
+            a.load[mine] = (float)kept;
+        }
+        dots[y] = s * kept;
+        n_sum[y] = kept;
+    }
+    __syncthreads();
     if (y == 0) {
-        for (int w = 1; w < 32; ++w) {
-            s += p[x][w];
-            all += n_all[x][w];
-            kept += n_kept[x][w];
-        }
-        if (e < a.E) {
-            a.counts[e] = all;
-            a.load[e] = (float)kept;
-        }
-        double dot = s * kept, n = kept;
+        double dot = dots[x], n = n_sum[x];
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             dot += __shfl_xor_sync(ALL, dot, o);
@@ -292,7 +344,7 @@ __global__ void __launch_bounds__(1024) router_loss_kernel(const LossArgs a) {
             a.part[2 * blockIdx.x] = dot;
             a.part[2 * blockIdx.x + 1] = n;
             __threadfence();
-            last = atomicAdd(a.ticket, 1) == (int)gridDim.x - 1;
+            last = gridDim.x == 1 || atomicAdd(a.ticket, 1) == (int)gridDim.x - 1;
             __threadfence();
         }
     }
@@ -335,7 +387,8 @@ struct BackwardArgs {
 
 template <typename T, int LANES, int C>
 __global__ void __launch_bounds__(THREADS) router_grad_kernel(const BackwardArgs a) {
-    constexpr int GROUPS = THREADS / LANES;
+    constexpr int GROUPS = THREADS / LANES, MINE = (MAX_K + LANES - 1) / LANES;
+    __shared__ __align__(16) float toward[GROUPS][LANES * C * 8];
     const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
     const float per_token = a.load[a.E];
     // E f_e / N g = E count_e / (N k) / N g
@@ -359,7 +412,9 @@ __global__ void __launch_bounds__(THREADS) router_grad_kernel(const BackwardArgs
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int e0 = (c * LANES + lane) * 8;
-            load_8(x + e0, a.E - e0, a.aligned, p[c]);
+            Eight<T> raw;
+            raw.load(x + e0, a.E - e0, a.aligned);
+            raw.get(p[c]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 p[c][i] = __expf(p[c][i] - r.x) * r.y;
@@ -367,22 +422,36 @@ __global__ void __launch_bounds__(THREADS) router_grad_kernel(const BackwardArgs
             }
         }
         if (a.g_weights) {
-            const float* gw = a.g_weights + (long long)t * a.k;
-            float dot = 0.f, inv = 1.f;
-            if (a.k > 1) {
-                const float* w = a.weights + (long long)t * a.k;
-                for (int j = 0; j < a.k; ++j) dot += gw[j] * w[j];
-                inv = __frcp_rn(r.z);
-            }
-            for (int j = 0; j < a.k; ++j) {
-                const int e = (int)a.experts[(long long)t * a.k + j];
-                const float g = (gw[j] - dot) * inv;
+            // a lane forms the gradient at every LANES-th choice and leaves it where the expert's lane picks it up
+            const long long at = (long long)t * a.k;
+            float g[MINE], dot = 0.f;
 #pragma unroll
-                for (int c = 0; c < C; ++c)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (e == (c * LANES + lane) * 8 + i) dp[c][i] += g;
+            for (int q = 0; q < MINE; ++q) {
+                const int j = q * LANES + lane;
+                g[q] = j < a.k ? a.g_weights[at + j] : 0.f;
+                if (a.k > 1 && j < a.k) dot += g[q] * a.weights[at + j];
             }
+            dot = group_sum<LANES>(dot);
+            const float inv = a.k > 1 ? __frcp_rn(r.z) : 1.f;
+            float4* clear = reinterpret_cast<float4*>(toward[group]);
+#pragma unroll
+            for (int c = 0; c < 2 * C; ++c) clear[c * LANES + lane] = make_float4(0.f, 0.f, 0.f, 0.f);
+            __syncwarp();
+#pragma unroll
+            for (int q = 0; q < MINE; ++q) {
+                const int j = q * LANES + lane;
+                if (j < a.k) toward[group][(int)a.experts[at + j]] = (g[q] - dot) * inv;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const float4* from = reinterpret_cast<const float4*>(&toward[group][(c * LANES + lane) * 8]);
+                const float4 lo = from[0], hi = from[1];
+                const float add[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) dp[c][i] += add[i];
+            }
+            __syncwarp();
         }
         float inner = 0.f;
 #pragma unroll
@@ -408,13 +477,18 @@ int lanes_for(int E) {
     return l;
 }
 
-// Blocks of the forward: four an SM keep the loads of a token's rows in flight; a block walks over several tokens once there
-// are more, so that what it leaves to join stays small.
-int router_blocks(long long tokens, int E) {
-    const long long groups = THREADS / lanes_for(E);
-    const long long need = (tokens + groups - 1) / groups, most = 4ll * neox_sm_count();
-    return (int)(need < 1 ? 1 : need < most ? need : most);
-}
+struct RouterPlan {
+    bool large;
+    int blocks;
+    RouterPlan(long long tokens, int E, int dtype) {
+        const int lanes = lanes_for(E);
+        const long long sms = neox_sm_count(), small_groups = THREADS / lanes;
+        const long long large_groups = (dtype != 1 && E <= 256 ? LARGE<__half, 1> : LARGE<__half, 2>) / lanes;
+        large = (tokens + small_groups - 1) / small_groups > sms;
+        const long long groups = large ? large_groups : small_groups, need = (tokens + groups - 1) / groups;
+        blocks = (int)(need < 1 ? 1 : need < sms ? need : sms);
+    }
+};
 
 #define FOR_TYPE(dtype, CALL)                                  \
     do {                                                       \
@@ -446,13 +520,14 @@ int launched() { return cudaGetLastError() == cudaSuccess ? 0 : NEOX_ERR_LAUNCH;
 extern "C" {
 
 // Blocks whose sums the forward leaves: `scratch` holds this * (E * 12 + 8) bytes, then 16 * 17 and 16 more.
-int neox_router_blocks(long long tokens, int E) { return router_blocks(tokens, E); }
+int neox_router_blocks(long long tokens, int E, int dtype) { return RouterPlan(tokens, E, dtype).blocks; }
 
 int neox_balanced_router(const void* x, long long stride, const void* kept, int tokens, int E, int k, int dtype, float* weights,
                          long long* experts, void* row, long long* counts, float* load, float* balance, float* z_loss, void* scratch,
                          void* stream) {
     if (tokens < 0 || E < 1 || E > 512 || k < 1 || k > MAX_K || k > E) return NEOX_ERR_SHAPE;
-    const int blocks = router_blocks(tokens, E);
+    const RouterPlan plan(tokens, E, dtype);
+    const int blocks = plan.blocks;
     double* z = (double*)scratch;
     double* part = z + blocks;                                  // 16 blocks of 32 experts at most
     int* ticket = (int*)(part + 2 * 17);
@@ -462,7 +537,8 @@ int neox_balanced_router(const void* x, long long stride, const void* kept, int 
                            rows_aligned(x, stride, E, dtype)};
     const LossArgs l = {sums, chosen, z, ticket, part, counts, load, balance, z_loss, blocks, E, k};
     cudaStream_t st = (cudaStream_t)stream;
-    FOR_TYPE(dtype, FOR_LANES(E, (router_kernel<T, L, C><<<blocks, THREADS, 0, st>>>(f))));
+    if (plan.large) FOR_TYPE(dtype, FOR_LANES(E, (router_kernel<T, L, C, LARGE<T, C>><<<blocks, LARGE<T, C>, 0, st>>>(f))));
+    else FOR_TYPE(dtype, FOR_LANES(E, (router_kernel<T, L, C, THREADS><<<blocks, THREADS, 0, st>>>(f))));
     if (launched() != 0) return NEOX_ERR_LAUNCH;
     return launch::overlapped(router_loss_kernel, dim3((E + 31) / 32), dim3(1024), 1, st, l);
 }

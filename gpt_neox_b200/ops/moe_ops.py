@@ -29,7 +29,7 @@ PAD = 64
 
 _P, _I, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
 native._ARGTYPES.update({
-    "neox_router_blocks": [_L, _I],
+    "neox_router_blocks": [_L, _I, _I],
     "neox_balanced_router": [_P, _L, _P, _I, _I, _I, _I, *[_P] * 9],
     "neox_balanced_router_grad": [_P, _L, _P, _I, _I, _I, _I, *[_P] * 9],
 })
@@ -126,11 +126,11 @@ def balanced_router_ref(logits, k, token_mask=None):
 
 
 @functools.lru_cache(maxsize=256)
-def _router_layout(tokens, experts, device):
+def _router_layout(tokens, experts, dtype, device):
     """Floats of one forward's buffer: ``[E + 1]`` loads (an even number), ``[T, 4]`` row statistics -- kept for the backward -- and
     the scratch that the kernels' blocks leave their sums in."""
     load, row = (experts + 4) // 4 * 4, 4 * tokens
-    blocks = native.lib().neox_router_blocks(tokens, experts)
+    blocks = native.lib().neox_router_blocks(tokens, experts, dtype)
     return load, load + row, load + row + (blocks * (experts * 12 + 8) + 16 * 17 + 16 + 3) // 4
 
 
@@ -142,7 +142,7 @@ def _balanced_values(x, k, kept):
     counts = torch.empty(E, dtype=torch.int64, device=dev)
     balance = torch.empty((), dtype=torch.float32, device=dev)
     z = torch.empty((), dtype=torch.float32, device=dev)
-    row, scratch, total = _router_layout(T, E, x.get_device())
+    row, scratch, total = _router_layout(T, E, _DT[x.dtype], x.get_device())
     buf = torch.empty(total, dtype=torch.float32, device=dev)
     load = buf.data_ptr()
     rc = native.lib().neox_balanced_router(x.data_ptr(), x.stride(0), None if kept is None else kept.data_ptr(), T, E, k,
@@ -176,7 +176,7 @@ class _BalancedRouterFn(torch.autograd.Function):
         with device_of(x):
             rc = native.lib().neox_balanced_router_grad(
                 x.data_ptr(), x.stride(0), None if kept is None else kept.data_ptr(), T, E, ctx.k, _DT[x.dtype],
-                weights.data_ptr(), experts.data_ptr(), load + 4 * _router_layout(T, E, x.get_device())[0], load,
+                weights.data_ptr(), experts.data_ptr(), load + 4 * _router_layout(T, E, _DT[x.dtype], x.get_device())[0], load,
                 None if gw is None else gw.data_ptr(), None if gb is None else gb.data_ptr(),
                 None if gz is None else gz.data_ptr(), dx.data_ptr(), native.stream_ptr())
         native.check(rc, "neox_balanced_router_grad")
