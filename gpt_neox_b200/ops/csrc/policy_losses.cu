@@ -229,13 +229,11 @@ struct StatsArgs {
     int chunks, most;              // of a row: as many as suit a batch that keeps everything, and the most there is room for
 };
 
-// Into how many chunks each of `rows` rows is cut.  A chunk's end costs a warp about what PER_CHUNK further elements do; a warp
-// that is left alone with its last chunk works about four times as fast as one among many.
-constexpr int PER_CHUNK = 1280;
-__host__ __device__ __forceinline__ float cut_cost(long long rows, int vocab, int chunks, int blocks, int warps) {
-    const long long block = (rows * chunks + blocks - 1) / blocks;
-    const float size = (float)((vocab + chunks - 1) / chunks), each = (float)block / (float)warps;
-    return fmaxf(each, 0.25f) * (size + PER_CHUNK) + 0.25f * size;
+// Into how many chunks each of `rows` rows is cut, by the time of the busiest warp in steps of its loads: its chunks, each with an
+// end that costs about 0.4 steps, and at the end one that is left alone, where a step takes 0.3 of what it takes among many.
+__host__ __device__ __forceinline__ float cut_cost(long long rows, int vocab, int chunks, int warps, int step) {
+    const float steps = (float)vocab / ((float)chunks * (float)step), each = (float)rows * (float)chunks / (float)warps;
+    return fmaxf(each, 1.f) * (steps + 0.4f) + 0.3f * (ceilf(steps) + 0.4f);
 }
 // Elements of a chunk; the count that goes with it is at most `chunks`.
 __host__ __device__ __forceinline__ int chunk_size(int vocab, int chunks) { return ((vocab + chunks - 1) / chunks + 7) / 8 * 8; }
@@ -421,7 +419,7 @@ __global__ void __launch_bounds__(Shape<FULL>::WARPS * 32, 1) stats_kernel(const
             float best = INFINITY;
             chunks = 1;
             for (int c = 1 + lane; c <= a.most; c += 32) {
-                const float cost = cut_cost((long long)kept * a.streams, a.vocab, c, gridDim.x, WARPS);
+                const float cost = cut_cost((long long)kept * a.streams, a.vocab, c, gridDim.x * WARPS, W::STEP * N);
                 if (cost < best) {
                     best = cost;
                     chunks = c;
@@ -436,8 +434,8 @@ __global__ void __launch_bounds__(Shape<FULL>::WARPS * 32, 1) stats_kernel(const
             a.ticket[0] = 0;
             a.ticket[1] = chunks;
         }
-        const long long items = (long long)kept * a.streams * chunks;
-        const int lo = (int)(items * blockIdx.x / gridDim.x), hi = (int)(items * (blockIdx.x + 1) / gridDim.x);
+        const int items = kept * a.streams * chunks, share = items / (int)gridDim.x, more = items - share * (int)gridDim.x;
+        const int lo = (int)blockIdx.x * share + min((int)blockIdx.x, more), hi = lo + share + ((int)blockIdx.x < more);
         const int first = lo / chunks, end = (hi + chunks - 1) / chunks;
         for (int k = 0; k < a.streams; ++k) {                   // the second stream's rows follow the first's
             int rank = before + k * kept;
@@ -559,6 +557,7 @@ __global__ void __launch_bounds__(Shape<FULL>::WARPS * 32, 1) stats_kernel(const
 // ---------------------------------------------------------------------------------------------- from rows to the loss
 constexpr int LANES = 8;                                        // lanes that join a row's chunks
 constexpr int ROWS = THREADS / LANES;                           // rows of a block
+constexpr int NEAR = 256;                                       // sequences whose sums stay in shared memory
 
 struct RowSums {
     const float2* part;
@@ -575,24 +574,29 @@ template <typename V> __device__ __forceinline__ V lanes_sum(V v) {
     for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
+// A lane's first chunk of a row, asked for before it is known how many there are.
+__device__ __forceinline__ float2 peek(const RowSums& r, int stream, int row, bool on) {
+    const int lane = threadIdx.x % LANES;
+    return on && lane < r.most ? r.part[((long long)stream * r.rows + row) * r.most + lane] : make_float2(-FLT_MAX, 0.f);
+}
 // Joins a row's chunks: maximum and sum, in 64 bits.  All lanes of a warp come here, each with its row.
-__device__ __forceinline__ void join(const RowSums& r, int chunks, int stream, int row, bool on, float& m, double& t) {
+__device__ __forceinline__ void join(const RowSums& r, int chunks, int stream, int row, bool on, float2 own, float& m, double& t) {
     const int lane = threadIdx.x % LANES;
     const float2* p = r.part + ((long long)stream * r.rows + row) * r.most;
-    m = -FLT_MAX;
+    if (lane >= chunks) own = make_float2(-FLT_MAX, 0.f);
+    m = own.x;
     if (on)
-        for (int k = lane; k < chunks; k += LANES) m = fmaxf(m, p[k].x);
+        for (int k = lane + LANES; k < chunks; k += LANES) m = fmaxf(m, p[k].x);
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    t = 0.0;
+    t = (double)own.y * (double)__expf(own.x - m);
     if (on)
-        for (int k = lane; k < chunks; k += LANES) t += (double)p[k].y * (double)__expf(p[k].x - m);
+        for (int k = lane + LANES; k < chunks; k += LANES) t += (double)p[k].y * (double)__expf(p[k].x - m);
     t = lanes_sum(t);
 }
-__device__ __forceinline__ double label_logp(const RowSums& r, int which, int row, float m, double t) {
-    const long long y = r.labels[row];
-    if (y < 0 || y >= r.vocab) return nan("");
-    return ((double)r.target[(long long)which * r.rows + row] - (double)m) - log(t);
+// Log-probability of a label whose logit is x.
+__device__ __forceinline__ double label_logp(const RowSums& r, long long label, float x, float m, double t) {
+    return label < 0 || label >= r.vocab ? nan("") : ((double)x - (double)m) - log(t);
 }
 
 // Sums of V values over the block, in a fixed order; the result is in thread 0.
@@ -645,19 +649,24 @@ __global__ void __launch_bounds__(THREADS) preference_kernel(const PreferenceArg
     const int seq = blockIdx.x / a.pieces, j = (blockIdx.x % a.pieces) * ROWS + threadIdx.x / LANES;
     const int row = seq * a.s + j;
     const float w = j < a.s ? a.mask[row] : 0.f;
+    const bool on = w != 0.f;
+    const long long label = on ? a.sums.labels[row] : 0;
+    const float given = on && a.ref_logp ? a.ref_logp[row] : 0.f;
     launch::wait_for_predecessor();
+    const float2 own = peek(a.sums, 0, row, on), own_r = a.has_ref_logits ? peek(a.sums, 1, row, on) : make_float2(0.f, 0.f);
+    const float x = on ? a.sums.target[row] : 0.f, y = on && a.has_ref_logits ? a.sums.target[(long long)a.sums.rows + row] : 0.f;
     const int chunks = a.sums.chunks ? a.sums.chunks : a.sums.ticket[1];
     double v[2] = {0.0, 0.0};
     float m, mr = 0.f;
     double t, tr = 0.0;
-    join(a.sums, chunks, 0, row, w != 0.f, m, t);
-    if (a.has_ref_logits) join(a.sums, chunks, 1, row, w != 0.f, mr, tr);
+    join(a.sums, chunks, 0, row, on, own, m, t);
+    if (a.has_ref_logits) join(a.sums, chunks, 1, row, on, own_r, mr, tr);
     if (j < a.s && threadIdx.x % LANES == 0) {
-        a.row[row] = w != 0.f ? make_float2(m, (float)(1.0 / t)) : make_float2(0.f, 0.f);
-        if (w != 0.f) {
-            v[0] = w * label_logp(a.sums, 0, row, m, t);
-            if (a.has_ref_logits) v[1] = w * label_logp(a.sums, 1, row, mr, tr);
-            else if (a.ref_logp) v[1] = (double)w * a.ref_logp[row];
+        a.row[row] = on ? make_float2(m, __frcp_rn((float)t)) : make_float2(0.f, 0.f);
+        if (on) {
+            v[0] = w * label_logp(a.sums, label, x, m, t);
+            if (a.has_ref_logits) v[1] = w * label_logp(a.sums, label, y, mr, tr);
+            else if (a.ref_logp) v[1] = (double)w * given;
         }
     }
     block_sum(v);
@@ -667,7 +676,8 @@ __global__ void __launch_bounds__(THREADS) preference_kernel(const PreferenceArg
     }
     if (!last_block(a.ticket)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    double* whole = a.partial + 2ll * gridDim.x;
+    __shared__ double near[2 * NEAR];
+    double* whole = a.n <= NEAR ? near : a.partial + 2ll * gridDim.x;
     for (int i = warp; i < a.n; i += THREADS / 32) {
         double p = 0.0, r = 0.0;
         for (int k = lane; k < a.pieces; k += 32) {
@@ -690,15 +700,14 @@ __global__ void __launch_bounds__(THREADS) preference_kernel(const PreferenceArg
         const double* c = whole + 2 * b;
         const double* r = whole + 2 * (b + pairs);
         const double z = a.beta * ((c[0] - r[0]) - (c[1] - r[1]));
-        const double small = exp(-fabs(z)), soft = log1p(small);
+        const float small = __expf(-fabsf((float)z)), soft = log1pf(small), even = (float)a.smoothing;
         double loss = (1.0 - a.smoothing) * (soft + fmax(-z, 0.0));
         if (a.smoothing != 0.0) loss += a.smoothing * (soft + fmax(z, 0.0));
         sum[0] += z != z ? z : loss;
-        const double up = z >= 0 ? 1.0 / (1.0 + small) : small / (1.0 + small);          // sigma(z)
-        const double down = z >= 0 ? small / (1.0 + small) : 1.0 / (1.0 + small);        // sigma(-z)
-        const double d = z != z ? z : -a.beta * ((1.0 - a.smoothing) * down - a.smoothing * up) / pairs;
-        a.coef[b] = (float)d;
-        a.coef[b + pairs] = (float)-d;
+        const float large = __frcp_rn(1.f + small), other = small * large;              // sigma(|z|), sigma(-|z|)
+        const float d = z != z ? (float)z : (float)(-a.beta / pairs) * ((1.f - even) * (z >= 0 ? other : large) - even * (z >= 0 ? large : other));
+        a.coef[b] = d;
+        a.coef[b + pairs] = -d;
     }
     block_sum(sum);
     if (threadIdx.x == 0) *a.loss = (float)(sum[0] / pairs);
@@ -733,16 +742,23 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(const PolicyArgs a) {
     const int seq = blockIdx.x / a.pieces, j = (blockIdx.x % a.pieces) * ROWS + threadIdx.x / LANES;
     const int row = seq * a.s + j;
     const float w = j < a.s ? a.mask[row] : 0.f;
+    const bool on = w != 0.f;
+    const long long label = on ? a.sums.labels[row] : 0;
+    const double adv = on ? a.advantages[seq * a.adv_n + j * a.adv_s] : 0.f;
+    const float old = on && a.old_logp ? a.old_logp[row] : 0.f, given = on && a.ref_logp ? a.ref_logp[row] : 0.f;
     launch::wait_for_predecessor();
+    const float2 own = peek(a.sums, 0, row, on), own_q = a.has_ref_logits ? peek(a.sums, 1, row, on) : make_float2(0.f, 0.f);
+    const bool two = a.has_ref_logits && a.kl != KL_FULL;
+    const float x = on ? a.sums.target[row] : 0.f, y = on && two ? a.sums.target[(long long)a.sums.rows + row] : 0.f;
     const int chunks = a.sums.chunks ? a.sums.chunks : a.sums.ticket[1];
     double v[4] = {0.0, 0.0, 0.0, 0.0};
     float m, mq = 0.f;
     double t, tq = 0.0, cross = 0.0;
-    join(a.sums, chunks, 0, row, w != 0.f, m, t);
-    if (a.has_ref_logits) join(a.sums, chunks, 1, row, w != 0.f, mq, tq);
+    join(a.sums, chunks, 0, row, on, own, m, t);
+    if (a.has_ref_logits) join(a.sums, chunks, 1, row, on, own_q, mq, tq);
     if (a.kl == KL_FULL) {
         const long long at = (long long)row * a.sums.most;
-        if (w != 0.f)
+        if (on)
             for (int k = threadIdx.x % LANES; k < chunks; k += LANES)
                 cross += (double)a.sums.cross[at + k] * (double)__expf(a.sums.part[at + k].x - m);
         cross = lanes_sum(cross);
@@ -750,12 +766,11 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(const PolicyArgs a) {
     if (j < a.s && threadIdx.x % LANES == 0) {
         float2 keep = make_float2(0.f, 0.f);
         float slope = 0.f, shift = 0.f, logp = 0.f;
-        if (w != 0.f) {
-            keep = make_float2(m, (float)(1.0 / t));
-            const double l = label_logp(a.sums, 0, row, m, t);
+        if (on) {
+            keep = make_float2(m, __frcp_rn((float)t));
+            const double l = label_logp(a.sums, label, x, m, t);
             logp = (float)l;
-            const double adv = a.advantages[seq * a.adv_n + j * a.adv_s];
-            const double ratio = a.old_logp ? exp(l - (double)a.old_logp[row]) : (l == l ? 1.0 : l);
+            const double ratio = a.old_logp ? exp(l - (double)old) : (l == l ? 1.0 : l);
             const double bounded = fmin(fmax(ratio, a.low), a.high);
             const double free = ratio * adv, held = bounded * adv;
             const bool clipped = free > held;
@@ -766,22 +781,22 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(const PolicyArgs a) {
                 shift = (float)(gap + kl);
             } else if (a.kl != KL_NONE) {
                 double ref;
-                if (a.has_ref_logits) ref = label_logp(a.sums, 1, row, mq, tq);
-                else ref = a.ref_logp[row];
-                const double x = l - ref;
+                if (a.has_ref_logits) ref = label_logp(a.sums, label, y, mq, tq);
+                else ref = given;
+                const double gap = l - ref;
                 double more;
                 if (a.kl == KL_PLAIN) {
-                    kl = x;
-                    more = x == x ? 1.0 : x;
+                    kl = gap;
+                    more = gap == gap ? 1.0 : gap;
                 } else if (a.kl == KL_ABS) {
-                    kl = fabs(x);
-                    more = x > 0.0 ? 1.0 : x < 0.0 ? -1.0 : x;
+                    kl = fabs(gap);
+                    more = gap > 0.0 ? 1.0 : gap < 0.0 ? -1.0 : gap;
                 } else if (a.kl == KL_MSE) {
-                    kl = 0.5 * x * x;
-                    more = x;
+                    kl = 0.5 * gap * gap;
+                    more = gap;
                 } else {
-                    const double e = expm1(-x);
-                    kl = e + x;
+                    const double e = expm1(-gap);
+                    kl = e + gap;
                     more = -e;
                 }
                 d += a.kl_beta * more;
@@ -804,7 +819,8 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(const PolicyArgs a) {
         for (int k = 0; k < 4; ++k) a.partial[4ll * blockIdx.x + k] = v[k];
     if (!last_block(a.ticket)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    double* whole = a.partial + 4ll * gridDim.x;
+    __shared__ double near[4 * NEAR];
+    double* whole = a.n <= NEAR ? near : a.partial + 4ll * gridDim.x;
     for (int i = warp; i < a.n; i += THREADS / 32) {
         double p[4] = {0.0, 0.0, 0.0, 0.0};
         for (int k = lane; k < a.pieces; k += 32)
@@ -963,14 +979,14 @@ struct GradPlan {
 struct StatsPlan {
     int chunks = 1, most;
     StatsPlan(long long rows, int vocab, int dtype, int full) {
-        const int least = 32 * (dtype == 1 ? 4 : 8), warps = full ? Shape<true>::WARPS : Shape<false>::WARPS;
+        const int n = dtype == 1 ? 4 : 8, least = 32 * n, step = least * Shape<true>::VECTORS / (full ? 2 : 1);
+        const int warps = (full ? Shape<true>::WARPS : Shape<false>::WARPS) * neox_sm_count();
         most = (vocab + least - 1) / least;
-        // a row of its own for every warp of the machine: no more than the chunks of a long row
-        const long long busy = (long long)warps * neox_sm_count(), usual = (vocab + 4095) / 4096;
-        if (rows > 2 * busy && most > usual) most = (int)usual;
+        const int usual = (vocab + 2 * step - 1) / (2 * step);
+        if (rows > 2ll * warps && most > usual) most = usual;   // a row of its own for every warp of the machine
         if (most > 64) most = 64;
         for (int c = 1; c <= most; ++c)
-            if (cut_cost(rows, vocab, c, neox_sm_count(), warps) < cut_cost(rows, vocab, chunks, neox_sm_count(), warps)) chunks = c;
+            if (cut_cost(rows, vocab, c, warps, step) < cut_cost(rows, vocab, chunks, warps, step)) chunks = c;
     }
 };
 

@@ -96,8 +96,14 @@ def _rows(t):
     return t if t is None or t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
 
 
+@functools.lru_cache(maxsize=1)
+def _mpu():
+    from ..parallel import mpu                  # which imports this package
+    return mpu
+
+
 def _tensor_parallel():
-    from ..parallel import mpu
+    mpu = _mpu()
     return mpu.get_model_parallel_world_size(), mpu.get_model_parallel_rank(), mpu.get_model_parallel_group
 
 
@@ -164,7 +170,8 @@ def _forward(x, y, labels, mask, width, loss, kl_mean, clipped, logp, ref, old_l
     tail = (ticket, sums, row, coef, slope, shift if full else 0, loss.data_ptr(), 0 if kl_mean is None else kl_mean.data_ptr(),
             0 if clipped is None else clipped.data_ptr(), logp.data_ptr(), 0 if ref is None else ref.data_ptr(),
             0 if old_logp is None else old_logp.data_ptr(), 0 if ref_logp is None else ref_logp.data_ptr(),
-            0 if adv is None else adv.data_ptr(), 0 if adv is None else adv.stride(0), 0 if adv is None else adv.stride(1),
+            *((0, 0, 0) if adv is None else (adv.data_ptr(), adv.stride(0) if adv.shape[0] > 1 else 0,
+                                             adv.stride(1) if adv.shape[1] > 1 else 0)),
             0, 0, 0, 0, 0, rank * v, tp * v, native.stream_ptr(), beta, smoothing, low, high, n, s, v, dt, kl, by_sequence)
     run = native.lib().neox_loss_forward
     policy = width == 4
@@ -214,10 +221,13 @@ def _grad_f32(g):
 
 
 class _PreferenceFn(torch.autograd.Function):
+    """All but the logits are constants and come as one argument: autograd looks at each of them otherwise."""
+
     @staticmethod
-    def forward(ctx, x, labels, mask, ref_logits, ref_logp, beta, smoothing):
+    def forward(ctx, x, rest):
+        labels, mask, ref_logits, ref_logp, beta, smoothing = rest
         with device_of(x):
-            loss, logp, ref, (buf, ctx.first) = _preference_values(x, labels, mask, ref_logits, ref_logp, beta, smoothing)
+            loss, logp, ref, (buf, ctx.first) = _preference_values(x, *rest)
         ctx.streams = 1 if ref_logits is None else 2
         ctx.save_for_backward(x, labels, mask, buf)
         ctx.mark_non_differentiable(ref)
@@ -227,11 +237,11 @@ class _PreferenceFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g_loss, g_logp, _):
         if g_loss is None and g_logp is None:
-            return (None,) * 7
+            return None, None
         x, labels, mask, buf = ctx.saved_tensors
         with device_of(x):
             g = _backward(x, None, labels, mask, buf, ctx.first, 2, ctx.streams, _grad_f32(g_loss), _grad_f32(g_logp), 0.0)
-        return once(g, x), None, None, None, None, None, None
+        return once(g, x), None
 
 
 def _policy_values(x, labels, mask, adv, old_logp, ref_logits, ref_logp, low, high, kl, kl_beta, by_sequence):
@@ -247,10 +257,10 @@ def _policy_values(x, labels, mask, adv, old_logp, ref_logits, ref_logp, low, hi
 
 class _PolicyFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, labels, mask, adv, old_logp, ref_logits, ref_logp, low, high, kl, kl_beta, by_sequence):
+    def forward(ctx, x, rest):
+        labels, mask, _, _, ref_logits, _, _, _, kl, kl_beta, _ = rest
         with device_of(x):
-            loss, kl_mean, clipped, logp, (buf, ctx.first) = _policy_values(x, labels, mask, adv, old_logp, ref_logits, ref_logp, low,
-                                                                            high, kl, kl_beta, by_sequence)
+            loss, kl_mean, clipped, logp, (buf, ctx.first) = _policy_values(x, *rest)
         ctx.streams, ctx.kl_beta = 1 if ref_logits is None else 2, kl_beta
         ctx.save_for_backward(x, labels, mask, buf, ref_logits if kl == KL_KINDS["full"] else None)
         ctx.mark_non_differentiable(kl_mean, clipped, logp)
@@ -260,11 +270,11 @@ class _PolicyFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g_loss, *_):
         if g_loss is None:
-            return (None,) * 12
+            return None, None
         x, labels, mask, buf, y = ctx.saved_tensors
         with device_of(x):
             g = _backward(x, y, labels, mask, buf, ctx.first, 4, ctx.streams, _grad_f32(g_loss), None, ctx.kl_beta)
-        return (once(g, x),) + (None,) * 11
+        return once(g, x), None
 
 
 # ---------------------------------------------------------------------------------------------- plain statements
@@ -378,12 +388,13 @@ def preference_loss(logits, labels, loss_mask, beta, ref_logits: Optional[torch.
         raise ValueError(f"label_smoothing is at least 0 and below 1, got {label_smoothing}")
     if not _k(logits):
         return preference_loss_ref(logits, labels, loss_mask, beta, ref_logits, ref_logp, label_smoothing)
-    args = (_rows(logits), _as(labels, torch.int64), _as(loss_mask, torch.float32), _rows(ref_logits),
-            _as(ref_logp, torch.float32), float(beta), float(label_smoothing))
+    x = _rows(logits)
+    rest = (_as(labels, torch.int64), _as(loss_mask, torch.float32), _rows(ref_logits), _as(ref_logp, torch.float32), float(beta),
+            float(label_smoothing))
     if native.plain_call(logits):
-        with device_of(logits):
-            return PreferenceLoss(*_preference_values(*args)[:3])
-    return PreferenceLoss(*_PreferenceFn.apply(*args))
+        with device_of(x):
+            return PreferenceLoss(*_preference_values(x, *rest)[:3])
+    return PreferenceLoss(*_PreferenceFn.apply(x, rest))
 
 
 def policy_loss(logits, labels, loss_mask, advantages, old_logp: Optional[torch.Tensor] = None,
@@ -430,12 +441,12 @@ def policy_loss(logits, labels, loss_mask, advantages, old_logp: Optional[torch.
     if advantages.dtype != torch.float32:
         advantages = advantages.to(torch.float32)
     kind = KL_KINDS[kl] if ref_logits is not None or ref_logp is not None else 0
-    args = (_rows(logits), _as(labels, torch.int64), _as(loss_mask, torch.float32), advantages.expand(n, s),
-            _as(old_logp, torch.float32), _rows(ref_logits), _as(ref_logp, torch.float32), 1.0 - clip_low, 1.0 + clip_high, kind,
-            float(kl_beta), reduce == "sequence")
+    x = _rows(logits)
+    rest = (_as(labels, torch.int64), _as(loss_mask, torch.float32), advantages, _as(old_logp, torch.float32), _rows(ref_logits),
+            _as(ref_logp, torch.float32), 1.0 - clip_low, 1.0 + clip_high, kind, float(kl_beta), reduce == "sequence")
     if native.plain_call(logits):
-        with device_of(logits):
-            loss, mean_kl, clipped, logp = _policy_values(*args)[:4]
+        with device_of(x):
+            loss, mean_kl, clipped, logp = _policy_values(x, *rest)[:4]
     else:
-        loss, mean_kl, clipped, logp = _PolicyFn.apply(*args)
+        loss, mean_kl, clipped, logp = _PolicyFn.apply(x, rest)
     return PolicyLoss(loss, logp, mean_kl, clipped)
