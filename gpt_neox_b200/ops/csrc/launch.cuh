@@ -43,4 +43,20 @@ int overlapped(void (*kernel)(Params...), dim3 grid, dim3 block, int cluster, cu
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...) == cudaSuccess ? 0 : NEOX_ERR_LAUNCH;
 }
 
+// The same with dynamic shared memory, which the caller has allowed.
+template <typename... Params, typename... Args>
+int overlapped_with(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...) == cudaSuccess ? 0 : NEOX_ERR_LAUNCH;
+}
+
 }  // namespace launch

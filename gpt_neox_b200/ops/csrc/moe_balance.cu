@@ -39,7 +39,7 @@ template <typename T> struct Eight {
     __device__ __forceinline__ void load(const T* p, int left, bool aligned) {
         if (aligned && left > 0) {
 #pragma unroll
-            for (int i = 0; i < WORDS; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+            for (int i = 0; i < WORDS; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
         } else {
             __align__(16) T t[8];
 #pragma unroll

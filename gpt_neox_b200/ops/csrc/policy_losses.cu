@@ -158,9 +158,35 @@ template <typename T> __device__ __forceinline__ void pairs_of(const uint4& u, f
 // Logits are read once a pass: they stay out of L1.
 __device__ __forceinline__ uint4 load_16(const void* p) {
     uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                  : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
+}
+
+// exp(x - m) of the elements of 16 bytes.  16-bit numbers are taken from their words by the subtraction itself (the widening is
+// exact), which saves an instruction an element.
+__device__ __forceinline__ f32x2 less(uint32_t w, float m, __nv_bfloat16) {
+    float a, b;
+    asm("{.reg .b16 x, y;\n mov.b32 {x, y}, %2;\n sub.rn.f32.bf16 %0, x, %3;\n sub.rn.f32.bf16 %1, y, %3;}" : "=f"(a), "=f"(b) : "r"(w), "f"(m));
+    return pair(a, b);
+}
+__device__ __forceinline__ f32x2 less(uint32_t w, float m, __half) {
+    float a, b;
+    asm("{.reg .b16 x, y;\n mov.b32 {x, y}, %2;\n sub.rn.f32.f16 %0, x, %3;\n sub.rn.f32.f16 %1, y, %3;}" : "=f"(a), "=f"(b) : "r"(w), "f"(m));
+    return pair(a, b);
+}
+template <typename T> __device__ __forceinline__ void exps_of(const uint4& u, float m, f32x2 (&e)[Elem<T>::PER_16 / 2]) {
+    if constexpr (Elem<T>::PER_16 == 4) {
+        e[0] = exp_of(pair(__uint_as_float(u.x), __uint_as_float(u.y)), pair(-m, -m));
+        e[1] = exp_of(pair(__uint_as_float(u.z), __uint_as_float(u.w)), pair(-m, -m));
+    } else {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 t = parts(mul(less(w[i], m, T()), pair(LOG2E, LOG2E)));
+            e[i] = pair(exp2_fast(t.x), exp2_fast(t.y));
+        }
+    }
 }
 
 // Asynchronous copies of 16 bytes to shared memory, in groups: `copies_here<K>` waits until all but the last K groups of this thread
@@ -301,8 +327,9 @@ template <typename T, bool FULL> struct Walk {
 };
 
 // What a lane has of a chunk so far: the largest logit and the sums against it.
-template <typename T, bool FULL> struct Running {
-    static constexpr int N = Elem<T>::PER_16, U = Shape<FULL>::VECTORS / (FULL ? 2 : 1);
+// PAIR: the reference's sums too; CROSS: and the sum of p (x - y).  U vectors at a time, STRIDE of them apart.
+template <typename T, bool PAIR, bool CROSS, int U, int STRIDE> struct Running {
+    static constexpr int N = Elem<T>::PER_16;
     float m, n;                    // policy, reference
     f32x2 t, r, w;                 // sum of exponentials (policy, reference), sum of p (x - y)
 
@@ -315,48 +342,58 @@ template <typename T, bool FULL> struct Running {
         const float k = __expf(m - px);
         m = px;
         t = mul(t, pair(k, k));
-        if constexpr (FULL) {
+        if constexpr (PAIR) {
             const float kr = __expf(n - qx);
             n = qx;
             r = mul(r, pair(kr, kr));
-            w = mul(w, pair(k, k));
+            if constexpr (CROSS) w = mul(w, pair(k, k));
         }
     }
-    __device__ __forceinline__ void add_vectors(const uint4 (&xr)[U], const uint4 (&yr)[FULL ? U : 1], int left, bool whole) {
+    __device__ __forceinline__ void add_vectors(const uint4 (&xr)[U], const uint4 (&yr)[PAIR ? U : 1], int left, bool whole) {
         uint32_t p = larger<T>(xr[0]), q = 0;
-        if constexpr (FULL) q = larger<T>(yr[0]);
+        if constexpr (PAIR) q = larger<T>(yr[0]);
 #pragma unroll
         for (int u = 1; u < U; ++u)
-            if (whole || u * 32 < left) {
+            if (whole || u * STRIDE < left) {
                 p = larger(p, larger<T>(xr[u]), T());
-                if constexpr (FULL) q = larger(q, larger<T>(yr[u]), T());
+                if constexpr (PAIR) q = larger(q, larger<T>(yr[u]), T());
             }
-        raise(fmaxf(m, as_max<T>(p)), FULL ? fmaxf(n, as_max<T>(q)) : 0.f);
+        const float px = as_max<T>(p), qx = PAIR ? as_max<T>(q) : n;
+        if (px > m || qx > n) raise(fmaxf(m, px), fmaxf(n, qx));
         const f32x2 xs = pair(-m, -m), ys = pair(-n, -n), minus = pair(-1.f, -1.f);
         f32x2 gap = pair(0.f, 0.f);
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (whole || u * 32 < left) {
-                f32x2 v[N / 2], q2[N / 2];
-                pairs_of<T>(xr[u], v);
-                if constexpr (FULL) pairs_of<T>(yr[u], q2);
+            if (whole || u * STRIDE < left) {
+                f32x2 e[N / 2];
+                if constexpr (CROSS) {
+                    f32x2 v[N / 2], q2[N / 2];
+                    pairs_of<T>(xr[u], v);
+                    pairs_of<T>(yr[u], q2);
 #pragma unroll
-                for (int i = 0; i < N / 2; ++i) {
-                    const f32x2 e = exp_of(v[i], xs);
-                    t = add(t, e);
-                    if constexpr (FULL) {
-                        gap = fma(e, fma(q2[i], minus, v[i]), gap);
+                    for (int i = 0; i < N / 2; ++i) {
+                        e[i] = exp_of(v[i], xs);
+                        gap = fma(e[i], fma(q2[i], minus, v[i]), gap);
                         r = add(r, exp_of(q2[i], ys));
                     }
+                } else {
+                    if constexpr (PAIR) {
+                        exps_of<T>(yr[u], n, e);
+#pragma unroll
+                        for (int i = 0; i < N / 2; ++i) r = add(r, e[i]);
+                    }
+                    exps_of<T>(xr[u], m, e);
                 }
+#pragma unroll
+                for (int i = 0; i < N / 2; ++i) t = add(t, e[i]);
             }
-        if constexpr (FULL) {
+        if constexpr (CROSS) {
             const float2 g = parts(gap);
             if (g.x + g.y != g.x + g.y) {                       // 0 times infinity somewhere: what is impossible adds nothing
                 float again = 0.f;
 #pragma unroll
                 for (int u = 0; u < U; ++u)
-                    if (u * 32 < left) {
+                    if (u * STRIDE < left) {
                         float v[N], q1[N];
                         unpack<T>(xr[u], v);
                         unpack<T>(yr[u], q1);
@@ -372,13 +409,11 @@ template <typename T, bool FULL> struct Running {
         }
     }
     __device__ __forceinline__ void add_one(float ex, float ey) {
-        raise(fmaxf(m, ex), FULL ? fmaxf(n, ey) : 0.f);
+        raise(fmaxf(m, ex), PAIR ? fmaxf(n, ey) : 0.f);
         const float e = __expf(ex - m);
         t = add(t, pair(e, 0.f));
-        if constexpr (FULL) {
-            w = add(w, pair(e > 0.f ? e * (ex - ey) : 0.f, 0.f));
-            r = add(r, pair(__expf(ey - n), 0.f));
-        }
+        if constexpr (CROSS) w = add(w, pair(e > 0.f ? e * (ex - ey) : 0.f, 0.f));
+        if constexpr (PAIR) r = add(r, pair(__expf(ey - n), 0.f));
     }
 };
 
@@ -461,7 +496,7 @@ __global__ void __launch_bounds__(Shape<FULL>::WARPS * 32, 1) stats_kernel(const
         W ahead, now;                                           // the walk of the copies and that of the sums
         ahead.item = now.item = lo + warp;
         unsigned taken = 0, begun = 0;
-        Running<T, FULL> run;
+        Running<T, FULL, FULL, U, 32> run;
         run.clear();
         if (now.item < hi) {
             ahead.enter(a, sm.list, first, chunks, chunk);
@@ -595,8 +630,8 @@ __device__ __forceinline__ void join(const RowSums& r, int chunks, int stream, i
     t = lanes_sum(t);
 }
 // Log-probability of a label whose logit is x.
-__device__ __forceinline__ double label_logp(const RowSums& r, long long label, float x, float m, double t) {
-    return label < 0 || label >= r.vocab ? nan("") : ((double)x - (double)m) - log(t);
+__device__ __forceinline__ double label_logp(long long vocab, long long label, float x, float m, double t) {
+    return label < 0 || label >= vocab ? nan("") : ((double)x - (double)m) - log(t);
 }
 
 // Sums of V values over the block, in a fixed order; the result is in thread 0.
@@ -664,8 +699,8 @@ __global__ void __launch_bounds__(THREADS) preference_kernel(const PreferenceArg
     if (j < a.s && threadIdx.x % LANES == 0) {
         a.row[row] = on ? make_float2(m, __frcp_rn((float)t)) : make_float2(0.f, 0.f);
         if (on) {
-            v[0] = w * label_logp(a.sums, label, x, m, t);
-            if (a.has_ref_logits) v[1] = w * label_logp(a.sums, label, y, mr, tr);
+            v[0] = w * label_logp(a.sums.vocab, label, x, m, t);
+            if (a.has_ref_logits) v[1] = w * label_logp(a.sums.vocab, label, y, mr, tr);
             else if (a.ref_logp) v[1] = (double)w * given;
         }
     }
@@ -736,8 +771,46 @@ struct PolicyArgs {
     float* coef;                   // [n]: what a row's slope is multiplied by
 };
 
-// Row by row: r = exp(l - old), term = -min(r A, clip(r) A) + kl_beta KL and its slope in l; sums of mask, mask * term,
-// mask * KL and mask * [clipped] by sequence, then the means.
+// A row's part of the policy loss: r = exp(l - old), term = -min(r A, clip(r) A) + kl_beta KL, and the term's slope in l (the KL over
+// the vocabulary has its own way into the logits).
+struct RowTerm {
+    double term, slope, kl;
+    bool clipped;
+    // l: log-probability; ref: the reference's, where a KL of tokens wants it; full: the KL over the vocabulary
+    __device__ __forceinline__ RowTerm(int kind, double low, double high, double kl_beta, double l, bool has_old, float old, double adv,
+                                       double ref, double full) {
+        const double ratio = has_old ? exp(l - (double)old) : (l == l ? 1.0 : l);
+        const double free = ratio * adv, held = fmin(fmax(ratio, low), high) * adv;
+        clipped = free > held;
+        term = clipped ? -held : -free;
+        slope = clipped ? 0.0 : -free;
+        kl = 0.0;
+        if (kind == KL_FULL) {
+            kl = full;
+        } else if (kind != KL_NONE) {
+            const double gap = l - ref;
+            double rise;
+            if (kind == KL_PLAIN) {
+                kl = gap;
+                rise = gap == gap ? 1.0 : gap;
+            } else if (kind == KL_ABS) {
+                kl = fabs(gap);
+                rise = gap > 0.0 ? 1.0 : gap < 0.0 ? -1.0 : gap;
+            } else if (kind == KL_MSE) {
+                kl = 0.5 * gap * gap;
+                rise = gap;
+            } else {
+                const double e = expm1(-gap);
+                kl = e + gap;
+                rise = -e;
+            }
+            slope += kl_beta * rise;
+        }
+        term += kl_beta * kl;
+    }
+};
+
+// Row by row the terms and their slopes; sums of mask, mask * term, mask * KL and mask * [clipped] by sequence, then the means.
 __global__ void __launch_bounds__(THREADS) policy_kernel(const PolicyArgs a) {
     const int seq = blockIdx.x / a.pieces, j = (blockIdx.x % a.pieces) * ROWS + threadIdx.x / LANES;
     const int row = seq * a.s + j;
@@ -768,45 +841,22 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(const PolicyArgs a) {
         float slope = 0.f, shift = 0.f, logp = 0.f;
         if (on) {
             keep = make_float2(m, __frcp_rn((float)t));
-            const double l = label_logp(a.sums, label, x, m, t);
+            const double l = label_logp(a.sums.vocab, label, x, m, t);
             logp = (float)l;
-            const double ratio = a.old_logp ? exp(l - (double)old) : (l == l ? 1.0 : l);
-            const double bounded = fmin(fmax(ratio, a.low), a.high);
-            const double free = ratio * adv, held = bounded * adv;
-            const bool clipped = free > held;
-            double term = clipped ? -held : -free, d = clipped ? 0.0 : -free, kl = 0.0;
+            double ref = given, full = 0.0;
             if (a.kl == KL_FULL) {
                 const double gap = ((double)m - (double)mq) + (log(t) - log(tq));
-                kl = cross / t - gap;
-                shift = (float)(gap + kl);
-            } else if (a.kl != KL_NONE) {
-                double ref;
-                if (a.has_ref_logits) ref = label_logp(a.sums, label, y, mq, tq);
-                else ref = given;
-                const double gap = l - ref;
-                double more;
-                if (a.kl == KL_PLAIN) {
-                    kl = gap;
-                    more = gap == gap ? 1.0 : gap;
-                } else if (a.kl == KL_ABS) {
-                    kl = fabs(gap);
-                    more = gap > 0.0 ? 1.0 : gap < 0.0 ? -1.0 : gap;
-                } else if (a.kl == KL_MSE) {
-                    kl = 0.5 * gap * gap;
-                    more = gap;
-                } else {
-                    const double e = expm1(-gap);
-                    kl = e + gap;
-                    more = -e;
-                }
-                d += a.kl_beta * more;
+                full = cross / t - gap;
+                shift = (float)(gap + full);
+            } else if (a.has_ref_logits) {
+                ref = label_logp(a.sums.vocab, label, y, mq, tq);
             }
-            term += a.kl_beta * kl;
-            slope = (float)(w * d);
+            const RowTerm r(a.kl, a.low, a.high, a.kl_beta, l, a.old_logp != nullptr, old, adv, ref, full);
+            slope = (float)(w * r.slope);
             v[0] = w;
-            v[1] = w * term;
-            v[2] = w * kl;
-            v[3] = clipped ? w : 0.0;
+            v[1] = w * r.term;
+            v[2] = w * r.kl;
+            v[3] = r.clipped ? w : 0.0;
         }
         a.row[row] = keep;
         a.slope[row] = slope;
@@ -874,7 +924,7 @@ struct GradArgs {
     const float* g_loss;           // gradient of the loss, or none
     const float* g_logp;           // [n], or none: gradient of the sequences' log-probabilities
     long long v0;
-    float kl_beta;
+    float kl_beta, expected;       // expected: of g_loss, where the forward has written the gradient for it
     int rows, s, vocab, splits, chunk;
 };
 
@@ -885,10 +935,47 @@ __device__ __forceinline__ float grad_of(float x, float y, float m, float scale,
     else return e * scale;
 }
 
-template <typename T, int G, int U, bool FULL>
-__global__ void __launch_bounds__(THREADS) grad_kernel(const GradArgs a) {
+// What a row's gradient is made of: dx[c] = coef [c == label] + exp(x - m) (scale + bscale ((x - y) - shift)).
+struct RowGrad {
+    float m, coef, scale, bscale, shift;
+    bool zero;                     // all of it is
+};
+
+// exp(x - m) * scale at the elements of 16 bytes.
+template <typename T> __device__ __forceinline__ uint4 grad_vector(const uint4& u, const RowGrad& r) {
     constexpr int N = Elem<T>::PER_16;
-    const unsigned item = blockIdx.x * (THREADS / G) + threadIdx.x / G;
+    f32x2 e[N / 2];
+    exps_of<T>(u, r.m, e);
+    float v[N];
+#pragma unroll
+    for (int k = 0; k < N / 2; ++k) {
+        const float2 f = parts(mul(e[k], pair(r.scale, r.scale)));
+        v[2 * k] = f.x;
+        v[2 * k + 1] = f.y;
+    }
+    return repack<T>(v);
+}
+
+// A row's gradient by G threads: zeros; and, where no common shift aligns it with the logits, element by element.
+template <typename T, int G> __device__ __forceinline__ void write_zeros(T* g, int count, int lane) {
+    const Cut<T> cut(g, count);
+    uint4* gv = reinterpret_cast<uint4*>(g + cut.head);
+#pragma unroll 4
+    for (int v = lane; v < cut.vectors; v += G) __stcs(gv + v, make_uint4(0, 0, 0, 0));
+    if (lane < cut.head) g[lane] = Elem<T>::put(0.f);
+    if (lane < cut.tail) g[cut.head + cut.vectors * Elem<T>::PER_16 + lane] = Elem<T>::put(0.f);
+}
+template <typename T, int G> __device__ __forceinline__ void write_apart(const T* x, T* g, int count, int lane, const RowGrad& r, int label) {
+    for (int c = lane; c < count; c += G) {
+        float v = r.zero ? 0.f : grad_of<T, false>(Elem<T>::get(x[c]), 0.f, r.m, r.scale, 0.f, 0.f);
+        if (c == label) v += r.coef;
+        g[c] = Elem<T>::put(v);
+    }
+}
+
+// One chunk of a row by G threads, at most U 16-byte vectors each.
+template <typename T, int G, int U, bool FULL> __device__ __forceinline__ void grad_chunk(const GradArgs& a, unsigned item) {
+    constexpr int N = Elem<T>::PER_16;
     const int lane = threadIdx.x % G;
     const int row = (int)(item / (unsigned)a.splits), part = (int)(item % (unsigned)a.splits);
     if (row >= a.rows) return;
@@ -960,6 +1047,313 @@ __global__ void __launch_bounds__(THREADS) grad_kernel(const GradArgs a) {
     }
 }
 
+template <typename T, int G, int U, bool FULL>
+__global__ void __launch_bounds__(THREADS) grad_kernel(const GradArgs a) {
+    grad_chunk<T, G, U, FULL>(a, blockIdx.x * (THREADS / G) + threadIdx.x / G);
+}
+
+// The same after a forward that has foreseen a gradient of the loss: nothing to do where it is that one, so few blocks look, and
+// they walk over the chunks where it is another.
+template <typename T, int G, int U>
+__global__ void __launch_bounds__(THREADS) grad_unless_kernel(const GradArgs a, unsigned items) {
+    if (*a.g_loss == a.expected) return;
+    for (unsigned item = blockIdx.x * (THREADS / G) + threadIdx.x / G; item < items; item += gridDim.x * (THREADS / G))
+        grad_chunk<T, G, U, false>(a, item);
+}
+
+// ---------------------------------------------------------------------------------------------- policy loss and gradient at once
+// All that a row of the policy loss needs from other rows is the sum of the mask, and that is known before.  So with the gradient of
+// the loss foreseen (1, or what the caller says) a block takes a row's statistics, its term and its gradient while the row is in
+// shared memory: logits are read once, not twice.  The backward then only looks whether it was asked for that gradient.
+// (Leaving the row to L2 in between, four blocks an SM, two fifths of the rows had gone when they were wanted again.)
+struct AtOnceArgs {
+    Rows x;
+    void* g;
+    long long gn, gs;
+    const long long* labels;
+    const float* mask;
+    const float* advantages;
+    long long adv_n, adv_s;
+    const float* old_logp;
+    const float* ref_logp;
+    int n, s, vocab, kl, by_sequence;
+    double low, high, kl_beta;
+    float expected;
+    float2* row;
+    float* slope;
+    float4* terms;                 // per row: mask, mask * term, mask * KL, mask * [clipped]
+    double* whole;                 // [n]: sums of the mask
+    int* order;                    // the kept rows, then the others; behind them, the number of kept ones
+    float* coef;                   // [n]
+    float* loss;
+    float* kl_mean;
+    float* share;
+    float* logp;                   // [n, s]
+};
+
+// What each sequence's slopes are multiplied by: 1 / (sum of the mask), of the whole batch or of the sequence and then shared by the
+// sequences that keep something; and the order of the rows.  One block; several warps a sequence where there are few.
+__global__ void __launch_bounds__(1024) policy_share_kernel(const AtOnceArgs a) {
+    __shared__ double near[32];
+    __shared__ int kept_by[32];
+    launch::let_successor_start();
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, rows = a.n * a.s;
+    const int each = a.n >= 32 ? 1 : 32 / a.n, teams = 32 / each;            // warps of a sequence, sequences at a time
+    double total = 0.0, filled = 0.0;
+    for (int first = 0; first < a.n; first += teams) {
+        const int i = first + warp / each, piece = warp % each;
+        double w = 0.0;
+        if (warp / each < teams && i < a.n)
+#pragma unroll 8
+            for (int j = piece * 32 + lane; j < a.s; j += each * 32) w += a.mask[(long long)i * a.s + j];
+        w = warp_sum(w);
+        __syncthreads();
+        if (lane == 0) near[warp] = w;
+        __syncthreads();
+        for (int t = 0; t < teams && first + t < a.n; ++t) {                 // all threads, the same order
+            double sum = 0.0;
+            for (int q = 0; q < each; ++q) sum += near[t * each + q];
+            total += sum;
+            filled += sum > 0.0 ? 1.0 : 0.0;
+            if (threadIdx.x == 0) a.whole[first + t] = sum;
+        }
+    }
+    // the rows in a warp's part of them: kept ones counted, then placed from the front, the others behind all kept ones
+    const int part = ((rows + 31) / 32 + 31) / 32 * 32, from = min(rows, warp * part), to = min(rows, from + part);
+    int mine = 0;
+    for (int r = from; r < to; r += 32 * SCAN) {
+        float w[SCAN];
+#pragma unroll
+        for (int k = 0; k < SCAN; ++k) w[k] = r + k * 32 + lane < to ? a.mask[r + k * 32 + lane] : 0.f;
+#pragma unroll
+        for (int k = 0; k < SCAN; ++k) mine += __popc(__ballot_sync(0xffffffffu, w[k] != 0.f));
+    }
+    if (lane == 0) kept_by[warp] = mine;
+    __syncthreads();
+    int before = 0, kept = 0;
+    for (int q = 0; q < 32; ++q) {
+        before += q < warp ? kept_by[q] : 0;
+        kept += kept_by[q];
+    }
+    int front = before, back = kept + from - before;
+    for (int r = from; r < to; r += 32) {
+        const bool in = r + lane < to, is = in && a.mask[r + lane] != 0.f;
+        const unsigned all = __ballot_sync(0xffffffffu, is), none = __ballot_sync(0xffffffffu, in && !is), below = (1u << lane) - 1;
+        if (is) a.order[front + __popc(all & below)] = r + lane;
+        else if (in) a.order[back + __popc(none & below)] = r + lane;
+        front += __popc(all);
+        back += __popc(none);
+    }
+    if (threadIdx.x == 0) a.order[rows] = kept;
+    for (int i = threadIdx.x; i < a.n; i += 1024) {
+        const double len = a.by_sequence ? a.whole[i] * filled : total;
+        a.coef[i] = len > 0.0 || (!a.by_sequence && len != 0.0) ? (float)(1.0 / len) : 0.f;
+    }
+}
+
+// A block walks over its rows.  A thread copies its own vectors of a row to shared memory, takes them for the sums as they arrive, and
+// when all threads have met for the row's numbers, once more for the gradient; each place that it has read the second time it fills
+// with the next row's vector.  Two blocks an SM where two rows fit (one is at its sums, the other at its gradient), else one.  The
+// rows that leave nothing are written in between: while a block waits for a row, memory has time for them.
+template <typename T, int TPB, int BLOCKS>
+__global__ void __launch_bounds__(TPB, BLOCKS) policy_row_kernel(const AtOnceArgs a, int places) {
+    constexpr int N = Elem<T>::PER_16, U = 4, TEAM = TPB / 32, PARTS = 4;
+    extern __shared__ __align__(16) unsigned char raw_smem[];
+    uint4* xs = reinterpret_cast<uint4*>(raw_smem);
+    __shared__ Sums ps[TEAM];
+    __shared__ RowGrad grad;
+    __shared__ int where;
+    const int tid = threadIdx.x, rows = a.n * a.s;
+    launch::wait_for_predecessor();
+    const int kept = a.order[rows];
+    const int part = (places + PARTS * TPB * U - 1) / (PARTS * TPB * U) * TPB * U;      // vectors of a part, copied as a group
+
+    struct Place {
+        const T* x;
+        int row, head, vectors;
+    };
+    auto place = [&](int pos) {
+        Place p;
+        p.row = a.order[pos];
+        const int i = p.row / a.s, j = p.row - i * a.s;
+        p.x = a.x.at<T>(i, j);
+        const Cut<T> cut(p.x, a.vocab);
+        p.head = cut.head;
+        p.vectors = cut.vectors;
+        return p;
+    };
+    auto request = [&](const Place& p, int v) { copy_16(xs + v, reinterpret_cast<const uint4*>(p.x + p.head) + v); };
+    // this block's rows: every gridDim.x-th of the kept ones and of the others
+    const int grid = gridDim.x, block = blockIdx.x;
+    const int mine = block < kept ? (kept - 1 - block) / grid + 1 : 0, others = block < rows - kept ? (rows - kept - 1 - block) / grid + 1 : 0;
+    int written = 0;
+    auto write_others = [&](int until) {
+        for (; written < until; ++written) {
+            const int row = a.order[kept + block + written * grid], i = row / a.s, j = row - i * a.s;
+            T* g = reinterpret_cast<T*>(a.g) + (long long)i * a.gn + (long long)j * a.gs;
+            write_zeros<T, TPB>(g, a.vocab, tid);
+            if (tid == 0) {
+                a.row[row] = make_float2(0.f, 0.f);
+                a.slope[row] = 0.f;
+                a.logp[row] = 0.f;
+                a.terms[row] = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        }
+    };
+    Place now = {};
+    if (mine > 0) {
+        now = place(block);
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q) {
+            for (int v = q * part + tid; v < min((q + 1) * part, now.vectors); v += TPB) request(now, v);
+            copies_sent();
+        }
+    }
+    for (int step = 0; step < mine; ++step) {
+        const int row = now.row, i = row / a.s, j = row - i * a.s;
+        const T* x = now.x;
+        const int tail = a.vocab - now.head - now.vectors * N;
+        long long label = 0;
+        float own = 0.f, old = 0.f, given = 0.f, adv = 0.f, weight = 0.f, per = 0.f;
+        if (tid == 0) {
+            label = a.labels[row];
+            weight = a.mask[row];
+            old = a.old_logp ? a.old_logp[row] : 0.f;
+            given = a.ref_logp ? a.ref_logp[row] : 0.f;
+            adv = a.advantages[i * a.adv_n + j * a.adv_s];
+            per = a.expected * a.coef[i];
+            own = label >= 0 && label < a.vocab ? Elem<T>::get(x[label]) : 0.f;
+        }
+        int edge = -1;                                          // head and tail of the row: at most one element a thread
+        if (tid < now.head) edge = tid;
+        else if (tid - N < tail && tid >= N) edge = now.head + now.vectors * N + tid - N;
+        const float ex = edge >= 0 ? Elem<T>::get(x[edge]) : 0.f;
+        Running<T, false, false, U, TPB> run;
+        run.clear();
+        if (edge >= 0) run.add_one(ex, 0.f);
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q) {
+            if (q == 0) copies_here<PARTS - 1>();
+            else if (q == 1) copies_here<PARTS - 2>();
+            else if (q == 2) copies_here<PARTS - 3>();
+            else copies_here<0>();
+            const int end = min((q + 1) * part, now.vectors);
+            for (int base = q * part + tid; base < end; base += U * TPB) {
+                uint4 xr[U], none[1];
+                if (base + (U - 1) * TPB < end) {
+#pragma unroll
+                    for (int u = 0; u < U; ++u) xr[u] = xs[base + u * TPB];
+                    run.add_vectors(xr, none, end - base, true);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+                        if (base + u * TPB < end) xr[u] = xs[base + u * TPB];
+                    run.add_vectors(xr, none, end - base, false);
+                }
+            }
+        }
+        const float2 halves = parts(run.t);
+        Sums p{run.m, halves.x + halves.y};
+        p.join_warp();
+        if (tid % 32 == 0) ps[tid / 32] = p;
+        __syncthreads();
+        if (tid < 32) {
+            const bool is = tid < TEAM;
+            const float m = warp_max(is ? ps[tid].m : -FLT_MAX);
+            const double t = warp_sum(is ? (double)ps[tid].t * (double)__expf(ps[tid].m - m) : 0.0);
+            if (tid == 0) {
+                const double l = label_logp(a.vocab, label, own, m, t);
+                const RowTerm r(a.kl, a.low, a.high, a.kl_beta, l, a.old_logp != nullptr, old, adv, given, 0.0);
+                const float slope = (float)(weight * r.slope), inv = __frcp_rn((float)t), coef = per * slope;
+                grad = RowGrad{m, coef, -coef * inv, 0.f, 0.f, coef == 0.f};
+                where = (int)label;                             // one that does not fit has made everything NaN
+                a.row[row] = make_float2(m, inv);
+                a.slope[row] = slope;
+                a.logp[row] = (float)l;
+                a.terms[row] = make_float4(weight, (float)(weight * r.term), (float)(weight * r.kl), r.clipped ? weight : 0.f);
+            }
+        }
+        Place next = {};
+        if (step + 1 < mine) next = place(block + (step + 1) * grid);
+        write_others((int)((long long)others * (step + 1) / mine));
+        __syncthreads();
+        const RowGrad r = grad;
+        const int hot = where;
+        T* g = reinterpret_cast<T*>(a.g) + (long long)i * a.gn + (long long)j * a.gs;
+        if ((((uintptr_t)x ^ (uintptr_t)g) & 15) != 0) {
+            write_apart<T, TPB>(x, g, a.vocab, tid, r, hot);
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) {
+                for (int v = q * part + tid; v < min((q + 1) * part, next.vectors); v += TPB) request(next, v);
+                copies_sent();
+            }
+        } else {
+            uint4* gv = reinterpret_cast<uint4*>(g + now.head);
+            const int spot = hot - now.head;
+            const bool own_it = spot >= 0 && spot < now.vectors * N && spot / N % TPB == tid;
+            const float xl = own_it ? Elem<T>::get(x[hot]) : 0.f;
+            const uint4* nv = reinterpret_cast<const uint4*>(next.x + next.head);
+            const int both = min(now.vectors, next.vectors), most = max(now.vectors, next.vectors);
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) {
+                int v = q * part + tid;
+                for (; v + (U - 1) * TPB < min((q + 1) * part, both); v += U * TPB) {
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        __stcs(gv + v + u * TPB, grad_vector<T>(xs[v + u * TPB], r));
+                        copy_16(xs + v + u * TPB, nv + v + u * TPB);
+                    }
+                }
+                for (; v < min((q + 1) * part, most); v += TPB) {
+                    if (v < now.vectors) __stcs(gv + v, grad_vector<T>(xs[v], r));
+                    if (v < next.vectors) request(next, v);
+                }
+                copies_sent();
+            }
+            if (own_it) g[hot] = Elem<T>::put(grad_of<T, false>(xl, 0.f, r.m, r.scale, 0.f, 0.f) + r.coef);
+            if (edge >= 0) {
+                float f = grad_of<T, false>(ex, 0.f, r.m, r.scale, 0.f, 0.f);
+                if (edge == hot) f += r.coef;
+                g[edge] = Elem<T>::put(f);
+            }
+        }
+        now = next;
+    }
+    copies_here<0>();
+    write_others(others);
+}
+
+// Means of the rows' terms, in a fixed order.  One block.
+__global__ void __launch_bounds__(1024) policy_mean_kernel(const AtOnceArgs a, int rows) {
+    __shared__ double red[32][4];
+    launch::wait_for_predecessor();
+    double v[4] = {0.0, 0.0, 0.0, 0.0};                         // mask, loss, KL, clipped
+#pragma unroll 4
+    for (int row = threadIdx.x; row < rows; row += 1024) {
+        const float4 t = a.terms[row];
+        v[0] += t.x;
+        v[1] += (double)t.y * a.coef[row / a.s];
+        v[2] += t.z;
+        v[3] += t.w;
+    }
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = warp_sum(v[k]);
+    if (lane == 0)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) red[warp][k] = v[k];
+    __syncthreads();
+    if (warp != 0) return;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = warp_sum(red[lane][k]);
+    if (lane == 0) {
+        const bool any = v[0] != 0.0;
+        *a.loss = any ? (float)v[1] : 0.f;
+        *a.kl_mean = any ? (float)(v[2] / v[0]) : 0.f;
+        *a.share = any ? (float)(v[3] / v[0]) : 0.f;
+    }
+}
+
 // How the gradient cuts a row: G threads with U loads each, for narrow vocabularies fewer of them, so that all have something to do.
 struct GradPlan {
     int threads, splits, chunk;
@@ -1005,6 +1399,25 @@ struct StatsPlan {
         else { constexpr int G = 256; CALL; }                      \
     } while (0)
 
+// Rows of the policy loss in shared memory: as many blocks an SM as rows fit, at most eight, or none.
+struct AtOncePlan {
+    int places, blocks;
+    size_t bytes;
+    AtOncePlan(int vocab, int dtype) {
+        places = vocab / (dtype == 1 ? 4 : 8) + 1;
+        bytes = (size_t)places * 16;
+        blocks = bytes <= most(8) ? 8 : bytes <= most(4) ? 4 : bytes <= most(3) ? 3 : bytes <= most(2) ? 2 : bytes <= most(1) ? 1 : 0;
+    }
+    // of 228 KB an SM, with 1 KB and what the kernel has besides for every block
+    static constexpr size_t most(int blocks) { return (228 * 1024 / blocks - 1536) / 1024 * 1024; }
+};
+
+template <typename T, int TPB, int BLOCKS>
+int rows_at_once(const AtOnceArgs& a, const AtOncePlan& p, dim3 grid, cudaStream_t st) {
+    if (!allow_dynamic_smem<policy_row_kernel<T, TPB, BLOCKS>>(AtOncePlan::most(BLOCKS))) return NEOX_ERR_LAUNCH;
+    return launch::overlapped_with(policy_row_kernel<T, TPB, BLOCKS>, grid, dim3(TPB), p.bytes, st, a, p.places);
+}
+
 #define LAUNCH_STATS(T, FULL)                                                                             \
     if (!allow_dynamic_smem<stats_kernel<T, FULL>>(sizeof(StatsSmem<FULL>))) return NEOX_ERR_LAUNCH;      \
     stats_kernel<T, FULL><<<blocks, Shape<FULL>::WARPS * 32, sizeof(StatsSmem<FULL>), st>>>(a)
@@ -1046,11 +1459,14 @@ struct LossCall {
     const float* g_logp;
     long long v0, whole;           // first word of this share of the vocabulary; words of all shares
     void* stream;
+    float* terms;                  // scratch of the policy loss with its gradient: [n * s, 4], n doubles, n * s + 1 ints
     double beta, smoothing, low, high;       // beta: of the preference, or the KL's weight
+    double expected;               // gradient of the loss that the forward writes its gradient for
     int n, s, vocab, dtype;
     int kl, by_sequence;
     int most, chunks;              // 0 chunks: as the statistics found
     int policy, first, second;     // which loss; whether to run the statistics and what joins them
+    int done;                      // forward: loss and gradient at once; backward: that was done
 };
 
 }  // namespace
@@ -1098,6 +1514,35 @@ int neox_loss_forward(const void* packed) {
     return launch::overlapped(preference_kernel, grid, dim3(THREADS), 1, st, a);
 }
 
+// Whether a row of that many words fits in shared memory.
+int neox_policy_fits(int vocab, int dtype) { return AtOncePlan(vocab, dtype).blocks > 0; }
+
+// The policy loss, without reference logits and over a whole vocabulary, together with its gradient for `expected`.
+int neox_policy_at_once(const void* packed) {
+    const LossCall& c = *(const LossCall*)packed;
+    const long long rows = (long long)c.n * c.s;
+    const AtOncePlan p(c.vocab, c.dtype);
+    if (c.n < 1 || c.s < 1 || c.vocab < 1 || c.y || c.kl == KL_FULL || p.blocks == 0) return NEOX_ERR_SHAPE;
+    if (rows >= (1ll << 31) - 1) return NEOX_ERR_TOO_LARGE;
+    double* whole = (double*)(c.terms + 4 * rows);
+    const AtOnceArgs a = {{c.x, c.xn, c.xs}, c.g, c.gn, c.gs, c.labels, c.mask, c.advantages, c.adv_n, c.adv_s, c.old_logp,
+                          c.ref_logp, c.n, c.s, c.vocab, c.kl, c.by_sequence, c.low, c.high, c.beta, (float)c.expected, c.row, c.slope,
+                          (float4*)c.terms, whole, (int*)(whole + c.n), c.coef, c.loss, c.kl_mean, c.clipped, c.logp};
+    cudaStream_t st = (cudaStream_t)c.stream;
+    policy_share_kernel<<<1, 1024, 0, st>>>(a);
+    if (launched() != 0) return NEOX_ERR_LAUNCH;
+    const long long most = (long long)p.blocks * neox_sm_count();
+    const dim3 grid((unsigned)(rows < most ? rows : most));
+    int rc = 0;
+    if (p.blocks == 8) FOR_TYPE(c.dtype, (rc = rows_at_once<T, 128, 8>(a, p, grid, st)));
+    else if (p.blocks == 4) FOR_TYPE(c.dtype, (rc = rows_at_once<T, 256, 4>(a, p, grid, st)));
+    else if (p.blocks == 3) FOR_TYPE(c.dtype, (rc = rows_at_once<T, 320, 3>(a, p, grid, st)));
+    else if (p.blocks == 2) FOR_TYPE(c.dtype, (rc = rows_at_once<T, 512, 2>(a, p, grid, st)));
+    else FOR_TYPE(c.dtype, (rc = rows_at_once<T, 768, 1>(a, p, grid, st)));
+    if (rc != 0) return rc;
+    return launch::overlapped(policy_mean_kernel, dim3(1), dim3(1024), 1, st, a, (int)rows);
+}
+
 int neox_loss_backward(const void* packed) {
     const LossCall& c = *(const LossCall*)packed;
     const bool full = c.shift != nullptr;
@@ -1107,10 +1552,19 @@ int neox_loss_backward(const void* packed) {
     if (rows == 0) return 0;
     if (!p.fits(rows, c.vocab)) return NEOX_ERR_TOO_LARGE;
     const GradArgs a = {{c.x, c.xn, c.xs}, {c.y, c.yn, c.ys}, c.g, c.gn, c.gs, c.labels, c.slope, c.mask, c.shift, c.row, c.coef,
-                        c.g_loss, c.g_logp, c.v0, (float)c.beta, (int)rows, c.s, c.vocab, p.splits, p.chunk};
+                        c.g_loss, c.g_logp, c.v0, (float)c.beta, (float)c.expected, (int)rows, c.s, c.vocab, p.splits,
+                        p.chunk};
     const long long per = THREADS / p.threads;
-    const unsigned grid = (unsigned)((rows * p.splits + per - 1) / per);
+    const long long items = rows * p.splits, need = (items + per - 1) / per;
     cudaStream_t st = (cudaStream_t)c.stream;
+    if (c.done) {
+        if (full || !c.g_loss) return NEOX_ERR_SHAPE;
+        const long long few = 8ll * neox_sm_count();
+        const unsigned grid = (unsigned)(need < few ? need : few);
+        FOR_TYPE(c.dtype, FOR_THREADS(p.threads, (grad_unless_kernel<T, G, U_ONE><<<grid, THREADS, 0, st>>>(a, (unsigned)items))));
+        return launched();
+    }
+    const unsigned grid = (unsigned)need;
     if (full) FOR_TYPE(c.dtype, FOR_THREADS(p.threads, (grad_kernel<T, G, U_FULL, true><<<grid, THREADS, 0, st>>>(a))));
     else FOR_TYPE(c.dtype, FOR_THREADS(p.threads, (grad_kernel<T, G, U_ONE, false><<<grid, THREADS, 0, st>>>(a))));
     return launched();

@@ -29,12 +29,14 @@ native._ARGTYPES.update({
     "neox_vocab_chunks": [ctypes.c_longlong, ctypes.c_int, ctypes.c_int, ctypes.c_int],
     "neox_loss_pieces": [ctypes.c_int],
     "neox_loss_forward": [ctypes.c_char_p],
+    "neox_policy_fits": [ctypes.c_int, ctypes.c_int],
+    "neox_policy_at_once": [ctypes.c_char_p],
     "neox_loss_backward": [ctypes.c_char_p],
 })
-native._CountingLib._NOT_LAUNCHES.update({"neox_vocab_chunks", "neox_loss_pieces"})
+native._CountingLib._NOT_LAUNCHES.update({"neox_vocab_chunks", "neox_loss_pieces", "neox_policy_fits"})
 
 # The kernels' arguments in the order of LossCall (csrc/policy_losses.cu): addresses and 64-bit words, doubles, ints.
-_CALL = struct.Struct("@35q4d11i4x")
+_CALL = struct.Struct("@36q5d12i")
 
 
 class PreferenceLoss(NamedTuple):
@@ -172,39 +174,44 @@ def _forward(x, y, labels, mask, width, loss, kl_mean, clipped, logp, ref, old_l
             0 if old_logp is None else old_logp.data_ptr(), 0 if ref_logp is None else ref_logp.data_ptr(),
             *((0, 0, 0) if adv is None else (adv.data_ptr(), adv.stride(0) if adv.shape[0] > 1 else 0,
                                              adv.stride(1) if adv.shape[1] > 1 else 0)),
-            0, 0, 0, 0, 0, rank * v, tp * v, native.stream_ptr(), beta, smoothing, low, high, n, s, v, dt, kl, by_sequence)
+            0, 0, 0, 0, 0, rank * v, tp * v, native.stream_ptr(), 0, beta, smoothing, low, high, 0.0, n, s, v, dt, kl, by_sequence)
     run = native.lib().neox_loss_forward
     policy = width == 4
     if tp == 1:
-        native.check(run(_CALL.pack(*head, part, cross, target, *tail, most, 0, policy, 1, 1)), "neox_loss_forward")
+        native.check(run(_CALL.pack(*head, part, cross, target, *tail, most, 0, policy, 1, 1, 0)), "neox_loss_forward")
     else:
-        native.check(run(_CALL.pack(*head, part, cross, target, *tail, most, 0, policy, 1, 0)), "neox_loss_forward")
+        native.check(run(_CALL.pack(*head, part, cross, target, *tail, most, 0, policy, 1, 0, 0)), "neox_loss_forward")
         pairs, targets, crosses = _reduced(buf, at, streams, n * s, most, full, group())
-        native.check(run(_CALL.pack(*head, pairs.data_ptr(), crosses.data_ptr(), targets.data_ptr(), *tail, 1, 1, policy, 0, 1)),
+        native.check(run(_CALL.pack(*head, pairs.data_ptr(), crosses.data_ptr(), targets.data_ptr(), *tail, 1, 1, policy, 0, 1, 0)),
                      "neox_loss_forward")
     return buf, rank * v
 
 
-def _backward(x, y, labels, mask, buf, first, width, streams, g_loss, g_logp, beta):
-    """Gradient of the logits, in their own memory order where that is dense.  ``y``: the reference, for the KL over the
-    vocabulary."""
-    n, s, v = x.shape
-    dt, full = _DT[x.dtype], int(y is not None)
-    _, *at, _ = _layout(n, s, v, dt, streams, width, full, x.get_device())
-    base = buf.data_ptr()
-    row, coef, slope, shift = [base + o for o in at[5:]]
+def _new_grad(x):
+    """A gradient in the logits' own memory order where that is dense."""
     g = torch.empty_like(x)
-    if g.stride(2) != 1:
-        g = torch.empty(n, s, v, dtype=x.dtype, device=x.device)
+    return g if g.stride(2) == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+def _backward(x, y, labels, mask, g, row, coef, slope, shift, first, g_loss, g_logp, beta, expected, done):
+    """Writes the gradient of the logits into ``g``.  ``y``: the reference, for the KL over the vocabulary; ``row`` to ``shift``: addresses of
+    what the forward kept; ``done``: ``g`` is already right if the gradient of the loss is ``expected``."""
+    n, s, v = x.shape
     y_ = x if y is None else y
-    weight = mask.data_ptr()
-    call = _CALL.pack(x.data_ptr(), x.stride(0), x.stride(1), y_.data_ptr(), y_.stride(0), y_.stride(1), labels.data_ptr(), weight,
-                      0, 0, 0, 0, 0, row, coef, slope if width == 4 else weight, shift if full else 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
-                      g.data_ptr(), g.stride(0), g.stride(1), 0 if g_loss is None else g_loss.data_ptr(),
-                      0 if g_logp is None else g_logp.data_ptr(), first, 0, native.stream_ptr(), beta, 0.0, 0.0, 0.0, n, s, v, dt,
-                      0, 0, 0, 0, 0, 0, 0)
+    call = _CALL.pack(x.data_ptr(), x.stride(0), x.stride(1), y_.data_ptr(), y_.stride(0), y_.stride(1), labels.data_ptr(),
+                      mask.data_ptr(), 0, 0, 0, 0, 0, row, coef, slope, shift, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, g.data_ptr(), g.stride(0),
+                      g.stride(1), 0 if g_loss is None else g_loss.data_ptr(), 0 if g_logp is None else g_logp.data_ptr(), first, 0,
+                      native.stream_ptr(), 0, beta, 0.0, 0.0, 0.0, expected, n, s, v, _DT[x.dtype], 0, 0, 0, 0, 0, 0, 0, done)
     native.check(native.lib().neox_loss_backward(call), "neox_loss_backward")
     return g
+
+
+def _kept(x, buf, streams, width, full):
+    """Addresses of what a forward kept in its buffer: row statistics, coefficients, slopes, shifts."""
+    n, s, v = x.shape
+    at = _layout(n, s, v, _DT[x.dtype], streams, width, full, x.get_device())
+    base = buf.data_ptr()
+    return base + at[6], base + at[7], base + at[8], base + at[9] if full else 0
 
 
 def _preference_values(x, labels, mask, ref_logits, ref_logp, beta, smoothing):
@@ -240,7 +247,9 @@ class _PreferenceFn(torch.autograd.Function):
             return None, None
         x, labels, mask, buf = ctx.saved_tensors
         with device_of(x):
-            g = _backward(x, None, labels, mask, buf, ctx.first, 2, ctx.streams, _grad_f32(g_loss), _grad_f32(g_logp), 0.0)
+            row, coef, _, _ = _kept(x, buf, ctx.streams, 2, 0)
+            g = _backward(x, None, labels, mask, _new_grad(x), row, coef, mask.data_ptr(), 0, ctx.first, _grad_f32(g_loss),
+                          _grad_f32(g_logp), 0.0, 0.0, 0)
         return once(g, x), None
 
 
@@ -255,14 +264,65 @@ def _policy_values(x, labels, mask, adv, old_logp, ref_logits, ref_logp, low, hi
     return loss, kl_mean, clipped, logp, kept
 
 
+@functools.lru_cache(maxsize=256)
+def _at_once_layout(n, s):
+    """As :func:`_layout`, for :func:`_policy_at_once`: ``row``, ``coef``, ``slope`` as there; ``terms`` [rows, 4], ``[n]`` fp64 and
+    ``[rows + 1]`` int32 of scratch."""
+    rows = n * s
+    sizes = (4 * rows, 2 * n, rows + 1, 2 * rows, n, rows)
+    at, offsets = 0, []
+    for size in sizes:
+        offsets.append(4 * at)
+        at += size + size % 2
+    terms, _, _, row, coef, slope = offsets
+    return row, coef, slope, terms, at
+
+
+def _policy_at_once(x, labels, mask, adv, old_logp, ref_logp, low, high, kl, kl_beta, by_sequence, expected):
+    """The policy loss and, from the same reading of the logits, its gradient for a gradient ``expected`` of the loss."""
+    n, s, v = x.shape
+    dev = x.device
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    kl_mean = torch.empty((), dtype=torch.float32, device=dev)
+    clipped = torch.empty((), dtype=torch.float32, device=dev)
+    logp = torch.empty(n, s, dtype=torch.float32, device=dev)
+    *at, total = _at_once_layout(n, s)
+    buf = torch.empty(total, dtype=torch.float32, device=dev)
+    row, coef, slope, terms = [buf.data_ptr() + o for o in at]
+    g = _new_grad(x)
+    call = _CALL.pack(x.data_ptr(), x.stride(0), x.stride(1), 0, 0, 0, labels.data_ptr(), mask.data_ptr(), 0, 0, 0, 0, 0, row, coef,
+                      slope, 0, loss.data_ptr(), kl_mean.data_ptr(), clipped.data_ptr(), logp.data_ptr(), 0,
+                      0 if old_logp is None else old_logp.data_ptr(), 0 if ref_logp is None else ref_logp.data_ptr(),
+                      adv.data_ptr(), adv.stride(0) if adv.shape[0] > 1 else 0, adv.stride(1) if adv.shape[1] > 1 else 0,
+                      g.data_ptr(), g.stride(0), g.stride(1), 0, 0, 0, v, native.stream_ptr(), terms, kl_beta, 0.0, low, high,
+                      expected, n, s, v, _DT[x.dtype], kl, by_sequence, 0, 0, 1, 0, 0, 1)
+    native.check(native.lib().neox_policy_at_once(call), "neox_policy_at_once")
+    return loss, kl_mean, clipped, logp, buf, g
+
+
+@functools.lru_cache(maxsize=256)
+def _one_reading_pays(vocab, dtype):
+    """A row that keeps a block busy and fits in shared memory; others are read twice."""
+    return vocab * dtype.itemsize >= 16384 and bool(native.lib().neox_policy_fits(vocab, _DT[dtype]))
+
+
 class _PolicyFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, rest):
-        labels, mask, _, _, ref_logits, _, _, _, kl, kl_beta, _ = rest
+        labels, mask, adv, old_logp, ref_logits, ref_logp, low, high, kl, kl_beta, by_sequence, expected = rest
+        # 16-bit floating-point numbers of five exponent bits need the loss scale before they are rounded
+        at_once = x.shape[1] > 0 and _tensor_parallel()[0] == 1 and (x.dtype != torch.float16 or expected != 1.0) \
+            and ref_logits is None and _one_reading_pays(x.shape[2], x.dtype)
+        ctx.full, ctx.kl_beta, ctx.expected, ctx.first, ctx.grad = int(kl == KL_KINDS["full"]), kl_beta, expected, 0, None
         with device_of(x):
-            loss, kl_mean, clipped, logp, (buf, ctx.first) = _policy_values(x, *rest)
-        ctx.streams, ctx.kl_beta = 1 if ref_logits is None else 2, kl_beta
-        ctx.save_for_backward(x, labels, mask, buf, ref_logits if kl == KL_KINDS["full"] else None)
+            if at_once:
+                loss, kl_mean, clipped, logp, buf, ctx.grad = _policy_at_once(x, labels, mask, adv, old_logp, ref_logp, low, high, kl, kl_beta,
+                                                                              by_sequence, expected)
+                ctx.streams = 0
+            else:
+                loss, kl_mean, clipped, logp, (buf, ctx.first) = _policy_values(x, *rest[:-1])
+                ctx.streams = 1 if ref_logits is None else 2
+        ctx.save_for_backward(x, labels, mask, buf, ref_logits if ctx.full else None)
         ctx.mark_non_differentiable(kl_mean, clipped, logp)
         ctx.set_materialize_grads(False)
         return loss, kl_mean, clipped, logp
@@ -272,8 +332,17 @@ class _PolicyFn(torch.autograd.Function):
         if g_loss is None:
             return None, None
         x, labels, mask, buf, y = ctx.saved_tensors
+        # handed out once: a second backward through a retained graph writes another
+        g, ctx.grad = ctx.grad, None
+        done = g is not None
         with device_of(x):
-            g = _backward(x, y, labels, mask, buf, ctx.first, 4, ctx.streams, _grad_f32(g_loss), None, ctx.kl_beta)
+            if ctx.streams:
+                row, coef, slope, shift = _kept(x, buf, ctx.streams, 4, ctx.full)
+            else:
+                row, coef, slope = (buf.data_ptr() + o for o in _at_once_layout(x.shape[0], x.shape[1])[:3])
+                shift = 0
+            g = _backward(x, y, labels, mask, g if done else _new_grad(x), row, coef, slope, shift, ctx.first, _grad_f32(g_loss), None,
+                          ctx.kl_beta, ctx.expected, done)
         return once(g, x), None
 
 
@@ -399,7 +468,8 @@ def preference_loss(logits, labels, loss_mask, beta, ref_logits: Optional[torch.
 
 def policy_loss(logits, labels, loss_mask, advantages, old_logp: Optional[torch.Tensor] = None,
                 ref_logits: Optional[torch.Tensor] = None, ref_logp: Optional[torch.Tensor] = None, clip_low: float = 0.2,
-                clip_high: Optional[float] = None, kl: str = "k3", kl_beta: float = 0.0, reduce: str = "token") -> PolicyLoss:
+                clip_high: Optional[float] = None, kl: str = "k3", kl_beta: float = 0.0, reduce: str = "token",
+                grad_scale: float = 1.0) -> PolicyLoss:
     """Clipped policy loss with a KL term.  With ``l`` the log-probability of a label, ``A`` its advantage::
 
         r = exp(l - old_logp)                                      (1 without old_logp: the policy that sampled is the present one)
@@ -412,6 +482,12 @@ def policy_loss(logits, labels, loss_mask, advantages, old_logp: Optional[torch.
 
     ``logits``, ``labels``, ``loss_mask``, ``ref_logits``, ``ref_logp`` as in :func:`preference_loss`; ``advantages``: ``[n, s]``, or
     ``[n]`` for one a sequence; ``old_logp``: ``[n, s]``.  All but ``logits`` are constants.
+
+    ``grad_scale`` is the gradient of the loss that the backward is expected to start from: 1 for ``loss.backward()``, a loss scale or
+    ``1 / accumulation steps`` for a scaled loss.  Where the logits ask for a gradient, it is computed for that value together with
+    the loss, while a row is at hand, and the backward only has to look; any other gradient of the loss is right as well, and
+    costs the second reading of the logits that was to be saved.  (With reference logits, with fp16 logits and ``grad_scale`` 1, and
+    for vocabularies that are short, split over ranks or too long for shared memory, logits are always read twice.)
     """
     _check(logits, labels, loss_mask, ref_logits, ref_logp)
     n, s = logits.shape[:2]
@@ -443,10 +519,10 @@ def policy_loss(logits, labels, loss_mask, advantages, old_logp: Optional[torch.
     kind = KL_KINDS[kl] if ref_logits is not None or ref_logp is not None else 0
     x = _rows(logits)
     rest = (_as(labels, torch.int64), _as(loss_mask, torch.float32), advantages, _as(old_logp, torch.float32), _rows(ref_logits),
-            _as(ref_logp, torch.float32), 1.0 - clip_low, 1.0 + clip_high, kind, float(kl_beta), reduce == "sequence")
+            _as(ref_logp, torch.float32), 1.0 - clip_low, 1.0 + clip_high, kind, float(kl_beta), reduce == "sequence", float(grad_scale))
     if native.plain_call(logits):
         with device_of(x):
-            loss, mean_kl, clipped, logp = _policy_values(x, *rest)[:4]
+            loss, mean_kl, clipped, logp = _policy_values(x, *rest[:-1])[:4]
     else:
         loss, mean_kl, clipped, logp = _PolicyFn.apply(x, rest)
     return PolicyLoss(loss, logp, mean_kl, clipped)

@@ -109,7 +109,8 @@ def test_preference_loss_matches_its_formula(n, s, v, dtype, order):
 @pytest.mark.parametrize("n,s,v,dtype,order", [
     (1, 1, 9, torch.float32, "bsv"), (3, 5, 64, torch.bfloat16, "sbv"), (2, 300, 1031, torch.float16, "shifted"),
     (3, 4, 8200, torch.float32, "padded"), (2, 7, 50257, torch.bfloat16, "bsv"), (1, 6, 32000, torch.float16, "strided"),
-    (5, 3, 1025, torch.bfloat16, "padded")])
+    (5, 3, 1025, torch.bfloat16, "padded"), (2, 400, 8200, torch.bfloat16, "sbv"), (3, 70, 12001, torch.float32, "shifted"),
+    (2, 90, 128256, torch.bfloat16, "bsv"), (40, 9, 9001, torch.float16, "padded")])
 def test_policy_loss_matches_its_formula(n, s, v, dtype, order, kl, reduce):
     seed = n * 11 + s + v
     x, labels = _logits(n, s, v, dtype, order, seed)
@@ -130,7 +131,9 @@ def test_policy_loss_matches_its_formula(n, s, v, dtype, order, kl, reduce):
     beta, scale = 0.25, 32.0
     args = dict(clip_low=0.2, clip_high=0.3, kl="k3" if kl == "none" else kl, kl_beta=beta, reduce=reduce)
     x = x.detach().requires_grad_()
-    out = PL.policy_loss(x, labels, mask, adv, old_logp=old, ref_logits=ref_logits, ref_logp=ref_logp, **args)
+    # the gradient that the forward foresees, and another one
+    out = PL.policy_loss(x, labels, mask, adv, old_logp=old, ref_logits=ref_logits, ref_logp=ref_logp, **args,
+                         grad_scale=scale if reduce == "token" else 1.0)
     grad, = torch.autograd.grad(out.loss, x, torch.tensor(scale, device=DEV))
     xd = x.detach().double().requires_grad_()
     wide = lambda t: None if t is None else t.double()             # noqa: E731
@@ -261,7 +264,7 @@ def test_losses_of_batches_that_keep_nothing():
     assert float(PL.policy_loss(y, short, none[:, :0], none[:, :0]).loss.detach()) == 0.0
 
 
-@pytest.mark.parametrize("op", ["preference", "policy", "full", "router"])
+@pytest.mark.parametrize("op", ["preference", "policy", "foreseen", "full", "router"])
 def test_losses_repeat_bit_by_bit_on_any_stream_and_in_graphs(op):
     """The same inputs give the same bits: again, on another stream, with a second call in between, and replayed from a CUDA graph
     whose inputs have changed since it was captured."""
@@ -277,8 +280,8 @@ def test_losses_repeat_bit_by_bit_on_any_stream_and_in_graphs(op):
         if op == "preference":
             out = PL.preference_loss(x, labels, mask, 0.1, ref_logits=ref)
             outs = [out.loss, out.logp]
-        elif op == "policy":
-            outs = [PL.policy_loss(x, labels, mask, mask, ref_logits=ref, kl_beta=0.1).loss]
+        elif op in ("policy", "foreseen"):
+            outs = [PL.policy_loss(x, labels, mask, mask, ref_logits=ref, kl_beta=0.1, grad_scale=1.0 if op == "foreseen" else 2.0).loss]
         elif op == "full":
             outs = [PL.policy_loss(x, labels, mask, mask, ref_logits=ref, kl="full", kl_beta=0.1).loss]
         else:
@@ -338,6 +341,36 @@ def test_loss_gradients_reach_what_asked_for_them():
         x.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         out.loss.backward()
+
+
+@pytest.mark.parametrize("kl", ["k3", "full"])
+def test_a_policy_gradient_is_right_whatever_was_foreseen(kl):
+    """The gradient for the foreseen gradient of the loss, for another one, and again through a retained graph; each a tensor of its
+    own, and accumulated in ``.grad`` as it should be."""
+    x, labels = _logits(2, 20, 9000, torch.float32)
+    ref, mask = x + 0.3 * torch.randn_like(x), _mask(2, 20, 2)
+    x.requires_grad_()
+    loss = lambda scale: PL.policy_loss(x, labels, mask, mask, ref_logits=ref, kl=kl, kl_beta=0.2, grad_scale=scale).loss  # noqa: E731
+    one = loss(1.0)
+    first, = torch.autograd.grad(one, x, retain_graph=True)
+    kept = first.clone()
+    again, = torch.autograd.grad(one, x, retain_graph=True)
+    twice, = torch.autograd.grad(one, x, torch.tensor(2.0, device=DEV))
+    assert first.data_ptr() != again.data_ptr() and torch.equal(first, kept)
+    # the same formula from statistics that were joined in another order: some roundings of numbers up to the coefficient
+    top = kept.abs().max()
+    _near(again, kept.double(), 2.0 ** -18 * top, "again")
+    assert torch.equal(twice, 2 * again)                         # a power of two
+    other, = torch.autograd.grad(loss(4.0), x)
+    _near(other, kept.double(), 2.0 ** -18 * top, "not foreseen")
+    scaled, = torch.autograd.grad(loss(4.0), x, torch.tensor(4.0, device=DEV))
+    assert torch.equal(scaled, 4 * kept)
+    for want in (1, 2):
+        one = loss(1.0)
+        one.backward(retain_graph=True)
+        _near(x.grad, want * kept.double(), want * 2.0 ** -18 * top, "accumulated")
+    one.backward()
+    _near(x.grad, 3 * kept.double(), 3 * 2.0 ** -18 * top, "accumulated from a retained graph")
 
 
 @pytest.mark.parametrize("full", [False, True])
