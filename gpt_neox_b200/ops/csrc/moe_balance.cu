@@ -525,7 +525,7 @@ int neox_router_blocks(long long tokens, int E, int dtype) { return RouterPlan(t
 int neox_balanced_router(const void* x, long long stride, const void* kept, int tokens, int E, int k, int dtype, float* weights,
                          long long* experts, void* row, long long* counts, float* load, float* balance, float* z_loss, void* scratch,
                          void* stream) {
-    if (tokens < 0 || E < 1 || E > 512 || k < 1 || k > MAX_K || k > E) return NEOX_ERR_SHAPE;
+    if (tokens < 0 || tokens >= 1 << 30 || E < 1 || E > 512 || k < 1 || k > MAX_K || k > E) return NEOX_ERR_SHAPE;
     const RouterPlan plan(tokens, E, dtype);
     const int blocks = plan.blocks;
     double* z = (double*)scratch;
@@ -546,7 +546,7 @@ int neox_balanced_router(const void* x, long long stride, const void* kept, int 
 int neox_balanced_router_grad(const void* x, long long stride, const void* kept, int tokens, int E, int k, int dtype,
                               const float* weights, const long long* experts, const void* row, const float* load,
                               const float* g_weights, const float* g_balance, const float* g_z, void* dx, void* stream) {
-    if (tokens < 0 || E < 1 || E > 512 || k < 1 || k > MAX_K || k > E) return NEOX_ERR_SHAPE;
+    if (tokens < 0 || tokens >= 1 << 30 || E < 1 || E > 512 || k < 1 || k > MAX_K || k > E) return NEOX_ERR_SHAPE;
     if (tokens == 0) return 0;
     const BackwardArgs b = {x, stride, (const uint8_t*)kept, weights, experts, (const float4*)row, load, g_weights, g_balance, g_z,
                             dx, tokens, E, k, rows_aligned(x, stride, E, dtype)};

@@ -327,8 +327,8 @@ template <typename T, bool FULL> struct Walk {
 };
 
 // What a lane has of a chunk so far: the largest logit and the sums against it.
-// PAIR: the reference's sums too; CROSS: and the sum of p (x - y).  U vectors at a time, STRIDE of them apart.
-template <typename T, bool PAIR, bool CROSS, int U, int STRIDE> struct Running {
+// FULL: the reference's sums too, and the sum of p (x - y).  U vectors at a time, STRIDE of them apart.
+template <typename T, bool FULL, int U, int STRIDE> struct Running {
     static constexpr int N = Elem<T>::PER_16;
     float m, n;                    // policy, reference
     f32x2 t, r, w;                 // sum of exponentials (policy, reference), sum of p (x - y)
@@ -342,23 +342,23 @@ template <typename T, bool PAIR, bool CROSS, int U, int STRIDE> struct Running {
         const float k = __expf(m - px);
         m = px;
         t = mul(t, pair(k, k));
-        if constexpr (PAIR) {
+        if constexpr (FULL) {
             const float kr = __expf(n - qx);
             n = qx;
             r = mul(r, pair(kr, kr));
-            if constexpr (CROSS) w = mul(w, pair(k, k));
+            w = mul(w, pair(k, k));
         }
     }
-    __device__ __forceinline__ void add_vectors(const uint4 (&xr)[U], const uint4 (&yr)[PAIR ? U : 1], int left, bool whole) {
+    __device__ __forceinline__ void add_vectors(const uint4 (&xr)[U], const uint4 (&yr)[FULL ? U : 1], int left, bool whole) {
         uint32_t p = larger<T>(xr[0]), q = 0;
-        if constexpr (PAIR) q = larger<T>(yr[0]);
+        if constexpr (FULL) q = larger<T>(yr[0]);
 #pragma unroll
         for (int u = 1; u < U; ++u)
             if (whole || u * STRIDE < left) {
                 p = larger(p, larger<T>(xr[u]), T());
-                if constexpr (PAIR) q = larger(q, larger<T>(yr[u]), T());
+                if constexpr (FULL) q = larger(q, larger<T>(yr[u]), T());
             }
-        const float px = as_max<T>(p), qx = PAIR ? as_max<T>(q) : n;
+        const float px = as_max<T>(p), qx = FULL ? as_max<T>(q) : n;
         if (px > m || qx > n) raise(fmaxf(m, px), fmaxf(n, qx));
         const f32x2 xs = pair(-m, -m), ys = pair(-n, -n), minus = pair(-1.f, -1.f);
         f32x2 gap = pair(0.f, 0.f);
@@ -366,7 +366,7 @@ template <typename T, bool PAIR, bool CROSS, int U, int STRIDE> struct Running {
         for (int u = 0; u < U; ++u)
             if (whole || u * STRIDE < left) {
                 f32x2 e[N / 2];
-                if constexpr (CROSS) {
+                if constexpr (FULL) {
                     f32x2 v[N / 2], q2[N / 2];
                     pairs_of<T>(xr[u], v);
                     pairs_of<T>(yr[u], q2);
@@ -377,17 +377,12 @@ template <typename T, bool PAIR, bool CROSS, int U, int STRIDE> struct Running {
                         r = add(r, exp_of(q2[i], ys));
                     }
                 } else {
-                    if constexpr (PAIR) {
-                        exps_of<T>(yr[u], n, e);
-#pragma unroll
-                        for (int i = 0; i < N / 2; ++i) r = add(r, e[i]);
-                    }
                     exps_of<T>(xr[u], m, e);
                 }
 #pragma unroll
                 for (int i = 0; i < N / 2; ++i) t = add(t, e[i]);
             }
-        if constexpr (CROSS) {
+        if constexpr (FULL) {
             const float2 g = parts(gap);
             if (g.x + g.y != g.x + g.y) {                       // 0 times infinity somewhere: what is impossible adds nothing
                 float again = 0.f;
@@ -409,11 +404,13 @@ template <typename T, bool PAIR, bool CROSS, int U, int STRIDE> struct Running {
         }
     }
     __device__ __forceinline__ void add_one(float ex, float ey) {
-        raise(fmaxf(m, ex), PAIR ? fmaxf(n, ey) : 0.f);
+        raise(fmaxf(m, ex), FULL ? fmaxf(n, ey) : 0.f);
         const float e = __expf(ex - m);
         t = add(t, pair(e, 0.f));
-        if constexpr (CROSS) w = add(w, pair(e > 0.f ? e * (ex - ey) : 0.f, 0.f));
-        if constexpr (PAIR) r = add(r, pair(__expf(ey - n), 0.f));
+        if constexpr (FULL) {
+            w = add(w, pair(e > 0.f ? e * (ex - ey) : 0.f, 0.f));
+            r = add(r, pair(__expf(ey - n), 0.f));
+        }
     }
 };
 
@@ -496,7 +493,7 @@ __global__ void __launch_bounds__(Shape<FULL>::WARPS * 32, 1) stats_kernel(const
         W ahead, now;                                           // the walk of the copies and that of the sums
         ahead.item = now.item = lo + warp;
         unsigned taken = 0, begun = 0;
-        Running<T, FULL, FULL, U, 32> run;
+        Running<T, FULL, U, 32> run;
         run.clear();
         if (now.item < hi) {
             ahead.enter(a, sm.list, first, chunks, chunk);
@@ -662,6 +659,26 @@ __device__ __forceinline__ bool last_block(int* ticket) {
     return last;
 }
 
+// Sums of every sequence's pieces, V values each, by as many neighbouring lanes as leave each four loads; `leave` gets them in one.
+template <int V, typename F> __device__ __forceinline__ void sum_pieces(const double* partial, int n, int pieces, F&& leave) {
+    int lanes = 1;
+    while (lanes < 32 && 4 * lanes < pieces) lanes *= 2;
+    const int place = threadIdx.x % lanes;
+    for (int first = 0; first < n; first += THREADS / lanes) {
+        const int i = first + threadIdx.x / lanes;
+        double p[V] = {};
+        if (i < n)
+#pragma unroll 4
+            for (int k = place; k < pieces; k += lanes)
+#pragma unroll
+                for (int q = 0; q < V; ++q) p[q] += __ldcg(partial + V * ((long long)i * pieces + k) + q);
+        for (int o = lanes / 2; o > 0; o >>= 1)
+#pragma unroll
+            for (int q = 0; q < V; ++q) p[q] += __shfl_xor_sync(0xffffffffu, p[q], o);
+        if (i < n && place == 0) leave(i, p);
+    }
+}
+
 struct PreferenceArgs {
     RowSums sums;
     const float* mask;
@@ -706,34 +723,24 @@ __global__ void __launch_bounds__(THREADS) preference_kernel(const PreferenceArg
     }
     block_sum(v);
     if (threadIdx.x == 0) {
-        a.partial[2 * blockIdx.x] = v[0];
-        a.partial[2 * blockIdx.x + 1] = v[1];
+        a.partial[2ll * blockIdx.x] = v[0];
+        a.partial[2ll * blockIdx.x + 1] = v[1];
     }
     if (!last_block(a.ticket)) return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     __shared__ double near[2 * NEAR];
     double* whole = a.n <= NEAR ? near : a.partial + 2ll * gridDim.x;
-    for (int i = warp; i < a.n; i += THREADS / 32) {
-        double p = 0.0, r = 0.0;
-        for (int k = lane; k < a.pieces; k += 32) {
-            p += __ldcg(a.partial + 2ll * (i * a.pieces + k));
-            r += __ldcg(a.partial + 2ll * (i * a.pieces + k) + 1);
-        }
-        p = warp_sum(p);
-        r = warp_sum(r);
-        if (lane == 0) {
-            whole[2 * i] = p;
-            whole[2 * i + 1] = r;
-            a.logp[i] = (float)p;
-            a.ref[i] = (float)r;
-        }
-    }
+    sum_pieces<2>(a.partial, a.n, a.pieces, [&](int i, const double (&p)[2]) {
+        whole[2ll * i] = p[0];
+        whole[2ll * i + 1] = p[1];
+        a.logp[i] = (float)p[0];
+        a.ref[i] = (float)p[1];
+    });
     __syncthreads();
     const int pairs = a.n / 2;
     double sum[1] = {0.0};
     for (int b = threadIdx.x; b < pairs; b += THREADS) {
-        const double* c = whole + 2 * b;
-        const double* r = whole + 2 * (b + pairs);
+        const double* c = whole + 2ll * b;
+        const double* r = whole + 2ll * (b + pairs);
         const double z = a.beta * ((c[0] - r[0]) - (c[1] - r[1]));
         const float small = __expf(-fabsf((float)z)), soft = log1pf(small), even = (float)a.smoothing;
         double loss = (1.0 - a.smoothing) * (soft + fmax(-z, 0.0));
@@ -868,29 +875,21 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(const PolicyArgs a) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) a.partial[4ll * blockIdx.x + k] = v[k];
     if (!last_block(a.ticket)) return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     __shared__ double near[4 * NEAR];
     double* whole = a.n <= NEAR ? near : a.partial + 4ll * gridDim.x;
-    for (int i = warp; i < a.n; i += THREADS / 32) {
-        double p[4] = {0.0, 0.0, 0.0, 0.0};
-        for (int k = lane; k < a.pieces; k += 32)
+    sum_pieces<4>(a.partial, a.n, a.pieces, [&](int i, const double (&p)[4]) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) p[q] += __ldcg(a.partial + 4ll * (i * a.pieces + k) + q);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) p[q] = warp_sum(p[q]);
-        if (lane == 0)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) whole[4 * i + q] = p[q];
-    }
+        for (int q = 0; q < 4; ++q) whole[4ll * i + q] = p[q];
+    });
     __syncthreads();
     // mask, term, KL, clipped, sequences with a kept token, their mean terms
     double sum[6] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
     for (int i = threadIdx.x; i < a.n; i += THREADS) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) sum[q] += whole[4 * i + q];
-        if (whole[4 * i] > 0.0) {
+        for (int q = 0; q < 4; ++q) sum[q] += whole[4ll * i + q];
+        if (whole[4ll * i] > 0.0) {
             sum[4] += 1.0;
-            sum[5] += whole[4 * i + 1] / whole[4 * i];
+            sum[5] += whole[4ll * i + 1] / whole[4ll * i];
         }
     }
     block_sum(sum);
@@ -905,7 +904,7 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(const PolicyArgs a) {
     }
     __syncthreads();
     for (int i = threadIdx.x; i < a.n; i += THREADS) {
-        const double len = a.by_sequence ? whole[4 * i] * filled : total;
+        const double len = a.by_sequence ? whole[4ll * i] * filled : total;
         a.coef[i] = len > 0.0 || (!a.by_sequence && len != 0.0) ? (float)(1.0 / len) : 0.f;
     }
 }
@@ -935,10 +934,9 @@ __device__ __forceinline__ float grad_of(float x, float y, float m, float scale,
     else return e * scale;
 }
 
-// What a row's gradient is made of: dx[c] = coef [c == label] + exp(x - m) (scale + bscale ((x - y) - shift)).
+// What the gradient of a row in shared memory is made of: dx[c] = coef [c == label] + exp(x - m) scale.
 struct RowGrad {
-    float m, coef, scale, bscale, shift;
-    bool zero;                     // all of it is
+    float m, coef, scale;
 };
 
 // exp(x - m) * scale at the elements of 16 bytes.
@@ -967,7 +965,7 @@ template <typename T, int G> __device__ __forceinline__ void write_zeros(T* g, i
 }
 template <typename T, int G> __device__ __forceinline__ void write_apart(const T* x, T* g, int count, int lane, const RowGrad& r, int label) {
     for (int c = lane; c < count; c += G) {
-        float v = r.zero ? 0.f : grad_of<T, false>(Elem<T>::get(x[c]), 0.f, r.m, r.scale, 0.f, 0.f);
+        float v = grad_of<T, false>(Elem<T>::get(x[c]), 0.f, r.m, r.scale, 0.f, 0.f);
         if (c == label) v += r.coef;
         g[c] = Elem<T>::put(v);
     }
@@ -1092,31 +1090,52 @@ struct AtOnceArgs {
 };
 
 // What each sequence's slopes are multiplied by: 1 / (sum of the mask), of the whole batch or of the sequence and then shared by the
-// sequences that keep something; and the order of the rows.  One block; several warps a sequence where there are few.
-__global__ void __launch_bounds__(1024) policy_share_kernel(const AtOnceArgs a) {
-    __shared__ double near[32];
+// sequences that keep something; and the order of the rows.  One block; what it does takes as long as three trips to memory or, for
+// many rows, as two readings of the mask.
+__global__ void __launch_bounds__(1024, 1) policy_share_kernel(const AtOnceArgs a) {
+    __shared__ double near[32][2];
     __shared__ int kept_by[32];
     launch::let_successor_start();
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, rows = a.n * a.s;
-    const int each = a.n >= 32 ? 1 : 32 / a.n, teams = 32 / each;            // warps of a sequence, sequences at a time
-    double total = 0.0, filled = 0.0;
-    for (int first = 0; first < a.n; first += teams) {
-        const int i = first + warp / each, piece = warp % each;
-        double w = 0.0;
-        if (warp / each < teams && i < a.n)
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, rows = a.n * a.s;
+    int each = 1;                                                            // threads of a sequence, a power of two
+    while (each < 32 && each < a.s) each *= 2;
+    while (each < 1024 && each < a.s && a.n <= 512 / each) each *= 2;
+    const int place = tid % each;
+    double total = 0.0, filled = 0.0, w = 0.0;
+    for (int first = 0; first < a.n; first += 1024 / each) {
+        const int i = first + tid / each;
+        w = 0.0;
+        if (i < a.n)
 #pragma unroll 8
-            for (int j = piece * 32 + lane; j < a.s; j += each * 32) w += a.mask[(long long)i * a.s + j];
-        w = warp_sum(w);
-        __syncthreads();
-        if (lane == 0) near[warp] = w;
-        __syncthreads();
-        for (int t = 0; t < teams && first + t < a.n; ++t) {                 // all threads, the same order
-            double sum = 0.0;
-            for (int q = 0; q < each; ++q) sum += near[t * each + q];
-            total += sum;
-            filled += sum > 0.0 ? 1.0 : 0.0;
-            if (threadIdx.x == 0) a.whole[first + t] = sum;
+            for (int j = place; j < a.s; j += each) w += a.mask[(long long)i * a.s + j];
+        for (int o = min(each, 32) / 2; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+        if (each > 32) {                                                     // there is one round
+            if (lane == 0) near[warp][0] = w;
+            __syncthreads();
+            w = 0.0;
+            if (place == 0)
+                for (int q = 0; q < each / 32; ++q) w += near[warp + q][0];
         }
+        if (place == 0 && i < a.n) {
+            a.whole[i] = w;
+            total += w;
+            filled += w > 0.0 ? 1.0 : 0.0;
+        }
+    }
+    total = warp_sum(total);
+    filled = warp_sum(filled);
+    __syncthreads();
+    if (lane == 0) {
+        near[warp][0] = total;
+        near[warp][1] = filled;
+    }
+    __syncthreads();
+    total = warp_sum(near[lane][0]);                                         // in every thread, in the same order
+    filled = warp_sum(near[lane][1]);
+    for (int i = tid / each; i < a.n; i += 1024 / each) {                    // sums that this thread has left itself
+        if (place != 0) break;
+        const double len = a.by_sequence ? (a.n > 1024 / each ? a.whole[i] : w) * filled : total;
+        a.coef[i] = len > 0.0 || (!a.by_sequence && len != 0.0) ? (float)(1.0 / len) : 0.f;
     }
     // the rows in a warp's part of them: kept ones counted, then placed from the front, the others behind all kept ones
     const int part = ((rows + 31) / 32 + 31) / 32 * 32, from = min(rows, warp * part), to = min(rows, from + part);
@@ -1136,19 +1155,23 @@ __global__ void __launch_bounds__(1024) policy_share_kernel(const AtOnceArgs a) 
         kept += kept_by[q];
     }
     int front = before, back = kept + from - before;
-    for (int r = from; r < to; r += 32) {
-        const bool in = r + lane < to, is = in && a.mask[r + lane] != 0.f;
-        const unsigned all = __ballot_sync(0xffffffffu, is), none = __ballot_sync(0xffffffffu, in && !is), below = (1u << lane) - 1;
-        if (is) a.order[front + __popc(all & below)] = r + lane;
-        else if (in) a.order[back + __popc(none & below)] = r + lane;
-        front += __popc(all);
-        back += __popc(none);
+    for (int r = from; r < to; r += 32 * SCAN) {
+        float w[SCAN];
+#pragma unroll
+        for (int k = 0; k < SCAN; ++k) w[k] = r + k * 32 + lane < to ? a.mask[r + k * 32 + lane] : 0.f;
+#pragma unroll
+        for (int k = 0; k < SCAN; ++k) {
+            const int row = r + k * 32 + lane;
+            const bool in = row < to, is = in && w[k] != 0.f;
+            const unsigned all = __ballot_sync(0xffffffffu, is), none = __ballot_sync(0xffffffffu, in && !is);
+            const unsigned below = (1u << lane) - 1;
+            if (is) a.order[front + __popc(all & below)] = row;
+            else if (in) a.order[back + __popc(none & below)] = row;
+            front += __popc(all);
+            back += __popc(none);
+        }
     }
-    if (threadIdx.x == 0) a.order[rows] = kept;
-    for (int i = threadIdx.x; i < a.n; i += 1024) {
-        const double len = a.by_sequence ? a.whole[i] * filled : total;
-        a.coef[i] = len > 0.0 || (!a.by_sequence && len != 0.0) ? (float)(1.0 / len) : 0.f;
-    }
+    if (tid == 0) a.order[rows] = kept;
 }
 
 // A block walks over its rows.  A thread copies its own vectors of a row to shared memory, takes them for the sums as they arrive, and
@@ -1228,7 +1251,7 @@ __global__ void __launch_bounds__(TPB, BLOCKS) policy_row_kernel(const AtOnceArg
         if (tid < now.head) edge = tid;
         else if (tid - N < tail && tid >= N) edge = now.head + now.vectors * N + tid - N;
         const float ex = edge >= 0 ? Elem<T>::get(x[edge]) : 0.f;
-        Running<T, false, false, U, TPB> run;
+        Running<T, false, U, TPB> run;
         run.clear();
         if (edge >= 0) run.add_one(ex, 0.f);
 #pragma unroll
@@ -1265,7 +1288,7 @@ __global__ void __launch_bounds__(TPB, BLOCKS) policy_row_kernel(const AtOnceArg
                 const double l = label_logp(a.vocab, label, own, m, t);
                 const RowTerm r(a.kl, a.low, a.high, a.kl_beta, l, a.old_logp != nullptr, old, adv, given, 0.0);
                 const float slope = (float)(weight * r.slope), inv = __frcp_rn((float)t), coef = per * slope;
-                grad = RowGrad{m, coef, -coef * inv, 0.f, 0.f, coef == 0.f};
+                grad = RowGrad{m, coef, -coef * inv};
                 where = (int)label;                             // one that does not fit has made everything NaN
                 a.row[row] = make_float2(m, inv);
                 a.slope[row] = slope;
@@ -1423,6 +1446,7 @@ int rows_at_once(const AtOnceArgs& a, const AtOncePlan& p, dim3 grid, cudaStream
     stats_kernel<T, FULL><<<blocks, Shape<FULL>::WARPS * 32, sizeof(StatsSmem<FULL>), st>>>(a)
 
 constexpr int U_ONE = 8, U_FULL = 4;
+constexpr long long MOST_TOKENS = 1ll << 30;                    // row numbers and steps past the last one stay within 32 bits
 
 int launched() { return cudaGetLastError() == cudaSuccess ? 0 : NEOX_ERR_LAUNCH; }
 
@@ -1488,7 +1512,7 @@ int neox_loss_forward(const void* packed) {
     const long long rows = (long long)c.n * c.s, pieces = neox_loss_pieces(c.s);
     const int streams = !full && c.y ? 2 : 1;
     if (c.n < (c.policy ? 1 : 2) || (!c.policy && c.n % 2) || c.s < 0 || c.vocab < 1 || (full && !c.y)) return NEOX_ERR_SHAPE;
-    if (rows * streams * c.most >= (1ll << 31) || c.n * pieces >= (1ll << 31)) return NEOX_ERR_TOO_LARGE;
+    if (rows >= MOST_TOKENS || rows * streams * c.most >= (1ll << 31) || c.n * pieces >= (1ll << 31)) return NEOX_ERR_TOO_LARGE;
     cudaStream_t st = (cudaStream_t)c.stream;
     if (c.first) {
         const StatsPlan p(rows, c.vocab, c.dtype, full);
@@ -1523,7 +1547,7 @@ int neox_policy_at_once(const void* packed) {
     const long long rows = (long long)c.n * c.s;
     const AtOncePlan p(c.vocab, c.dtype);
     if (c.n < 1 || c.s < 1 || c.vocab < 1 || c.y || c.kl == KL_FULL || p.blocks == 0) return NEOX_ERR_SHAPE;
-    if (rows >= (1ll << 31) - 1) return NEOX_ERR_TOO_LARGE;
+    if (rows >= MOST_TOKENS) return NEOX_ERR_TOO_LARGE;
     double* whole = (double*)(c.terms + 4 * rows);
     const AtOnceArgs a = {{c.x, c.xn, c.xs}, c.g, c.gn, c.gs, c.labels, c.mask, c.advantages, c.adv_n, c.adv_s, c.old_logp,
                           c.ref_logp, c.n, c.s, c.vocab, c.kl, c.by_sequence, c.low, c.high, c.beta, (float)c.expected, c.row, c.slope,

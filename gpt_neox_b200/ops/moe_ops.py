@@ -198,6 +198,8 @@ def balanced_router(logits, k, token_mask=None):
         raise ValueError(f"router logits are [tokens, experts] floating-point numbers, got {tuple(logits.shape)} {logits.dtype}")
     if not 1 <= k <= logits.shape[1]:
         raise ValueError(f"top-k is between 1 and the number of experts, got {k} of {logits.shape[1]}")
+    if logits.shape[0] >= 1 << 30:
+        raise ValueError(f"a router takes fewer than {1 << 30} tokens, got {logits.shape[0]}")
     if token_mask is not None:
         if token_mask.shape != logits.shape[:1] or token_mask.dtype != torch.bool:
             raise ValueError(f"token_mask is bool [{logits.shape[0]}], got {token_mask.dtype} {tuple(token_mask.shape)}")

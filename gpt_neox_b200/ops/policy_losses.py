@@ -35,6 +35,8 @@ native._ARGTYPES.update({
 })
 native._CountingLib._NOT_LAUNCHES.update({"neox_vocab_chunks", "neox_loss_pieces", "neox_policy_fits"})
 
+_MOST_TOKENS = 1 << 30                  # the kernels number them, and steps past the last one, in 32 bits
+
 # The kernels' arguments in the order of LossCall (csrc/policy_losses.cu): addresses and 64-bit words, doubles, ints.
 _CALL = struct.Struct("@36q5d12i")
 
@@ -68,6 +70,8 @@ def _check(logits, labels, loss_mask, ref_logits, ref_logp):
         raise ValueError(f"logits are [sequences, tokens, vocabulary] of at least one sequence and word, got {tuple(logits.shape)}")
     if not logits.is_floating_point():
         raise ValueError(f"logits are floating-point numbers, got {logits.dtype}")
+    if logits.shape[0] * logits.shape[1] >= _MOST_TOKENS:
+        raise ValueError(f"a batch has fewer than {_MOST_TOKENS} tokens, got {tuple(logits.shape)}")
     for name, t in (("labels", labels), ("loss_mask", loss_mask), ("ref_logp", ref_logp)):
         if t is not None and t.shape != logits.shape[:2]:
             raise ValueError(f"{name} is {tuple(t.shape)}, the logits' sequences are {tuple(logits.shape[:2])}")
@@ -188,9 +192,18 @@ def _forward(x, y, labels, mask, width, loss, kl_mean, clipped, logp, ref, old_l
 
 
 def _new_grad(x):
-    """A gradient in the logits' own memory order where that is dense."""
-    g = torch.empty_like(x)
-    return g if g.stride(2) == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    """A gradient whose rows lie as the logits' do, so that both are read and written 16 bytes at a time: logits without their last
+    position or without padding words leave the same gaps in it, as long as it is half full."""
+    n, s, v = x.shape
+    if x.is_contiguous() and not x.data_ptr() & 15:
+        return torch.empty_like(x)
+    (a, size_a), (b, size_b) = sorted(((x.stride(0), n), (x.stride(1), s)))
+    inner = a * (size_a - 1) + v
+    span = b * (size_b - 1) + inner
+    if (size_a > 1 and a < v) or (size_b > 1 and b < inner) or span > 2 * x.numel():
+        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    shift = (x.data_ptr() & 15) // x.element_size()
+    return torch.empty(shift + span, dtype=x.dtype, device=x.device).as_strided(x.shape, x.stride(), shift)
 
 
 def _backward(x, y, labels, mask, g, row, coef, slope, shift, first, g_loss, g_logp, beta, expected, done):

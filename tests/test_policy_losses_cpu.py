@@ -300,3 +300,14 @@ def _router_z_loss(rank, world):
 
 def test_router_z_loss_joins_the_balance_loss():
     run_distributed(_router_z_loss, 1)
+
+
+def test_more_tokens_than_the_kernels_number_are_refused():
+    many = torch.zeros(1, 1, 1).expand(2 ** 15, 2 ** 15, 1)
+    labels, mask = torch.zeros(1, 1, dtype=torch.long).expand(2 ** 15, 2 ** 15), many[..., 0]
+    with pytest.raises(ValueError, match="fewer than"):
+        PL.preference_loss(many, labels, mask, 0.1)
+    with pytest.raises(ValueError, match="fewer than"):
+        PL.policy_loss(many, labels, mask, mask)
+    with pytest.raises(ValueError, match="fewer than"):
+        MO.balanced_router(torch.zeros(1, 2).expand(2 ** 30, 2), 1)

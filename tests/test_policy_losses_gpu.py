@@ -1,8 +1,8 @@
 """Preference loss, clipped policy loss and the router with its losses on a GPU against their formulas in 64 bits.
 
 Where the tolerances come from.  A kernel takes exp(x - max) in 32 bits with a fast exponential: a relative error of 2^-22 and,
-for terms that count (x - max above -16), 2^-20 from the rounded argument; a thread adds at most 32 of them in a row (2^-19), the
-joins a few roundings more.  So a row's log-sum -- and with it a label's log-probability -- is off by at most 2^-18 =: ROW, and a
+for terms that count (x - max above -16), 2^-20 from the rounded argument; a thread adds some hundred of them to a running sum, whose
+roundings (2^-24 each, of either sign) come to about 2^-20, the joins to a few more.  So a row's log-sum -- and with it a label's log-probability -- is off by at most 2^-18 =: ROW, and a
 probability by that relative to itself.  All sums behind the rows are in 64 bits, results are rounded once to 32 bits (2^-24) or to
 the type of the gradient (eps / 2 of it, and half of the smallest number of fp16, 2^-25; 32-bit numbers below 2^-126 are zero)."""
 import pytest
@@ -110,7 +110,8 @@ def test_preference_loss_matches_its_formula(n, s, v, dtype, order):
     (1, 1, 9, torch.float32, "bsv"), (3, 5, 64, torch.bfloat16, "sbv"), (2, 300, 1031, torch.float16, "shifted"),
     (3, 4, 8200, torch.float32, "padded"), (2, 7, 50257, torch.bfloat16, "bsv"), (1, 6, 32000, torch.float16, "strided"),
     (5, 3, 1025, torch.bfloat16, "padded"), (2, 400, 8200, torch.bfloat16, "sbv"), (3, 70, 12001, torch.float32, "shifted"),
-    (2, 90, 128256, torch.bfloat16, "bsv"), (40, 9, 9001, torch.float16, "padded")])
+    (2, 90, 128256, torch.bfloat16, "bsv"), (40, 9, 9001, torch.float16, "padded"), (1100, 1, 8200, torch.bfloat16, "shifted"),
+    (50, 70, 4099, torch.float32, "padded")])
 def test_policy_loss_matches_its_formula(n, s, v, dtype, order, kl, reduce):
     seed = n * 11 + s + v
     x, labels = _logits(n, s, v, dtype, order, seed)
@@ -264,7 +265,7 @@ def test_losses_of_batches_that_keep_nothing():
     assert float(PL.policy_loss(y, short, none[:, :0], none[:, :0]).loss.detach()) == 0.0
 
 
-@pytest.mark.parametrize("op", ["preference", "policy", "foreseen", "full", "router"])
+@pytest.mark.parametrize("op", ["preference", "policy", "foreseen", "not foreseen", "full", "router"])
 def test_losses_repeat_bit_by_bit_on_any_stream_and_in_graphs(op):
     """The same inputs give the same bits: again, on another stream, with a second call in between, and replayed from a CUDA graph
     whose inputs have changed since it was captured."""
@@ -280,8 +281,10 @@ def test_losses_repeat_bit_by_bit_on_any_stream_and_in_graphs(op):
         if op == "preference":
             out = PL.preference_loss(x, labels, mask, 0.1, ref_logits=ref)
             outs = [out.loss, out.logp]
-        elif op in ("policy", "foreseen"):
-            outs = [PL.policy_loss(x, labels, mask, mask, ref_logits=ref, kl_beta=0.1, grad_scale=1.0 if op == "foreseen" else 2.0).loss]
+        elif op == "policy":
+            outs = [PL.policy_loss(x, labels, mask, mask, ref_logits=ref, kl_beta=0.1).loss]
+        elif op in ("foreseen", "not foreseen"):
+            outs = [PL.policy_loss(x, labels, mask, mask, ref_logp=-mask, kl_beta=0.1, grad_scale=1.0 if op == "foreseen" else 2.0).loss]
         elif op == "full":
             outs = [PL.policy_loss(x, labels, mask, mask, ref_logits=ref, kl="full", kl_beta=0.1).loss]
         else:
@@ -343,14 +346,16 @@ def test_loss_gradients_reach_what_asked_for_them():
         out.loss.backward()
 
 
-@pytest.mark.parametrize("kl", ["k3", "full"])
+@pytest.mark.parametrize("kl", ["k3", "k3 of tokens", "full"])
 def test_a_policy_gradient_is_right_whatever_was_foreseen(kl):
     """The gradient for the foreseen gradient of the loss, for another one, and again through a retained graph; each a tensor of its
     own, and accumulated in ``.grad`` as it should be."""
     x, labels = _logits(2, 20, 9000, torch.float32)
-    ref, mask = x + 0.3 * torch.randn_like(x), _mask(2, 20, 2)
+    mask = _mask(2, 20, 2)
+    ref = dict(ref_logp=-mask) if kl == "k3 of tokens" else dict(ref_logits=x + 0.3 * torch.randn_like(x))
     x.requires_grad_()
-    loss = lambda scale: PL.policy_loss(x, labels, mask, mask, ref_logits=ref, kl=kl, kl_beta=0.2, grad_scale=scale).loss  # noqa: E731
+    loss = lambda scale: PL.policy_loss(x, labels, mask, mask, **ref, kl="full" if kl == "full" else "k3",     # noqa: E731
+                                        kl_beta=0.2, grad_scale=scale).loss
     one = loss(1.0)
     first, = torch.autograd.grad(one, x, retain_graph=True)
     kept = first.clone()
@@ -539,3 +544,31 @@ def test_post_training_steps_on_a_gpu(kind):
     r = subprocess.run([sys.executable, os.path.join(ROOT, "tests", "workers", "post_training_worker.py"), kind], env=env,
                        capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "POST_TRAINING_OK" in r.stdout, (r.stdout + r.stderr)[-4000:]
+
+
+@pytest.mark.parametrize("dtype,v", [(torch.bfloat16, 9001), (torch.float32, 2051)])
+def test_gradients_of_sliced_logits_lie_as_the_logits_do(dtype, v):
+    """Logits without their last position, of an odd vocabulary: the gradient's rows begin where the logits' do, what lies between them
+    is not touched, and the whole gradient is the sliced one with zeros behind."""
+    whole, labels = _logits(3, 8, v, dtype)
+    whole.requires_grad_()
+    mask = torch.ones(3, 7, device=DEV)
+    for scale in (1.0, 2.0):                                       # foreseen and not
+        for op in ("policy", "preference"):
+            x = (whole if op == "policy" else whole[:2])[:, :-1]
+            n = x.shape[0]
+            if op == "policy":
+                loss = PL.policy_loss(x, labels[:, :-1], mask, mask, grad_scale=scale).loss
+            else:
+                loss = PL.preference_loss(x, labels[:2, :-1], mask[:2], 0.1).loss
+            part, all_of_it = torch.autograd.grad(loss, [x, whole])
+            assert part.stride() == x.stride() and part.data_ptr() % 16 == x.data_ptr() % 16
+            assert torch.equal(all_of_it[:n, :-1], part) and not all_of_it[:, -1].any() and not all_of_it[n:].any()
+    # logits that lie too far apart for that, or on one another
+    apart = whole.detach()[:, ::4].requires_grad_()
+    loss = PL.policy_loss(apart, labels[:, ::4], mask[:, :2], mask[:, :2]).loss
+    assert torch.autograd.grad(loss, apart)[0].is_contiguous()
+    same = whole.detach()[:1].expand(4, 8, v).requires_grad_()
+    loss = PL.policy_loss(same, labels[:1].expand(4, 8), mask[:1, :1].expand(4, 8), mask[:1, :1].expand(4, 8)).loss
+    grad, = torch.autograd.grad(loss, same)
+    assert grad.is_contiguous() and torch.equal(grad[0], grad[3])
