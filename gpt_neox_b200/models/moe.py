@@ -18,8 +18,8 @@ Data flow for T local tokens, E experts, top-k::
 
 The auxiliary load-balancing loss returned with the output is ``E * sum_e f_e * P_e`` (``f_e`` fraction of
 assignments routed to expert e, ``P_e`` mean router probability), plus the mean of ``logsumexp(router(x))^2`` where
-``moe_z_loss_coeff`` asks for it; ``training.py`` scales it by ``moe_loss_coeff``.  Expert weights are tagged ``expert_parallel`` so the optimizer reduces their gradients
-over the expert-data-parallel group only.
+``moe_z_loss_coeff`` asks for it; ``training.py`` scales it by ``moe_loss_coeff``.  Expert weights are tagged
+``expert_parallel`` so the optimizer reduces their gradients over the expert-data-parallel group only.
 """
 from __future__ import annotations
 

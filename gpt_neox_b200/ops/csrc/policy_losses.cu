@@ -8,10 +8,14 @@
 // with one a (and, for the KL over the whole vocabulary, one b) a row.
 //
 // Three kernels.  `stats_kernel` streams the kept rows once and leaves (max, sum of exponentials) of every chunk of a row;
-// `preference_kernel` / `policy_kernel` join them, one thread a row, in 64 bits from the sums on, and the last block to finish
+// `preference_kernel` / `policy_kernel` join them, eight lanes a row, in 64 bits from the sums on, and the last block to finish
 // forms the loss and what the backward multiplies; `grad_kernel` streams the rows a second time and writes the gradient, zeros
 // where the coefficient is zero, without reading.  The second pass over the logits cannot be saved for a preference loss: a
-// pair's coefficient depends on all of its rows.
+// pair's coefficient depends on all of its rows.  It can be for a policy loss, whose rows need only the sum of the mask from one
+// another: `policy_row_kernel`, further down, has a row in shared memory and writes its gradient with its loss.
+//
+// All of it is bound by memory traffic.  8 x 1024 tokens over 50304 bf16 words, 4506 kept, on a machine whose copies run at 6.55
+// TB/s: statistics 80 us (5.7 TB/s), joining 7, gradient 190 (6.7 TB/s); loss and gradient at once 235 (5.4 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <float.h>
@@ -167,12 +171,14 @@ __device__ __forceinline__ uint4 load_16(const void* p) {
 // exact), which saves an instruction an element.
 __device__ __forceinline__ f32x2 less(uint32_t w, float m, __nv_bfloat16) {
     float a, b;
-    asm("{.reg .b16 x, y;\n mov.b32 {x, y}, %2;\n sub.rn.f32.bf16 %0, x, %3;\n sub.rn.f32.bf16 %1, y, %3;}" : "=f"(a), "=f"(b) : "r"(w), "f"(m));
+    asm("{.reg .b16 x, y;\n mov.b32 {x, y}, %2;\n sub.rn.f32.bf16 %0, x, %3;\n sub.rn.f32.bf16 %1, y, %3;}"
+        : "=f"(a), "=f"(b) : "r"(w), "f"(m));
     return pair(a, b);
 }
 __device__ __forceinline__ f32x2 less(uint32_t w, float m, __half) {
     float a, b;
-    asm("{.reg .b16 x, y;\n mov.b32 {x, y}, %2;\n sub.rn.f32.f16 %0, x, %3;\n sub.rn.f32.f16 %1, y, %3;}" : "=f"(a), "=f"(b) : "r"(w), "f"(m));
+    asm("{.reg .b16 x, y;\n mov.b32 {x, y}, %2;\n sub.rn.f32.f16 %0, x, %3;\n sub.rn.f32.f16 %1, y, %3;}"
+        : "=f"(a), "=f"(b) : "r"(w), "f"(m));
     return pair(a, b);
 }
 template <typename T> __device__ __forceinline__ void exps_of(const uint4& u, float m, f32x2 (&e)[Elem<T>::PER_16 / 2]) {
@@ -414,9 +420,13 @@ template <typename T, bool FULL, int U, int STRIDE> struct Running {
     }
 };
 
-// One block an SM.  It counts the mask, so that every block gets the same number of chunks of kept rows; its warps then walk over
-// them.  A lane copies its own 16-byte vectors to shared memory ahead of the step it works on and reads back what it copied itself, so nothing waits for another lane until a chunk ends in one
-// (max, sum) that the next kernel joins.
+// One block an SM.  It counts the mask, so that every block gets the same number of chunks of kept rows (a sequence's prompt and
+// padding leave whole stretches without one), and its warps take them one by one.  A lane copies its own 16-byte vectors to shared
+// memory ahead of the step it works on and reads back what it copied itself, so nothing waits for another lane until a chunk ends
+// in one (max, sum) that the next kernel joins.  What bounds it is memory traffic, then the issue of some 3.3 instructions an element:
+// pairs of 32-bit numbers, the widening folded into the subtraction (5.5 with single additions, multiplications and conversions).
+// The rows above took 106 us with a block for each chunk of a row and its loads in registers; policy and reference for the KL over
+// the vocabulary 218, now 150 (6.0 TB/s).
 template <typename T, bool FULL>
 __global__ void __launch_bounds__(Shape<FULL>::WARPS * 32, 1) stats_kernel(const StatsArgs a) {
     using W = Walk<T, FULL>;
@@ -482,7 +492,8 @@ __global__ void __launch_bounds__(Shape<FULL>::WARPS * 32, 1) stats_kernel(const
                     const int at = rank + __popc(all & ((1u << lane) - 1));
                     if (w[q] != 0.f && at >= first && at < end) {
                         const int row = r + q * 32 + lane, i = row / a.s, j = row - i * a.s;
-                        sm.list[at - first] = Kept{(k ? a.y : a.x).template at<T>(i, j), FULL ? a.y.template at<T>(i, j) : nullptr, row, k};
+                        const T* other = FULL ? a.y.template at<T>(i, j) : nullptr;
+                        sm.list[at - first] = Kept{(k ? a.y : a.x).template at<T>(i, j), other, row, k};
                     }
                     rank += __popc(all);
                 }
@@ -694,9 +705,10 @@ struct PreferenceArgs {
     float* coef;                   // [n]: d loss / d logp
 };
 
-// Each block joins ROWS rows of one sequence and leaves their sums; the last block adds those up in order, a warp a
-// sequence, and forms, pair by pair,  z = beta ((P_c - P_r) - (R_c - R_r)),
+// Each block joins ROWS rows of one sequence and leaves their sums; the last block adds those up in order and forms, pair by pair,
+// z = beta ((P_c - P_r) - (R_c - R_r)),
 // loss = -(1 - e) log sigma(z) - e log sigma(-z),  d loss / d P_c = -beta ((1 - e) sigma(-z) - e sigma(z)) / pairs = -d/d P_r.
+// Latency bounds it, a dozen trips to L2 one after another: some 7 us behind the statistics, whether of 96 rows or of 8192.
 __global__ void __launch_bounds__(THREADS) preference_kernel(const PreferenceArgs a) {
     const int seq = blockIdx.x / a.pieces, j = (blockIdx.x % a.pieces) * ROWS + threadIdx.x / LANES;
     const int row = seq * a.s + j;
@@ -747,7 +759,8 @@ __global__ void __launch_bounds__(THREADS) preference_kernel(const PreferenceArg
         if (a.smoothing != 0.0) loss += a.smoothing * (soft + fmax(z, 0.0));
         sum[0] += z != z ? z : loss;
         const float large = __frcp_rn(1.f + small), other = small * large;              // sigma(|z|), sigma(-|z|)
-        const float d = z != z ? (float)z : (float)(-a.beta / pairs) * ((1.f - even) * (z >= 0 ? other : large) - even * (z >= 0 ? large : other));
+        const float toward = z >= 0 ? other : large, away = z >= 0 ? large : other;     // sigma(-z), sigma(z)
+        const float d = z != z ? (float)z : (float)(-a.beta / pairs) * ((1.f - even) * toward - even * away);
         a.coef[b] = d;
         a.coef[b + pairs] = -d;
     }
@@ -963,7 +976,8 @@ template <typename T, int G> __device__ __forceinline__ void write_zeros(T* g, i
     if (lane < cut.head) g[lane] = Elem<T>::put(0.f);
     if (lane < cut.tail) g[cut.head + cut.vectors * Elem<T>::PER_16 + lane] = Elem<T>::put(0.f);
 }
-template <typename T, int G> __device__ __forceinline__ void write_apart(const T* x, T* g, int count, int lane, const RowGrad& r, int label) {
+template <typename T, int G>
+__device__ __forceinline__ void write_apart(const T* x, T* g, int count, int lane, const RowGrad& r, int label) {
     for (int c = lane; c < count; c += G) {
         float v = grad_of<T, false>(Elem<T>::get(x[c]), 0.f, r.m, r.scale, 0.f, 0.f);
         if (c == label) v += r.coef;
@@ -971,7 +985,9 @@ template <typename T, int G> __device__ __forceinline__ void write_apart(const T
     }
 }
 
-// One chunk of a row by G threads, at most U 16-byte vectors each.
+// One chunk of a row by G threads, at most U 16-byte vectors each, all asked for before the first is used: eight of one kind of logits
+// or four of both.  Rows without a gradient are written, not read.  Bound by memory traffic; for the KL over the vocabulary (1.73 GB
+// in 289 us) by that and the issue of its arithmetic alike.
 template <typename T, int G, int U, bool FULL> __device__ __forceinline__ void grad_chunk(const GradArgs& a, unsigned item) {
     constexpr int N = Elem<T>::PER_16;
     const int lane = threadIdx.x % G;
@@ -1063,7 +1079,11 @@ __global__ void __launch_bounds__(THREADS) grad_unless_kernel(const GradArgs a, 
 // All that a row of the policy loss needs from other rows is the sum of the mask, and that is known before.  So with the gradient of
 // the loss foreseen (1, or what the caller says) a block takes a row's statistics, its term and its gradient while the row is in
 // shared memory: logits are read once, not twice.  The backward then only looks whether it was asked for that gradient.
-// (Leaving the row to L2 in between, four blocks an SM, two fifths of the rows had gone when they were wanted again.)
+// 8 x 1024 tokens over 50304 words, 4506 kept: 244 us with its two small companions, against 287 for two readings; over 16384 words
+// 98 against 109; 4 x 8192 over 32064 633 against 745.  What it waits for is that all threads of a block have met between sums and
+// gradient.  (Leaving the row to L2 in between, four blocks an SM, 273 us: two fifths of the rows had gone when they were wanted
+// again.  Rows spread over a cluster's blocks, four of them an SM: 262.  Reference logits beside the policy's, one block an SM or a
+// cluster: 0.77 to 0.96 times as fast as two readings.)
 struct AtOnceArgs {
     Rows x;
     void* g;
@@ -1208,7 +1228,8 @@ __global__ void __launch_bounds__(TPB, BLOCKS) policy_row_kernel(const AtOnceArg
     auto request = [&](const Place& p, int v) { copy_16(xs + v, reinterpret_cast<const uint4*>(p.x + p.head) + v); };
     // this block's rows: every gridDim.x-th of the kept ones and of the others
     const int grid = gridDim.x, block = blockIdx.x;
-    const int mine = block < kept ? (kept - 1 - block) / grid + 1 : 0, others = block < rows - kept ? (rows - kept - 1 - block) / grid + 1 : 0;
+    const int mine = block < kept ? (kept - 1 - block) / grid + 1 : 0;
+    const int others = block < rows - kept ? (rows - kept - 1 - block) / grid + 1 : 0;
     int written = 0;
     auto write_others = [&](int until) {
         for (; written < until; ++written) {

@@ -3,9 +3,9 @@ with a KL term.
 
 Both are functions of the log-probabilities that a policy gives the labels of the positions whose ``loss_mask`` is not zero.
 Positions of mask zero -- prompts, padding -- are not read: their logits may hold anything and their gradient is zero.  On a GPU
-the logits are streamed once for the loss and once for its gradient (``csrc/policy_losses.cu``), in their own type and memory
-order; the sums over a sequence and everything behind them are in 64 bits.  ``*_ref`` are the same losses in plain PyTorch: the
-CPU path and the statement the kernels are tested against.
+the logits are streamed once for the loss and once for its gradient -- a policy loss writes both from one reading where it can --
+(``csrc/policy_losses.cu``), in their own type and memory order; the sums over a sequence and everything behind them are in 64 bits.
+``*_ref`` are the same losses in plain PyTorch: the CPU path and the statement the kernels are tested against.
 
 Reference counterparts: the DPO and REINFORCE objectives of ``megatron/training.py:533-939``, which form ``[b, s, V]``
 log-probabilities in fp32.
@@ -207,8 +207,8 @@ def _new_grad(x):
 
 
 def _backward(x, y, labels, mask, g, row, coef, slope, shift, first, g_loss, g_logp, beta, expected, done):
-    """Writes the gradient of the logits into ``g``.  ``y``: the reference, for the KL over the vocabulary; ``row`` to ``shift``: addresses of
-    what the forward kept; ``done``: ``g`` is already right if the gradient of the loss is ``expected``."""
+    """Writes the gradient of the logits into ``g``.  ``y``: the reference, for the KL over the vocabulary; ``row`` to ``shift``:
+    addresses of what the forward kept; ``done``: ``g`` is already right if the gradient of the loss is ``expected``."""
     n, s, v = x.shape
     y_ = x if y is None else y
     call = _CALL.pack(x.data_ptr(), x.stride(0), x.stride(1), y_.data_ptr(), y_.stride(0), y_.stride(1), labels.data_ptr(),
@@ -329,8 +329,8 @@ class _PolicyFn(torch.autograd.Function):
         ctx.full, ctx.kl_beta, ctx.expected, ctx.first, ctx.grad = int(kl == KL_KINDS["full"]), kl_beta, expected, 0, None
         with device_of(x):
             if at_once:
-                loss, kl_mean, clipped, logp, buf, ctx.grad = _policy_at_once(x, labels, mask, adv, old_logp, ref_logp, low, high, kl, kl_beta,
-                                                                              by_sequence, expected)
+                loss, kl_mean, clipped, logp, buf, ctx.grad = _policy_at_once(x, labels, mask, adv, old_logp, ref_logp, low, high, kl,
+                                                                              kl_beta, by_sequence, expected)
                 ctx.streams = 0
             else:
                 loss, kl_mean, clipped, logp, (buf, ctx.first) = _policy_values(x, *rest[:-1])
