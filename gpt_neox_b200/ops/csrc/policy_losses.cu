@@ -1079,7 +1079,7 @@ __global__ void __launch_bounds__(THREADS) grad_unless_kernel(const GradArgs a, 
 // All that a row of the policy loss needs from other rows is the sum of the mask, and that is known before.  So with the gradient of
 // the loss foreseen (1, or what the caller says) a block takes a row's statistics, its term and its gradient while the row is in
 // shared memory: logits are read once, not twice.  The backward then only looks whether it was asked for that gradient.
-// 8 x 1024 tokens over 50304 words, 4506 kept: 244 us with its two small companions, against 287 for two readings; over 16384 words
+// 8 x 1024 tokens over 50304 words, 4506 kept: 241 us with the mask's sums before it, against 287 for two readings; over 16384 words
 // 98 against 109; 4 x 8192 over 32064 633 against 745.  What it waits for is that all threads of a block have met between sums and
 // gradient.  (Leaving the row to L2 in between, four blocks an SM, 273 us: two fifths of the rows had gone when they were wanted
 // again.  Rows spread over a cluster's blocks, four of them an SM: 262.  Reference logits beside the policy's, one block an SM or a
@@ -1099,9 +1099,9 @@ struct AtOnceArgs {
     float expected;
     float2* row;
     float* slope;
-    float4* terms;                 // per row: mask, mask * term, mask * KL, mask * [clipped]
+    double* parts;                 // per block: sums of mask, mask * term * coef, mask * KL, mask * [clipped]
     double* whole;                 // [n]: sums of the mask
-    int* order;                    // the kept rows, then the others; behind them, the number of kept ones
+    int* order;                    // the kept rows, then the others; behind them the number of kept ones and a ticket
     float* coef;                   // [n]
     float* loss;
     float* kl_mean;
@@ -1191,7 +1191,37 @@ __global__ void __launch_bounds__(1024, 1) policy_share_kernel(const AtOnceArgs 
             back += __popc(none);
         }
     }
-    if (tid == 0) a.order[rows] = kept;
+    if (tid == 0) {
+        a.order[rows] = kept;
+        a.order[rows + 1] = 0;
+    }
+}
+
+constexpr int MOST_PARTS = 2048;                                // blocks of a grid
+
+// Means from what the blocks have added up, in a fixed order.  One block; `red`: room for four numbers a warp.
+template <int TPB> __device__ __forceinline__ void take_means(const AtOnceArgs& a, double (*red)[4]) {
+    double v[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll 2
+    for (int b = threadIdx.x; b < (int)gridDim.x; b += TPB)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] += __ldcg(a.parts + 4 * b + k);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = warp_sum(v[k]);
+    if (lane == 0)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) red[warp][k] = v[k];
+    __syncthreads();
+    if (warp != 0) return;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = warp_sum(lane < TPB / 32 ? red[lane][k] : 0.0);
+    if (lane == 0) {
+        const bool any = v[0] != 0.0;
+        *a.loss = any ? (float)v[1] : 0.f;
+        *a.kl_mean = any ? (float)(v[2] / v[0]) : 0.f;
+        *a.share = any ? (float)(v[3] / v[0]) : 0.f;
+    }
 }
 
 // A block walks over its rows.  A thread copies its own vectors of a row to shared memory, takes them for the sums as they arrive, and
@@ -1206,6 +1236,8 @@ __global__ void __launch_bounds__(TPB, BLOCKS) policy_row_kernel(const AtOnceArg
     __shared__ Sums ps[TEAM];
     __shared__ RowGrad grad;
     __shared__ int where;
+    __shared__ double terms[4], sums[4];                        // of a row and of all of them
+    if (threadIdx.x < 4) sums[threadIdx.x] = 0.0;
     const int tid = threadIdx.x, rows = a.n * a.s;
     launch::wait_for_predecessor();
     const int kept = a.order[rows];
@@ -1240,7 +1272,6 @@ __global__ void __launch_bounds__(TPB, BLOCKS) policy_row_kernel(const AtOnceArg
                 a.row[row] = make_float2(0.f, 0.f);
                 a.slope[row] = 0.f;
                 a.logp[row] = 0.f;
-                a.terms[row] = make_float4(0.f, 0.f, 0.f, 0.f);
             }
         }
     };
@@ -1258,14 +1289,14 @@ __global__ void __launch_bounds__(TPB, BLOCKS) policy_row_kernel(const AtOnceArg
         const T* x = now.x;
         const int tail = a.vocab - now.head - now.vectors * N;
         long long label = 0;
-        float own = 0.f, old = 0.f, given = 0.f, adv = 0.f, weight = 0.f, per = 0.f;
+        float own = 0.f, old = 0.f, given = 0.f, adv = 0.f, weight = 0.f, coef_i = 0.f;
         if (tid == 0) {
             label = a.labels[row];
             weight = a.mask[row];
             old = a.old_logp ? a.old_logp[row] : 0.f;
             given = a.ref_logp ? a.ref_logp[row] : 0.f;
             adv = a.advantages[i * a.adv_n + j * a.adv_s];
-            per = a.expected * a.coef[i];
+            coef_i = a.coef[i];
             own = label >= 0 && label < a.vocab ? Elem<T>::get(x[label]) : 0.f;
         }
         int edge = -1;                                          // head and tail of the row: at most one element a thread
@@ -1308,13 +1339,16 @@ __global__ void __launch_bounds__(TPB, BLOCKS) policy_row_kernel(const AtOnceArg
             if (tid == 0) {
                 const double l = label_logp(a.vocab, label, own, m, t);
                 const RowTerm r(a.kl, a.low, a.high, a.kl_beta, l, a.old_logp != nullptr, old, adv, given, 0.0);
-                const float slope = (float)(weight * r.slope), inv = __frcp_rn((float)t), coef = per * slope;
+                const float slope = (float)(weight * r.slope), inv = __frcp_rn((float)t), coef = a.expected * coef_i * slope;
                 grad = RowGrad{m, coef, -coef * inv};
                 where = (int)label;                             // one that does not fit has made everything NaN
                 a.row[row] = make_float2(m, inv);
                 a.slope[row] = slope;
                 a.logp[row] = (float)l;
-                a.terms[row] = make_float4(weight, (float)(weight * r.term), (float)(weight * r.kl), r.clipped ? weight : 0.f);
+                terms[0] = weight;
+                terms[1] = weight * r.term * coef_i;
+                terms[2] = weight * r.kl;
+                terms[3] = r.clipped ? weight : 0.0;
             }
         }
         Place next = {};
@@ -1323,6 +1357,7 @@ __global__ void __launch_bounds__(TPB, BLOCKS) policy_row_kernel(const AtOnceArg
         __syncthreads();
         const RowGrad r = grad;
         const int hot = where;
+        if (tid < 4) sums[tid] += terms[tid];
         T* g = reinterpret_cast<T*>(a.g) + (long long)i * a.gn + (long long)j * a.gs;
         if ((((uintptr_t)x ^ (uintptr_t)g) & 15) != 0) {
             write_apart<T, TPB>(x, g, a.vocab, tid, r, hot);
@@ -1365,37 +1400,8 @@ __global__ void __launch_bounds__(TPB, BLOCKS) policy_row_kernel(const AtOnceArg
     }
     copies_here<0>();
     write_others(others);
-}
-
-// Means of the rows' terms, in a fixed order.  One block.
-__global__ void __launch_bounds__(1024) policy_mean_kernel(const AtOnceArgs a, int rows) {
-    __shared__ double red[32][4];
-    launch::wait_for_predecessor();
-    double v[4] = {0.0, 0.0, 0.0, 0.0};                         // mask, loss, KL, clipped
-#pragma unroll 4
-    for (int row = threadIdx.x; row < rows; row += 1024) {
-        const float4 t = a.terms[row];
-        v[0] += t.x;
-        v[1] += (double)t.y * a.coef[row / a.s];
-        v[2] += t.z;
-        v[3] += t.w;
-    }
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = warp_sum(v[k]);
-    if (lane == 0)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) red[warp][k] = v[k];
-    __syncthreads();
-    if (warp != 0) return;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = warp_sum(red[lane][k]);
-    if (lane == 0) {
-        const bool any = v[0] != 0.0;
-        *a.loss = any ? (float)v[1] : 0.f;
-        *a.kl_mean = any ? (float)(v[2] / v[0]) : 0.f;
-        *a.share = any ? (float)(v[3] / v[0]) : 0.f;
-    }
+    if (tid < 4) a.parts[4 * block + tid] = sums[tid];
+    if (last_block(a.order + rows + 1)) take_means<TPB>(a, reinterpret_cast<double(*)[4]>(raw_smem));
 }
 
 // How the gradient cuts a row: G threads with U loads each, for narrow vocabularies fewer of them, so that all have something to do.
@@ -1449,7 +1455,7 @@ struct AtOncePlan {
     size_t bytes;
     AtOncePlan(int vocab, int dtype) {
         places = vocab / (dtype == 1 ? 4 : 8) + 1;
-        bytes = (size_t)places * 16;
+        bytes = places < 64 ? 1024 : (size_t)places * 16;       // and the last block's sums
         blocks = bytes <= most(8) ? 8 : bytes <= most(4) ? 4 : bytes <= most(3) ? 3 : bytes <= most(2) ? 2 : bytes <= most(1) ? 1 : 0;
     }
     // of 228 KB an SM, with 1 KB and what the kernel has besides for every block
@@ -1504,7 +1510,7 @@ struct LossCall {
     const float* g_logp;
     long long v0, whole;           // first word of this share of the vocabulary; words of all shares
     void* stream;
-    float* terms;                  // scratch of the policy loss with its gradient: [n * s, 4], n doubles, n * s + 1 ints
+    float* terms;                  // scratch of the policy loss with its gradient: 4 doubles a block, n doubles, n * s + 2 ints
     double beta, smoothing, low, high;       // beta: of the preference, or the KL's weight
     double expected;               // gradient of the loss that the forward writes its gradient for
     int n, s, vocab, dtype;
@@ -1569,14 +1575,14 @@ int neox_policy_at_once(const void* packed) {
     const AtOncePlan p(c.vocab, c.dtype);
     if (c.n < 1 || c.s < 1 || c.vocab < 1 || c.y || c.kl == KL_FULL || p.blocks == 0) return NEOX_ERR_SHAPE;
     if (rows >= MOST_TOKENS) return NEOX_ERR_TOO_LARGE;
-    double* whole = (double*)(c.terms + 4 * rows);
+    double* whole = (double*)c.terms + 4 * (rows < MOST_PARTS ? rows : MOST_PARTS);
     const AtOnceArgs a = {{c.x, c.xn, c.xs}, c.g, c.gn, c.gs, c.labels, c.mask, c.advantages, c.adv_n, c.adv_s, c.old_logp,
                           c.ref_logp, c.n, c.s, c.vocab, c.kl, c.by_sequence, c.low, c.high, c.beta, (float)c.expected, c.row, c.slope,
-                          (float4*)c.terms, whole, (int*)(whole + c.n), c.coef, c.loss, c.kl_mean, c.clipped, c.logp};
+                          (double*)c.terms, whole, (int*)(whole + c.n), c.coef, c.loss, c.kl_mean, c.clipped, c.logp};
     cudaStream_t st = (cudaStream_t)c.stream;
     policy_share_kernel<<<1, 1024, 0, st>>>(a);
     if (launched() != 0) return NEOX_ERR_LAUNCH;
-    const long long most = (long long)p.blocks * neox_sm_count();
+    const long long fit = (long long)p.blocks * neox_sm_count(), most = fit < MOST_PARTS ? fit : MOST_PARTS;
     const dim3 grid((unsigned)(rows < most ? rows : most));
     int rc = 0;
     if (p.blocks == 8) FOR_TYPE(c.dtype, (rc = rows_at_once<T, 128, 8>(a, p, grid, st)));
@@ -1584,8 +1590,7 @@ int neox_policy_at_once(const void* packed) {
     else if (p.blocks == 3) FOR_TYPE(c.dtype, (rc = rows_at_once<T, 320, 3>(a, p, grid, st)));
     else if (p.blocks == 2) FOR_TYPE(c.dtype, (rc = rows_at_once<T, 512, 2>(a, p, grid, st)));
     else FOR_TYPE(c.dtype, (rc = rows_at_once<T, 768, 1>(a, p, grid, st)));
-    if (rc != 0) return rc;
-    return launch::overlapped(policy_mean_kernel, dim3(1), dim3(1024), 1, st, a, (int)rows);
+    return rc;
 }
 
 int neox_loss_backward(const void* packed) {

@@ -279,10 +279,10 @@ def _policy_values(x, labels, mask, adv, old_logp, ref_logits, ref_logp, low, hi
 
 @functools.lru_cache(maxsize=256)
 def _at_once_layout(n, s):
-    """As :func:`_layout`, for :func:`_policy_at_once`: ``row``, ``coef``, ``slope`` as there; ``terms`` [rows, 4], ``[n]`` fp64 and
-    ``[rows + 1]`` int32 of scratch."""
+    """As :func:`_layout`, for :func:`_policy_at_once`: ``row``, ``coef``, ``slope`` as there; of scratch, 4 fp64 for each of
+    at most 2048 blocks, ``[n]`` fp64 and ``[rows + 2]`` int32."""
     rows = n * s
-    sizes = (4 * rows, 2 * n, rows + 1, 2 * rows, n, rows)
+    sizes = (8 * min(rows, 2048), 2 * n, rows + 2, 2 * rows, n, rows)
     at, offsets = 0, []
     for size in sizes:
         offsets.append(4 * at)

@@ -111,7 +111,8 @@ def test_preference_loss_matches_its_formula(n, s, v, dtype, order):
     (3, 4, 8200, torch.float32, "padded"), (2, 7, 50257, torch.bfloat16, "bsv"), (1, 6, 32000, torch.float16, "strided"),
     (5, 3, 1025, torch.bfloat16, "padded"), (2, 400, 8200, torch.bfloat16, "sbv"), (3, 70, 12001, torch.float32, "shifted"),
     (2, 90, 128256, torch.bfloat16, "bsv"), (40, 9, 9001, torch.float16, "padded"), (1100, 1, 8200, torch.bfloat16, "shifted"),
-    (50, 70, 4099, torch.float32, "padded")])
+    (50, 70, 4099, torch.float32, "padded"), (2, 21, 100003, torch.bfloat16, "bsv"), (1, 3, 115711, torch.float16, "sbv"),
+    (1, 3, 115712, torch.float16, "sbv"), (160, 2, 57856, torch.bfloat16, "shifted")])
 def test_policy_loss_matches_its_formula(n, s, v, dtype, order, kl, reduce):
     seed = n * 11 + s + v
     x, labels = _logits(n, s, v, dtype, order, seed)
