@@ -1585,11 +1585,13 @@ int neox_policy_at_once(const void* packed) {
     const long long fit = (long long)p.blocks * neox_sm_count(), most = fit < MOST_PARTS ? fit : MOST_PARTS;
     const dim3 grid((unsigned)(rows < most ? rows : most));
     int rc = 0;
+    // threads: 32 short of what registers would hold or more, where the compiler then keeps more loads under way (4 x 8192 tokens over
+    // 32064 words: 665 us with 320, 600 with 256; 8 x 1024 over 50304: 248 with 512, 241 with 384; over 100000: 501 with 768, 476 with 640)
     if (p.blocks == 8) FOR_TYPE(c.dtype, (rc = rows_at_once<T, 128, 8>(a, p, grid, st)));
     else if (p.blocks == 4) FOR_TYPE(c.dtype, (rc = rows_at_once<T, 256, 4>(a, p, grid, st)));
-    else if (p.blocks == 3) FOR_TYPE(c.dtype, (rc = rows_at_once<T, 320, 3>(a, p, grid, st)));
-    else if (p.blocks == 2) FOR_TYPE(c.dtype, (rc = rows_at_once<T, 512, 2>(a, p, grid, st)));
-    else FOR_TYPE(c.dtype, (rc = rows_at_once<T, 768, 1>(a, p, grid, st)));
+    else if (p.blocks == 3) FOR_TYPE(c.dtype, (rc = rows_at_once<T, 256, 3>(a, p, grid, st)));
+    else if (p.blocks == 2) FOR_TYPE(c.dtype, (rc = rows_at_once<T, 384, 2>(a, p, grid, st)));
+    else FOR_TYPE(c.dtype, (rc = rows_at_once<T, 640, 1>(a, p, grid, st)));
     return rc;
 }
 
