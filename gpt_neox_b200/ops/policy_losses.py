@@ -313,6 +313,12 @@ def _policy_at_once(x, labels, mask, adv, old_logp, ref_logp, low, high, kl, kl_
     return loss, kl_mean, clipped, logp, buf, g
 
 
+# Bytes of logits from which on a reference's log-probabilities are taken first, in launches of their own, so that the policy's logits
+# are read once: forward and backward of 8 x 1024 tokens over 50304 16-bit words (824 MB) 336 us so, 361 with both read together and
+# the policy's twice; 4 x 4096 over 32064 (1 GB) 433 and 473; 4 x 512 over 50304 (206 MB) 116 and 118, but 30 us more for the host.
+_REF_FIRST = 1 << 29
+
+
 @functools.lru_cache(maxsize=256)
 def _one_reading_pays(vocab, dtype):
     """A row that keeps a block busy and fits in shared memory; others are read twice."""
@@ -325,10 +331,13 @@ class _PolicyFn(torch.autograd.Function):
         labels, mask, adv, old_logp, ref_logits, ref_logp, low, high, kl, kl_beta, by_sequence, expected = rest
         # 16-bit floating-point numbers of five exponent bits need the loss scale before they are rounded
         at_once = x.shape[1] > 0 and _tensor_parallel()[0] == 1 and (x.dtype != torch.float16 or expected != 1.0) \
-            and ref_logits is None and _one_reading_pays(x.shape[2], x.dtype)
+            and (ref_logits is None or (kl != KL_KINDS["full"] and x.numel() * x.element_size() >= _REF_FIRST)) \
+            and _one_reading_pays(x.shape[2], x.dtype)
         ctx.full, ctx.kl_beta, ctx.expected, ctx.first, ctx.grad = int(kl == KL_KINDS["full"]), kl_beta, expected, 0, None
         with device_of(x):
             if at_once:
+                if ref_logits is not None:
+                    ref_logp = _policy_values(ref_logits, labels, mask, adv, None, None, None, low, high, 0, 0.0, False)[3]
                 loss, kl_mean, clipped, logp, buf, ctx.grad = _policy_at_once(x, labels, mask, adv, old_logp, ref_logp, low, high, kl,
                                                                               kl_beta, by_sequence, expected)
                 ctx.streams = 0
@@ -499,8 +508,9 @@ def policy_loss(logits, labels, loss_mask, advantages, old_logp: Optional[torch.
     ``grad_scale`` is the gradient of the loss that the backward is expected to start from: 1 for ``loss.backward()``, a loss scale or
     ``1 / accumulation steps`` for a scaled loss.  Where the logits ask for a gradient, it is computed for that value together with
     the loss, while a row is at hand, and the backward only has to look; any other gradient of the loss is right as well, and
-    costs the second reading of the logits that was to be saved.  (With reference logits, with fp16 logits and ``grad_scale`` 1, and
-    for vocabularies that are short, split over ranks or too long for shared memory, logits are always read twice.)
+    costs the second reading of the logits that was to be saved.  (With the KL over the whole vocabulary, with fp16 logits and
+    ``grad_scale`` 1, with reference logits in a small batch, and for vocabularies that are short, split over ranks or too long for
+    shared memory, logits are always read twice.)
     """
     _check(logits, labels, loss_mask, ref_logits, ref_logp)
     n, s = logits.shape[:2]

@@ -182,6 +182,16 @@ def test_policy_loss_matches_its_formula(n, s, v, dtype, order, kl, reduce):
     assert not grad[~keep].any()
 
 
+@pytest.mark.parametrize("kl", ["kl", "abs", "mse", "k3"])
+@pytest.mark.parametrize("n,s,v,dtype,order,reduce", [
+    (2, 6, 50257, torch.bfloat16, "bsv", "token"), (5, 5, 9001, torch.float32, "padded", "sequence"),
+    (3, 6, 32001, torch.float16, "sbv", "token")])
+def test_policy_loss_whose_reference_is_read_first(n, s, v, dtype, order, reduce, kl, monkeypatch):
+    """As large batches have it: the reference's log-probabilities before the policy's one reading."""
+    monkeypatch.setattr(PL, "_REF_FIRST", 0)
+    test_policy_loss_matches_its_formula(n, s, v, dtype, order, kl, reduce)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("v", [40, 3000, 20001])
 def test_loss_rows_of_extreme_logits(v, dtype):
