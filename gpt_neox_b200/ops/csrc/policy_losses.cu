@@ -15,7 +15,7 @@
 // another: `policy_row_kernel`, further down, has a row in shared memory and writes its gradient with its loss.
 //
 // All of it is bound by memory traffic.  8 x 1024 tokens over 50304 bf16 words, 4506 kept, on a machine whose copies run at 6.55
-// TB/s: statistics 80 us (5.7 TB/s), joining 7, gradient 190 (6.7 TB/s); loss and gradient at once 235 (5.4 TB/s).
+// TB/s: statistics 80 us (5.7 TB/s), joining 7, gradient 190 (6.7 TB/s); loss and gradient at once 226 (5.7 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <float.h>
@@ -1079,8 +1079,8 @@ __global__ void __launch_bounds__(THREADS) grad_unless_kernel(const GradArgs a, 
 // All that a row of the policy loss needs from other rows is the sum of the mask, and that is known before.  So with the gradient of
 // the loss foreseen (1, or what the caller says) a block takes a row's statistics, its term and its gradient while the row is in
 // shared memory: logits are read once, not twice.  The backward then only looks whether it was asked for that gradient.
-// 8 x 1024 tokens over 50304 words, 4506 kept: 241 us with the mask's sums before it, against 287 for two readings; over 16384 words
-// 98 against 109; 4 x 8192 over 32064 633 against 745.  What it waits for is that all threads of a block have met between sums and
+// 8 x 1024 tokens over 50304 words, 4506 kept: 232 us with the mask's sums before it, against 287 for two readings; over 16384 words
+// 90 against 109; 4 x 8192 over 32064 610 against 742.  What it waits for is that all threads of a block have met between sums and
 // gradient.  (Leaving the row to L2 in between, four blocks an SM, 273 us: two fifths of the rows had gone when they were wanted
 // again.  Rows spread over a cluster's blocks, four of them an SM: 262.  Reference logits beside the policy's, one block an SM or a
 // cluster: 0.77 to 0.96 times as fast as two readings.)
