@@ -330,7 +330,7 @@ class _PolicyFn(torch.autograd.Function):
     def forward(ctx, x, rest):
         labels, mask, adv, old_logp, ref_logits, ref_logp, low, high, kl, kl_beta, by_sequence, expected = rest
         # 16-bit floating-point numbers of five exponent bits need the loss scale before they are rounded
-        at_once = x.shape[1] > 0 and _tensor_parallel()[0] == 1 and (x.dtype != torch.float16 or expected != 1.0) \
+        at_once = ctx.needs_input_grad[0] and x.shape[1] > 0 and _tensor_parallel()[0] == 1 and (x.dtype != torch.float16 or expected != 1.0) \
             and (ref_logits is None or (kl != KL_KINDS["full"] and x.numel() * x.element_size() >= _REF_FIRST)) \
             and _one_reading_pays(x.shape[2], x.dtype)
         ctx.full, ctx.kl_beta, ctx.expected, ctx.first, ctx.grad = int(kl == KL_KINDS["full"]), kl_beta, expected, 0, None
@@ -507,10 +507,10 @@ def policy_loss(logits, labels, loss_mask, advantages, old_logp: Optional[torch.
 
     ``grad_scale`` is the gradient of the loss that the backward is expected to start from: 1 for ``loss.backward()``, a loss scale or
     ``1 / accumulation steps`` for a scaled loss.  Where the logits ask for a gradient, it is computed for that value together with
-    the loss, while a row is at hand, and the backward only has to look; any other gradient of the loss is right as well, and
-    costs the second reading of the logits that was to be saved.  (With the KL over the whole vocabulary, with fp16 logits and
-    ``grad_scale`` 1, with reference logits in a small batch, and for vocabularies that are short, split over ranks or too long for
-    shared memory, logits are always read twice.)
+    the loss, while a row is at hand (its memory is taken then), and the backward only has to look; any other gradient of the loss
+    is right as well, and costs the second reading of the logits that was to be saved.  (With the KL over the whole vocabulary, with
+    fp16 logits and ``grad_scale`` 1, with reference logits in a small batch, and for vocabularies that are short, split over ranks
+    or too long for shared memory, logits are always read twice.)
     """
     _check(logits, labels, loss_mask, ref_logits, ref_logp)
     n, s = logits.shape[:2]

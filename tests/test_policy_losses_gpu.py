@@ -276,6 +276,29 @@ def test_losses_of_batches_that_keep_nothing():
     assert float(PL.policy_loss(y, short, none[:, :0], none[:, :0]).loss.detach()) == 0.0
 
 
+def test_policy_gradients_of_long_rows_that_are_not_kept_or_not_asked_for():
+    x, labels = _logits(3, 50, 20000, torch.bfloat16)
+    adv, mask = torch.ones(3, 50, device=DEV), torch.zeros(3, 50, device=DEV)
+    x.requires_grad_()
+    for kept in (0, 1, 2):                                         # rows that leave something: none, one, two of one sequence
+        if kept:
+            mask[1, 7 * kept] = 1.0
+        for reduce in ("token", "sequence"):
+            for scale in (1.0, 3.0, 0.0, float("nan")):
+                out = PL.policy_loss(x, labels, mask, adv, reduce=reduce, grad_scale=scale)
+                grad, = torch.autograd.grad(out.loss, x)
+                assert not grad[mask == 0].any() and bool(grad.isfinite().all()) and bool(grad[mask != 0].any()) == bool(kept)
+                want = PL.policy_loss_ref(x.detach().double().requires_grad_(), labels, mask.double(), adv.double(), reduce=reduce).loss
+                _near(out.loss.detach(), want.detach(), 2.0 ** -22, "loss")
+    # nobody asks for a gradient: none is written
+    y = x.detach()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out = PL.policy_loss(y, labels, mask, adv)
+    assert not out.loss.requires_grad and torch.cuda.max_memory_allocated() - before < y.numel()
+
+
 @pytest.mark.parametrize("op", ["preference", "policy", "foreseen", "not foreseen", "full", "router"])
 def test_losses_repeat_bit_by_bit_on_any_stream_and_in_graphs(op):
     """The same inputs give the same bits: again, on another stream, with a second call in between, and replayed from a CUDA graph
