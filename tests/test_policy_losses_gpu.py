@@ -606,3 +606,52 @@ def test_gradients_of_sliced_logits_lie_as_the_logits_do(dtype, v):
     loss = PL.policy_loss(same, labels[:1].expand(4, 8), mask[:1, :1].expand(4, 8), mask[:1, :1].expand(4, 8)).loss
     grad, = torch.autograd.grad(loss, same)
     assert grad.is_contiguous() and torch.equal(grad[0], grad[3])
+
+
+@pytest.mark.parametrize("op", ["preference", "policy", "not foreseen", "full"])
+def test_losses_of_more_logits_than_32_bits_number(op):
+    """More than 2^31 logits of which the last positions of two sequences are kept: loss and gradient are those of these positions
+    alone, and zero elsewhere.  Both sides round a gradient once to bf16, from coefficients and probabilities that are ROW apart."""
+    n, s, v, last = 44, 1000, 50304, 3
+    pair = [n // 2 - 1, n - 1]
+    x = torch.empty(n, s, v, device=DEV, dtype=torch.bfloat16).normal_()
+    y = torch.empty_like(x).normal_() if op == "full" else None
+    labels = torch.randint(0, v, (n, s), device=DEV)
+    mask = torch.zeros(n, s, device=DEV)
+    mask[pair, -last:] = 1.0
+
+    def run(x, labels, mask, y):
+        x = x.detach().requires_grad_()
+        if op == "preference":
+            out = PL.preference_loss(x, labels, mask, 0.5)
+            grad, = torch.autograd.grad(out.loss, x, torch.tensor(float(x.shape[0] // 2), device=DEV))
+            return out.logp[-1].detach(), grad
+        out = PL.policy_loss(x, labels, mask, mask, ref_logits=y, kl="full" if op == "full" else "k3", kl_beta=0.3,
+                             grad_scale=2.0 if op == "not foreseen" else 1.0)
+        return out.loss.detach(), torch.autograd.grad(out.loss, x)[0]
+
+    got, grad = run(x, labels, mask, y)
+    few = [t[pair][:, -last:].clone() if t is not None else None for t in (x, labels, mask, y)]
+    want, want_grad = run(*few)
+    _near(got, want.double(), 8 * ROW * (1 + want.double().abs()), "value")
+    eps = torch.finfo(torch.bfloat16).eps
+    size = want_grad.double().abs()
+    # a probability is below 2^-8 here, a coefficient at most twice the largest gradient, which stands at a label
+    _near(grad[pair][:, -last:], want_grad.double(), eps * size + 8 * ROW * size.max() * (2.0 ** -8 + (size > size.max() / 8)), "gradient")
+    grad[pair, -last:] = 0
+    assert not grad.any()
+
+
+def test_router_of_more_logits_than_32_bits_number():
+    tokens, experts, k, last = 4_300_000, 512, 4, 999
+    x = torch.empty(tokens, experts, device=DEV, dtype=torch.bfloat16).normal_().requires_grad_()
+    out = MO.balanced_router(x, k)
+    few = x.detach()[-last:].clone().requires_grad_()
+    want = MO.balanced_router(few, k)
+    assert torch.equal(out.experts[-last:], want.experts) and torch.equal(out.weights[-last:], want.weights)
+    assert int(out.counts.sum()) == tokens * k
+    g = torch.zeros(tokens, k, device=DEV)
+    g[-last:] = torch.randn(last, k, device=DEV)
+    grad, = torch.autograd.grad(out.weights, x, g)
+    want_grad, = torch.autograd.grad(want.weights, few, g[-last:].contiguous())
+    assert torch.equal(grad[-last:], want_grad) and not grad[:-last].any()
