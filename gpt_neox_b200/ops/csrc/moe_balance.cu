@@ -149,6 +149,9 @@ struct ForwardArgs {
 // experts: 6.4 against 8.1 us).
 template <typename T, int C> constexpr int LARGE = sizeof(T) == 2 && C == 1 ? 1024 : 512;
 
+// A lane sorts its eight candidates once (19 exchanges), and a choice is the largest head among the lanes: log LANES shuffles and a
+// shift of the winner's list.  That, not the bytes, bounds many tokens: 32768 of 128 experts, eight choices, 12.8 us for 12 MB
+// (1.8 us); with every choice a search over all candidates the two forward kernels took 33.4 us, now 16.9.
 template <typename T, int LANES, int C, int THREADS>
 __global__ void __launch_bounds__(THREADS) router_kernel(const ForwardArgs a) {
     constexpr int GROUPS = THREADS / LANES, WARPS = THREADS / 32, SLOTS = LANES * C * 8;
@@ -296,7 +299,8 @@ struct LossArgs {
     int blocks, E, k;
 };
 
-// Joins what the router's blocks left: 32 experts a block, 32 threads an expert, and the last block forms the losses.
+// Joins what the router's blocks left: 32 experts a block, 32 threads an expert, and the last block forms the losses.  Latency:
+// 4 to 6 us behind the router, for 8 experts as for 128.
 __global__ void __launch_bounds__(1024) router_loss_kernel(const LossArgs a) {
     __shared__ double p[32][33];
     __shared__ int n_all[32][33], n_kept[32][33];
@@ -385,6 +389,8 @@ struct BackwardArgs {
     int tokens, E, k, aligned;
 };
 
+// One pass: a token's logits give p again from its maximum and sum.  The loads' latency bounds it: 32768 tokens of 128 experts 7.6 us
+// for 21 MB (3.3 us at the rate of a copy), 16384 of 512 experts 14.2 us for 36 MB (5.5 us).
 template <typename T, int LANES, int C>
 __global__ void __launch_bounds__(THREADS) router_grad_kernel(const BackwardArgs a) {
     constexpr int GROUPS = THREADS / LANES, MINE = (MAX_K + LANES - 1) / LANES;

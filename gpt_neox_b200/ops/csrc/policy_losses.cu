@@ -1226,8 +1226,8 @@ template <int TPB> __device__ __forceinline__ void take_means(const AtOnceArgs& 
 
 // A block walks over its rows.  A thread copies its own vectors of a row to shared memory, takes them for the sums as they arrive, and
 // when all threads have met for the row's numbers, once more for the gradient; each place that it has read the second time it fills
-// with the next row's vector.  Two blocks an SM where two rows fit (one is at its sums, the other at its gradient), else one.  The
-// rows that leave nothing are written in between: while a block waits for a row, memory has time for them.
+// with the next row's vector.  As many blocks an SM as rows fit, up to eight: while one is at its sums, another is at its gradient.
+// The rows that leave nothing are written in between: while a block waits for a row, memory has time for them.
 template <typename T, int TPB, int BLOCKS>
 __global__ void __launch_bounds__(TPB, BLOCKS) policy_row_kernel(const AtOnceArgs a, int places) {
     constexpr int N = Elem<T>::PER_16, U = 4, TEAM = TPB / 32, PARTS = 4;
