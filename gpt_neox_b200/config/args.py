@@ -557,6 +557,13 @@ class NeoXArgs:
             assert not self.is_pipe_parallel, "MoE not supported with pipeline parallelism"
             assert self.zero_optimization["stage"] != 3, "MoE not compatible with zero3"
             assert self.sequence_parallel is False, "MoE not compatible with Sequence Parallel"
+            if self.moe_z_loss_coeff:
+                # it travels in the layers' auxiliary loss: refused where that never reaches the router
+                assert self.moe_loss_coeff, "moe_z_loss_coeff needs a moe_loss_coeff that is not zero: both losses travel as one"
+                assert self.train_impl == "normal", \
+                    f"moe_z_loss_coeff needs train_impl normal: {self.train_impl} leaves the layers' auxiliary losses out"
+                assert not self.checkpoint_activations, \
+                    "moe_z_loss_coeff is not compatible with checkpoint_activations, which records no gradient of the auxiliary losses"
 
         # attention pattern
         if self.num_layers is not None:

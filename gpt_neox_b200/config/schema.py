@@ -318,7 +318,7 @@ moe_type : str = 'megablocks'
 moe_glu : bool = False
 moe_lbl_in_fp32 : bool = False
 moe_jitter_eps : float = None
-moe_z_loss_coeff : float = 0.0
+moe_z_loss_coeff : float = 0.0                     # weight of the mean of logsumexp(router logits)^2, per layer; needs train_impl normal, moe_loss_coeff and no checkpoint_activations
 enable_expert_tensor_parallelism : bool = False
 
 [engine]

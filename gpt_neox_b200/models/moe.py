@@ -125,6 +125,8 @@ class Router(nn.Module):
         if neox_args.moe_z_loss_coeff and not neox_args.moe_loss_coeff:
             raise ValueError("moe_z_loss_coeff needs a moe_loss_coeff that is not zero: both losses travel as one")
         self.z_share = neox_args.moe_z_loss_coeff / neox_args.moe_loss_coeff if neox_args.moe_z_loss_coeff else 0.0
+        # ``moe_type: deepspeed`` adds the balance loss to the reported loss as a constant, and the z loss with its gradient
+        self.balance_trains = neox_args.moe_type != "deepspeed"
 
     def forward(self, x):
         if self.training and self.jitter_eps:
@@ -143,7 +145,9 @@ class Router(nn.Module):
 
     def _loss(self, balance, z):
         """The layer's auxiliary loss: what ``moe_loss_coeff`` multiplies later, so the z loss enters in its units."""
-        return balance + self.z_share * z() if self.z_share else balance
+        if not self.z_share:
+            return balance
+        return (balance if self.balance_trains else balance.detach()) + self.z_share * z()
 
 
 class ParallelMoE(nn.Module):

@@ -226,7 +226,10 @@ def forward_step(data_iterator, model, neox_args, timers, return_logits=False, i
                 labels = labels[:, : neox_args.curriculum_seqlen].contiguous()
             loss = cross_entropy(outputs, (labels, loss_mask), _fp16=neox_args.fp16_lm_cross_entropy)
             if neox_args.moe_num_experts > 1:
-                if neox_args.moe_type == "deepspeed":
+                if neox_args.moe_type == "deepspeed" and neox_args.moe_z_loss_coeff:
+                    # the layers hand on their balance losses as constants and their z losses with a gradient
+                    loss = loss + neox_args.moe_loss_coeff * torch.stack([m.float() for m in moe_losses]).sum()
+                elif neox_args.moe_type == "deepspeed":
                     # reference semantics: the summed per-layer losses enter as a detached constant
                     loss = loss + neox_args.moe_loss_coeff * sum(float(m) for m in moe_losses)
                 else:

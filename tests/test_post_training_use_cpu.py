@@ -1,0 +1,69 @@
+"""How training reaches the post-training losses and the router's losses, without a GPU: what a configuration's keys do or that they are
+refused, and what online data has to bring."""
+import pickle
+import socket
+import threading
+
+import pytest
+import torch
+
+from common import make_args, run_distributed
+
+MOE = {"moe_num_experts": 4, "moe_top_k": 2, "expert_interval": 1, "gpt_j_residual": False, "moe_loss_coeff": 0.1}
+
+
+def _z_loss_step(rank, world, cfg, coeff, path):
+    """``forward_step`` and its gradient: the loss, the gradient of the last layer's router weight, and what its router saw."""
+    from gpt_neox_b200.initialize import initialize_megatron
+    from gpt_neox_b200.models.moe import Router
+    from gpt_neox_b200.training import forward_step, setup_model_and_optimizer
+    from gpt_neox_b200.utils import Timers
+    args = make_args(**{**cfg, "moe_z_loss_coeff": coeff, "global_num_gpus": world})
+    args.configure_distributed_args()
+    initialize_megatron(args)
+    model, _, _, _ = setup_model_and_optimizer(args)
+    routers = [m for m in model.module.modules() if isinstance(m, Router)]
+    seen = []
+    for r in routers:
+        r.layer.register_forward_hook(lambda m, i, o: seen.append(i[0].detach().double()))
+    text = torch.randint(1, 60, (2, args.seq_length + 1), generator=torch.Generator().manual_seed(1))
+    loss, _ = forward_step(iter([{"text": text}]), model, args, Timers(), is_train=True)
+    loss.backward()
+    weight = routers[-1].layer.weight
+    grad = weight.main_grad if getattr(weight, "main_grad", None) is not None and weight.grad is None else weight.grad
+    torch.save({"loss": loss.detach().double(), "grad": grad.detach().double().clone(), "seen": seen,
+                "weights": [r.layer.weight.detach().double() for r in routers]}, path)
+
+
+@pytest.mark.parametrize("kind", ["megablocks", "deepspeed", "deepspeed dense"])
+def test_z_loss_of_the_configuration_trains_the_router(kind, tmp_path):
+    """The coefficient times the layers' mean of logsumexp^2 -- their mean or, for ``moe_type: deepspeed``, their sum, as the balance
+    loss is taken -- enters the loss, and its gradient the router's weight."""
+    cfg = {**MOE, "moe_type": kind.split()[0], "moe_use_residual": not kind.endswith("dense")}
+    coeff, got = 0.05, []
+    for i, c in enumerate((0.0, coeff)):
+        run_distributed(_z_loss_step, 1, cfg, c, str(tmp_path / f"{i}.pt"))
+        got.append(torch.load(tmp_path / f"{i}.pt"))
+    off, on = got
+    assert all(torch.equal(a, b) for a, b in zip(off["weights"], on["weights"]))
+    z = torch.stack([(x.reshape(-1, w.shape[1]) @ w.t()).logsumexp(-1).square().mean() for x, w in zip(on["seen"], on["weights"])])
+    share = z.sum() if kind.startswith("deepspeed") else z.mean()
+    # losses of a few units and their differences in 32 bits: some roundings of 2^-24 each
+    torch.testing.assert_close(on["loss"] - off["loss"], coeff * share, rtol=0, atol=2.0 ** -19)
+    w = on["weights"][-1].requires_grad_()
+    last = (on["seen"][-1].reshape(-1, w.shape[1]) @ w.t()).logsumexp(-1).square().mean() / (1 if kind.startswith("deepspeed") else len(z))
+    want, = torch.autograd.grad(coeff * last, w)
+    # a gradient in 32 bits is off by some hundred roundings of its largest terms, on either side of the difference
+    torch.testing.assert_close(on["grad"] - off["grad"], want, rtol=0, atol=2.0 ** -15 * float(on["grad"].abs().max()))
+    assert float(want.abs().max()) > 2.0 ** -12 * float(on["grad"].abs().max())
+
+
+@pytest.mark.parametrize("change,words", [
+    ({"train_impl": "dpo"}, "train_impl"), ({"train_impl": "reinforce"}, "train_impl"), ({"train_impl": "kto"}, "train_impl"),
+    ({"train_impl": "rm"}, "train_impl"), ({"checkpoint_activations": True}, "checkpoint_activations"), ({"moe_loss_coeff": 0.0}, "moe_loss_coeff")])
+def test_a_z_loss_that_would_not_train_is_refused(change, words):
+    """Where a layer's auxiliary loss does not reach the router: objectives that leave it out, layers that run without a record first."""
+    with pytest.raises(AssertionError, match=words):
+        make_args(**{**MOE, "moe_z_loss_coeff": 0.01, **change})
+    make_args(**{**MOE, **change})                                 # none asked for
+    make_args(**{**MOE, "moe_z_loss_coeff": 0.01})
