@@ -58,7 +58,11 @@ class OnlineDataset(torch.utils.data.Dataset):
         centred = rewards - baseline
         prefix = list(batch["prefix"])
         # log-probabilities of the completions' tokens under the policy that sampled them, for the clipped loss
-        logps = batch.get("logprobs") or [None] * len(batch["completions"])
+        logps = batch.get("logprobs")
+        if logps is None or len(logps) == 0:
+            logps = [None] * len(batch["completions"])
+        elif len(logps) != len(batch["completions"]):
+            raise ValueError(f"the data server sent log-probabilities of {len(logps)} completions with {len(batch['completions'])}")
         for comp, rw, raw, logp in zip(batch["completions"], centred, rewards, logps):
             toks = (prefix + list(comp))[: self.seq_length + 1]
             n = len(toks)

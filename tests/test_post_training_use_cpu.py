@@ -67,3 +67,38 @@ def test_a_z_loss_that_would_not_train_is_refused(change, words):
         make_args(**{**MOE, "moe_z_loss_coeff": 0.01, **change})
     make_args(**{**MOE, **change})                                 # none asked for
     make_args(**{**MOE, "moe_z_loss_coeff": 0.01})
+
+
+# ---------------------------------------------------------------------------------------------- online samples
+BATCH = {"prefix": [5, 6], "completions": [[8, 9], [10, 11, 12]], "rewards": [1.0, 0.0], "logprobs": [[-0.5, -0.25], [-1.0, -2.0, -3.0]]}
+
+
+def _online(*batches, **kw):
+    """An ``OnlineDataset`` on a server that sends these batches."""
+    from gpt_neox_b200.data.online_dataset import OnlineDataset
+    srv = socket.socket()
+    srv.bind(("127.0.0.1", 0))
+    srv.listen(2)
+
+    def serve():
+        for batch in batches:
+            conn, _ = srv.accept()
+            conn.recv(64)
+            conn.sendall(pickle.dumps(batch))
+            conn.close()
+    threading.Thread(target=serve, daemon=True).start()
+    return OnlineDataset(num_samples=4, seq_length=6, leave_one_out=True, dataserver_ips="127.0.0.1", dataserver_ports=srv.getsockname()[1],
+                         **kw)
+
+
+@pytest.mark.parametrize("logprobs", [[[-0.5, -0.25]], [[-0.5, -0.25], [-1.0, -2.0, -3.0], [-1.0]]])
+def test_online_log_probabilities_of_other_completions_are_refused(logprobs):
+    """One list a completion: with fewer, samples whose rewards are in the baseline would be lost."""
+    with pytest.raises(ValueError, match=f"log-probabilities of {len(logprobs)} completions"):
+        _online({**BATCH, "logprobs": logprobs})[0]
+
+
+def test_online_log_probabilities_may_come_as_arrays():
+    import numpy as np
+    ds = _online({**BATCH, "completions": [[8, 9], [10, 11]], "logprobs": np.array([[-0.5, -0.25], [-1.0, -2.0]])})
+    assert ds[0]["old_logp"].tolist() == [0, 0, -0.5, -0.25, 0, 0, 0] and ds[1]["old_logp"].tolist() == [0, 0, -1, -2, 0, 0, 0]
