@@ -222,7 +222,8 @@ def build_train_valid_test_data_loaders(neox_args):
             mk = lambda split, n: OnlineDataset(leave_one_out=a.reinforce_leave_one_out, data_split=split,
                                                 num_samples=n, seq_length=a.seq_length,
                                                 dataserver_ips=a.online_dataserver_ips,
-                                                dataserver_ports=a.online_dataserver_ports)
+                                                dataserver_ports=a.online_dataserver_ports,
+                                                needs_logprobs=a.train_impl == "reinforce" and a.reinforce_clip is not None)
             train_ds, valid_ds, test_ds = mk("train", nsamp[0]), mk("valid", nsamp[1]), mk("test", nsamp[2])
         elif _synthetic(a):
             mk = lambda n, s: SyntheticDataset(max(n or 0, a.train_batch_size), a.seq_length, a.padded_vocab_size,

@@ -3,7 +3,7 @@
 ``{"prefix": [...], "completions": [[...], ...], "rewards": [...]}`` batch; rewards are centred with a
 leave-one-out baseline or a moving average, and every completion becomes one sample with the prompt positions
 labelled -100.  An optional ``"logprobs": [[...], ...]`` (of every completion's tokens under the policy that sampled them) becomes
-``old_logp``, which ``reinforce_clip`` needs."""
+``old_logp``, which ``reinforce_clip`` needs (``needs_logprobs``: a batch without them is an error)."""
 from __future__ import annotations
 
 import pickle
@@ -17,9 +17,9 @@ import torch
 
 class OnlineDataset(torch.utils.data.Dataset):
     def __init__(self, num_samples, seq_length, leave_one_out=False, data_split="train", dataserver_ips="localhost",
-                 dataserver_ports=10000):
+                 dataserver_ports=10000, needs_logprobs=False):
         self.num_samples, self.seq_length, self.leave_one_out = num_samples, seq_length, leave_one_out
-        self.data_split = data_split
+        self.data_split, self.needs_logprobs = data_split, needs_logprobs
         self.ips = dataserver_ips if isinstance(dataserver_ips, (list, tuple)) else [dataserver_ips]
         self.ports = dataserver_ports if isinstance(dataserver_ports, (list, tuple)) else [dataserver_ports]
         self.queue = deque()
@@ -60,6 +60,8 @@ class OnlineDataset(torch.utils.data.Dataset):
         # log-probabilities of the completions' tokens under the policy that sampled them, for the clipped loss
         logps = batch.get("logprobs")
         if logps is None or len(logps) == 0:
+            if self.needs_logprobs:
+                raise ValueError("reinforce_clip compares with the sampler's log-probabilities, and the data server sent no logprobs")
             logps = [None] * len(batch["completions"])
         elif len(logps) != len(batch["completions"]):
             raise ValueError(f"the data server sent log-probabilities of {len(logps)} completions with {len(batch['completions'])}")

@@ -134,6 +134,9 @@ def get_batch(neox_args, data_iterator):
     if impl == "reinforce":
         clipped = neox_args.reinforce_clip is not None
         # the clipped loss compares with the sampler's log-probabilities, which only the completion's tokens have
+        for key in ("label", "old_logp") if clipped and data is not None else ():
+            if key not in data:
+                raise ValueError(f"reinforce_clip needs {key} in every batch, got {', '.join(sorted(data))}")
         tup = _get_batch(neox_args, neox_args.tokenizer, ["text", "label"] if clipped else ["text"], data, dt,
                          label_mask_zero=True)
         rws = broadcast_data(["reward", "raw_reward"], data, torch.float)

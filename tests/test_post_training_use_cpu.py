@@ -102,3 +102,20 @@ def test_online_log_probabilities_may_come_as_arrays():
     import numpy as np
     ds = _online({**BATCH, "completions": [[8, 9], [10, 11]], "logprobs": np.array([[-0.5, -0.25], [-1.0, -2.0]])})
     assert ds[0]["old_logp"].tolist() == [0, 0, -0.5, -0.25, 0, 0, 0] and ds[1]["old_logp"].tolist() == [0, 0, -1, -2, 0, 0, 0]
+
+
+def test_clipped_reinforce_names_what_its_samples_lack():
+    """Samples without the sampler's log-probabilities: the error says which key asked for them, where the data comes in and where
+    another loader's batch does."""
+    from gpt_neox_b200.training import get_batch
+    plain = {k: v for k, v in BATCH.items() if k != "logprobs"}
+    with pytest.raises(ValueError, match="reinforce_clip.*logprobs"):
+        _online(plain, needs_logprobs=True)[0]
+    assert "old_logp" not in _online(plain)[0]
+    assert "old_logp" in _online(BATCH, needs_logprobs=True)[0]
+    args = make_args(train_impl="reinforce", reinforce_clip=0.2)
+    text = torch.ones(2, 33, dtype=torch.long)
+    whole = {"text": text, "label": text, "reward": torch.ones(2, 33), "raw_reward": torch.ones(2), "old_logp": torch.zeros(2, 33)}
+    for key in ("label", "old_logp"):
+        with pytest.raises(ValueError, match=f"reinforce_clip needs {key}"):
+            get_batch(args, iter([{k: v for k, v in whole.items() if k != key}]))
