@@ -565,6 +565,12 @@ class NeoXArgs:
                 assert not self.checkpoint_activations, \
                     "moe_z_loss_coeff is not compatible with checkpoint_activations, which records no gradient of the auxiliary losses"
 
+        # options of the clipped objective
+        if self.reinforce_clip is None:
+            for key in ("reinforce_clip_high", "reinforce_sequence_mean"):
+                value = getattr(self, key)
+                assert value is None or value is False, f"{key} needs reinforce_clip: without it nothing is clipped"
+
         # attention pattern
         if self.num_layers is not None:
             cfg = self.attention_config if self.attention_config is not None else [[["global"], self.num_layers]]

@@ -216,7 +216,7 @@ data_impl : lit[infer|mmap|cached] = 'infer'
 pack_impl : lit[packed|pack_until_overflow|unpacked] = 'packed'
 dataset_impl : lit[gpt2|pairwise|online] = 'gpt2'
 train_impl : lit[normal|dpo|rm|kto|reinforce] = 'normal'
-dpo_fp32 : bool = True
+dpo_fp32 : bool = True                             # DPO in fp32, without a GPU; on one, logits are read in their own type, with statistics in fp32
 dpo_reference_free : bool = False
 dpo_beta : float = 0.1
 kto_fp32 : bool = True
@@ -224,13 +224,13 @@ kto_desirable_weight : float = 1.0
 kto_undesirable_weight : float = 1.0
 z_loss : float = 0.0
 kto_beta : float = 0.1
-fp32_reinforce : bool = True
+fp32_reinforce : bool = True                       # plain REINFORCE in fp32; the clipped objective reads logits in their own type, with statistics in fp32
 kl_impl : lit[abs|mse|kl|full|k3] = 'mse'
 kl_div_beta : float = 0.1
 reinforce_leave_one_out : bool = False
-reinforce_clip : float = None
-reinforce_clip_high : float = None
-reinforce_sequence_mean : bool = False
+reinforce_clip : float = None                      # the ratio to the sampler's log-probabilities is clipped from 1 - this; None = plain REINFORCE
+reinforce_clip_high : float = None                 # to 1 + this; None = as reinforce_clip
+reinforce_sequence_mean : bool = False             # with reinforce_clip: mean over sequences of their own means instead of over tokens
 allow_chopped : bool = True
 mmap_warmup : bool = False
 save : str = None

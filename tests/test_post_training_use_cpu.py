@@ -119,3 +119,10 @@ def test_clipped_reinforce_names_what_its_samples_lack():
     for key in ("label", "old_logp"):
         with pytest.raises(ValueError, match=f"reinforce_clip needs {key}"):
             get_batch(args, iter([{k: v for k, v in whole.items() if k != key}]))
+
+
+@pytest.mark.parametrize("key,value", [("reinforce_clip_high", 0.3), ("reinforce_clip_high", 0.0), ("reinforce_sequence_mean", True)])
+def test_options_of_the_clipped_objective_need_it(key, value):
+    with pytest.raises(AssertionError, match=f"{key} needs reinforce_clip"):
+        make_args(train_impl="reinforce", **{key: value})
+    make_args(train_impl="reinforce", reinforce_clip=0.2, **{key: value})
