@@ -59,12 +59,14 @@ class Sampler:
             if src in live and dst in sd and sd[dst].shape == live[src].shape:
                 sd[dst].copy_(live[src])
 
-    def generate(self, prompt_ids, n, max_new_tokens):
+    def generate(self, prompt_ids, n, max_new_tokens, whole=False):
+        """``whole``: from the whole distribution, which is what :meth:`logprobs` gives the log-probabilities of."""
         import torch
         ids = torch.tensor([prompt_ids], device="cuda")
+        cut = {"top_p": 1.0, "top_k": 0} if whole else {"top_p": 0.95}
         with torch.no_grad():
-            out = self.model.generate(ids, do_sample=True, temperature=1.0, top_p=0.95, num_return_sequences=n,
-                                      max_new_tokens=max_new_tokens, pad_token_id=self.tok.eos_token_id)
+            out = self.model.generate(ids, do_sample=True, temperature=1.0, num_return_sequences=n,
+                                      max_new_tokens=max_new_tokens, pad_token_id=self.tok.eos_token_id, **cut)
         return [o[len(prompt_ids):].tolist() for o in out]
 
     def logprobs(self, prompt_ids, completions):
@@ -99,7 +101,7 @@ def serve(args):
             sampler.refresh()
             text = random.choice(prompts)
             prefix = sampler.tok.apply_chat_template([{"role": "user", "content": text}], add_generation_prompt=True)
-            comps = sampler.generate(prefix, args.num_completions, args.max_new_tokens)
+            comps = sampler.generate(prefix, args.num_completions, args.max_new_tokens, whole=args.logprobs)
             payload = {"prefix": prefix, "completions": comps, "rewards": [reward_fn(sampler.tok, c) for c in comps]}
             if args.logprobs:
                 payload["logprobs"] = sampler.logprobs(prefix, comps)
@@ -116,5 +118,5 @@ if __name__ == "__main__":
     ap.add_argument("--prompts", default=None, help="text file with one prompt per line")
     ap.add_argument("--num-completions", type=int, default=4)
     ap.add_argument("--max-new-tokens", type=int, default=256)
-    ap.add_argument("--logprobs", action="store_true", help="send the tokens' log-probabilities (reinforce_clip)")
+    ap.add_argument("--logprobs", action="store_true", help="sample from the whole distribution and send the tokens' log-probabilities (reinforce_clip)")
     serve(ap.parse_args())

@@ -126,3 +126,23 @@ def test_options_of_the_clipped_objective_need_it(key, value):
     with pytest.raises(AssertionError, match=f"{key} needs reinforce_clip"):
         make_args(train_impl="reinforce", **{key: value})
     make_args(train_impl="reinforce", reinforce_clip=0.2, **{key: value})
+
+
+def test_example_server_samples_from_the_policy_whose_log_probabilities_it_sends(monkeypatch):
+    """With ``--logprobs`` the completions come from the whole distribution that the log-probabilities are of, not from its head."""
+    import importlib.util
+    import os
+    from types import SimpleNamespace
+    from common import ROOT
+    spec = importlib.util.spec_from_file_location("server", os.path.join(ROOT, "post-training", "online_data_example_llama3.py"))
+    server = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(server)
+    own = torch.tensor
+    monkeypatch.setattr(torch, "tensor", lambda *a, device=None, **kw: own(*a, **kw))
+    seen = []
+    sampler = server.Sampler.__new__(server.Sampler)
+    sampler.tok = SimpleNamespace(eos_token_id=0)
+    sampler.model = SimpleNamespace(generate=lambda ids, **kw: seen.append(kw) or torch.cat([ids, ids], 1))
+    assert sampler.generate([3, 4], 1, 2) == [[3, 4]] and seen[0]["top_p"] == 0.95
+    sampler.generate([3, 4], 1, 2, whole=True)
+    assert seen[1]["top_p"] == 1.0 and seen[1]["top_k"] == 0 and seen[1]["temperature"] == 1.0 and seen[1]["do_sample"]
