@@ -754,13 +754,13 @@ __global__ void __launch_bounds__(THREADS) preference_kernel(const PreferenceArg
         const double* c = whole + 2ll * b;
         const double* r = whole + 2ll * (b + pairs);
         const double z = a.beta * ((c[0] - r[0]) - (c[1] - r[1]));
-        const float small = __expf(-fabsf((float)z)), soft = log1pf(small), even = (float)a.smoothing;
+        const double small = exp(-fabs(z)), soft = log1p(small);
         double loss = (1.0 - a.smoothing) * (soft + fmax(-z, 0.0));
         if (a.smoothing != 0.0) loss += a.smoothing * (soft + fmax(z, 0.0));
-        sum[0] += z != z ? z : loss;
-        const float large = __frcp_rn(1.f + small), other = small * large;              // sigma(|z|), sigma(-|z|)
-        const float toward = z >= 0 ? other : large, away = z >= 0 ? large : other;     // sigma(-z), sigma(z)
-        const float d = z != z ? (float)z : (float)(-a.beta / pairs) * ((1.f - even) * toward - even * away);
+        sum[0] += loss;
+        const double large = 1.0 / (1.0 + small), other = small * large;                // sigma(|z|), sigma(-|z|)
+        const double toward = z >= 0 ? other : large, away = z >= 0 ? large : other;    // sigma(-z), sigma(z)
+        const float d = (float)(-a.beta / pairs * ((1.0 - a.smoothing) * toward - a.smoothing * away));
         a.coef[b] = d;
         a.coef[b + pairs] = -d;
     }

@@ -1,0 +1,36 @@
+"""Preference and policy loss on a GPU where their digits, their graphs and their choice of a path could differ from what is documented.
+
+ROW bounds what a row's log-probability is off by (``test_policy_losses_gpu.py`` derives it); where a log-probability is exact by
+construction the tests below allow roundings of the result alone."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from gpt_neox_b200.ops import policy_losses as PL
+
+DEV = "cuda"
+ROW = 2.0 ** -18
+
+
+def test_pairs_are_joined_in_64_bits():
+    """A vocabulary of two words 1024 apart has the log-probabilities 0 and -1024 exactly, so z is exact in 64 bits.  What is left is
+    one rounding of the loss (2^-24 of it) and, in the gradient, the roundings of the pair's coefficient, of its product with the
+    gradient of the loss, and of the result."""
+    x = torch.zeros(2, 1, 2, device=DEV)
+    x[0, 0, 1] = -1024.0
+    x[1, 0, 0] = -1024.0
+    mask = torch.ones(2, 1, device=DEV)
+    for label, sign in ((0, 1.0), (1, -1.0)):                      # the chosen answer more probable, and less
+        labels = torch.full((2, 1), label, device=DEV)
+        for size in (1e-3, 0.1, 0.7, 2.3, 5.1, 9.7, 13.3, 17.9, 25.1, 33.7, 51.3, 71.9):
+            for eps in (0.0, 0.1):
+                xl = x.clone().requires_grad_()
+                out = PL.preference_loss(xl, labels, mask, size / 1024.0, label_smoothing=eps)
+                grad, = torch.autograd.grad(out.loss, xl)
+                z = torch.tensor(sign * (size / 1024.0 * 1024.0), dtype=torch.float64)
+                want = -(1 - eps) * torch.nn.functional.logsigmoid(z) - eps * torch.nn.functional.logsigmoid(-z)
+                assert abs(float(out.loss.detach().double() - want)) <= 2.0 ** -24 * float(want) * 1.001, (size, sign, eps)
+                slope = -size / 1024.0 * ((1 - eps) * torch.sigmoid(-z) - eps * torch.sigmoid(z))
+                hot = abs(float(grad[0, 0, 1].double()))          # coefficient * (1 - 0) or (0 - 1), whichever word is impossible
+                assert abs(hot - (abs(float(slope)) if label else 0.0)) <= 2.0 ** -22 * abs(float(slope)), (size, sign, eps)
