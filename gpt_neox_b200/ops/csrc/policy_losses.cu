@@ -1339,7 +1339,8 @@ __global__ void __launch_bounds__(TPB, BLOCKS) policy_row_kernel(const AtOnceArg
             if (tid == 0) {
                 const double l = label_logp(a.vocab, label, own, m, t);
                 const RowTerm r(a.kl, a.low, a.high, a.kl_beta, l, a.old_logp != nullptr, old, adv, given, 0.0);
-                const float slope = (float)(weight * r.slope), inv = __frcp_rn((float)t), coef = a.expected * coef_i * slope;
+                const float slope = (float)(weight * r.slope), inv = __frcp_rn((float)t);
+                const float coef = slope == 0.f ? 0.f : a.expected * coef_i * slope;    // as in the second reading
                 grad = RowGrad{m, coef, -coef * inv};
                 where = (int)label;                             // one that does not fit has made everything NaN
                 a.row[row] = make_float2(m, inv);

@@ -34,3 +34,19 @@ def test_pairs_are_joined_in_64_bits():
                 slope = -size / 1024.0 * ((1 - eps) * torch.sigmoid(-z) - eps * torch.sigmoid(z))
                 hot = abs(float(grad[0, 0, 1].double()))          # coefficient * (1 - 0) or (0 - 1), whichever word is impossible
                 assert abs(hot - (abs(float(slope)) if label else 0.0)) <= 2.0 ** -22 * abs(float(slope)), (size, sign, eps)
+
+
+def test_clipped_tokens_leave_nothing_whatever_gradient_was_foreseen():
+    """A slope of zero gives zeros, also where the gradient of the loss is infinite and was foreseen."""
+    x = torch.randn(2, 6, 9000, device=DEV)
+    labels = torch.zeros(2, 6, dtype=torch.long, device=DEV)
+    mask, adv = torch.ones(2, 6, device=DEV), torch.ones(2, 6, device=DEV)
+    old = x.log_softmax(-1)[..., 0] - 1.0                          # a ratio of e: clipped, since the advantage is positive
+    old[0, 0] += 1.0                                              # but for one token
+    for foreseen in (float("inf"), 1.0):
+        xl = x.clone().requires_grad_()
+        out = PL.policy_loss(xl, labels, mask, adv, old_logp=old, grad_scale=foreseen)
+        grad, = torch.autograd.grad(out.loss, xl, torch.tensor(float("inf"), device=DEV))
+        rest = grad.flatten(0, 1)[1:]
+        assert not rest.any() and not bool(rest.isnan().any()), foreseen
+        assert not bool(grad[0, 0].isfinite().any()), foreseen
