@@ -43,3 +43,14 @@ extern "C" int neox_read_status() {
 }
 
 extern "C" int neox_sm_count_c() { return neox_sm_count(); }
+
+// Which capture a stream is part of: its number, unlike that of any other capture of the process, or 0 where nothing is captured.
+extern "C" unsigned long long neox_capture_id(void* stream) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (cudaStreamGetCaptureInfo((cudaStream_t)stream, &status, &id) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    return status == cudaStreamCaptureStatusActive ? id : 0;
+}

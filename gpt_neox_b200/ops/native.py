@@ -46,7 +46,9 @@ _ARGTYPES = {
     "neox_gemm_splits": [c_int, c_int, c_int],
     "neox_gemm_accumulate_16": [*_GEMM_HEAD, c_int, c_int, c_float, c_int, c_void_p, c_int, c_void_p],
     "neox_gemm_16_2cta": [*_GEMM_HEAD, c_int, c_int, *_GEMM_EPILOGUE, c_int, c_void_p],
+    "neox_capture_id": [c_void_p],
 }
+_RESTYPES = {"neox_capture_id": ctypes.c_ulonglong}    # others return an int
 
 launch_count = 0   # number of kernel-launching library calls made by this process (see bench.py)
 
@@ -55,7 +57,7 @@ class _CountingLib:
     """Proxy over the CDLL that counts calls into kernel launchers (``neox_*`` entry points that take a
     stream); pure queries such as ``neox_read_status`` are not counted."""
     _NOT_LAUNCHES = {"neox_read_status", "neox_norm_bwd_blocks", "neox_sm_count_c", "neox_causal_conv_blocks",
-                     "neox_gemm_splits"}
+                     "neox_gemm_splits", "neox_capture_id"}
 
     def __init__(self, cdll):
         self._cdll = cdll
@@ -67,6 +69,8 @@ class _CountingLib:
             raw = getattr(self._cdll, name)
             if name in _ARGTYPES:
                 raw.argtypes = _ARGTYPES[name]
+            if name in _RESTYPES:
+                raw.restype = _RESTYPES[name]
             if name in self._NOT_LAUNCHES:
                 fn = raw
             else:
@@ -113,6 +117,11 @@ def stream_ptr() -> int:
     """Handle of the current stream of the current device, without the Stream object that ``torch.cuda.current_stream()``
     builds around it (15 us)."""
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def capture_id() -> int:
+    """Number of the CUDA graph capture that the current stream is part of, 0 outside of one."""
+    return lib().neox_capture_id(stream_ptr())
 
 
 def plain_call(*tensors) -> bool:

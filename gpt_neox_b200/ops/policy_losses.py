@@ -340,7 +340,7 @@ class _PolicyFn(torch.autograd.Function):
                     ref_logp = _policy_values(ref_logits, labels, mask, adv, None, None, None, low, high, 0, 0.0, False)[3]
                 loss, kl_mean, clipped, logp, buf, ctx.grad = _policy_at_once(x, labels, mask, adv, old_logp, ref_logp, low, high, kl,
                                                                               kl_beta, by_sequence, expected)
-                ctx.streams = 0
+                ctx.streams, ctx.capture = 0, native.capture_id()
             else:
                 loss, kl_mean, clipped, logp, (buf, ctx.first) = _policy_values(x, *rest[:-1])
                 ctx.streams = 1 if ref_logits is None else 2
@@ -354,10 +354,13 @@ class _PolicyFn(torch.autograd.Function):
         if g_loss is None:
             return None, None
         x, labels, mask, buf, y = ctx.saved_tensors
-        # handed out once: a second backward through a retained graph writes another
-        g, ctx.grad = ctx.grad, None
-        done = g is not None
         with device_of(x):
+            # handed out once: a second backward through a retained graph writes another, as does one that is replayed without the
+            # forward or the other way round, since a gradient may be changed by whoever got it
+            done = ctx.grad is not None and native.capture_id() == ctx.capture
+            g = None
+            if done:
+                g, ctx.grad = ctx.grad, None
             if ctx.streams:
                 row, coef, slope, shift = _kept(x, buf, ctx.streams, 4, ctx.full)
             else:

@@ -50,3 +50,69 @@ def test_clipped_tokens_leave_nothing_whatever_gradient_was_foreseen():
         rest = grad.flatten(0, 1)[1:]
         assert not rest.any() and not bool(rest.isnan().any()), foreseen
         assert not bool(grad[0, 0].isfinite().any()), foreseen
+
+
+def test_a_captured_backward_of_an_eager_forward_writes_its_gradient_at_every_replay():
+    """The foreseen gradient is written once, by the forward: a backward that is replayed without it computes its own each time, and
+    the eager backward after it still finds the right one."""
+    x = torch.randn(2, 20, 9000, device=DEV)
+    labels = torch.randint(0, 9000, (2, 20), device=DEV)
+    mask = torch.ones(2, 20, device=DEV)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        leaf = x.clone().requires_grad_()
+        y = leaf * 1.0                                            # what is asked for is not a leaf
+        one = torch.ones((), device=DEV)
+        warm, = torch.autograd.grad(PL.policy_loss(y, labels, mask, mask).loss, y, one)
+        want = warm.clone()
+        loss = PL.policy_loss(y, labels, mask, mask).loss
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        grad, = torch.autograd.grad(loss, y, one, retain_graph=True)
+        grad.mul_(0.5)                                            # as a clipping of gradients does
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    # the same formula from the same statistics: roundings of the coefficient's products
+    top = want.abs().max()
+    assert float((grad - 0.5 * want).abs().max()) <= 2.0 ** -18 * float(top)
+    with torch.cuda.stream(stream):
+        again, = torch.autograd.grad(loss, y, one)
+    torch.cuda.synchronize()
+    assert float((again - want).abs().max()) <= 2.0 ** -18 * float(top)
+
+
+def test_an_eager_backward_of_a_captured_forward_has_a_gradient_of_its_own():
+    """The forward is replayed, its backward is not part of the graph: a gradient that was handed out stays as it is when the forward
+    is replayed on other logits."""
+    x = torch.randn(2, 20, 9000, device=DEV)
+    labels = torch.randint(0, 9000, (2, 20), device=DEV)
+    mask = torch.ones(2, 20, device=DEV)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        base = x.clone()
+        leaf = base.requires_grad_()
+        one = torch.ones((), device=DEV)
+        torch.autograd.grad(PL.policy_loss(leaf * 1.0, labels, mask, mask).loss, leaf, one)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        y = leaf * 1.0
+        loss = PL.policy_loss(y, labels, mask, mask).loss
+    with torch.cuda.stream(stream):
+        graph.replay()
+        first, = torch.autograd.grad(loss, y, one, retain_graph=True)
+        kept = first.clone()
+        with torch.no_grad():
+            base.mul_(0.25)
+        graph.replay()
+        second, = torch.autograd.grad(loss, y, one, retain_graph=True)
+    torch.cuda.synchronize()
+    assert torch.equal(first, kept)
+    yl = (0.25 * x).requires_grad_()
+    want, = torch.autograd.grad(PL.policy_loss(yl, labels, mask, mask).loss, yl, one)
+    assert float((second - want).abs().max()) <= 2.0 ** -18 * float(want.abs().max())
+    assert not torch.equal(first, second)
