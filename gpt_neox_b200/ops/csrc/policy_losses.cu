@@ -200,6 +200,9 @@ template <typename T> __device__ __forceinline__ void exps_of(const uint4& u, fl
 __device__ __forceinline__ void copy_16(void* to, const void* from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
 }
+__device__ __forceinline__ void copy_8(void* to, const void* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
 __device__ __forceinline__ void copies_sent() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int K> __device__ __forceinline__ void copies_here() { asm volatile("cp.async.wait_group %0;" ::"n"(K) : "memory"); }
 
@@ -788,6 +791,7 @@ struct PolicyArgs {
     float* kl_mean;
     float* share;                  // of clipped tokens
     float* logp;                   // [n, s]
+    double* wide;                  // [n, s] or none: the same of the kept rows, not rounded
     float* coef;                   // [n]: what a row's slope is multiplied by
 };
 
@@ -863,6 +867,7 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(const PolicyArgs a) {
             keep = make_float2(m, __frcp_rn((float)t));
             const double l = label_logp(a.sums.vocab, label, x, m, t);
             logp = (float)l;
+            if (a.wide) a.wide[row] = l;
             double ref = given, full = 0.0;
             if (a.kl == KL_FULL) {
                 const double gap = ((double)m - (double)mq) + (log(t) - log(tq));
@@ -1094,6 +1099,7 @@ struct AtOnceArgs {
     long long adv_n, adv_s;
     const float* old_logp;
     const float* ref_logp;
+    const double* ref_wide;        // or these: of the kept rows
     int n, s, vocab, kl, by_sequence;
     double low, high, kl_beta;
     float expected;
@@ -1237,6 +1243,8 @@ __global__ void __launch_bounds__(TPB, BLOCKS) policy_row_kernel(const AtOnceArg
     __shared__ RowGrad grad;
     __shared__ int where;
     __shared__ double terms[4], sums[4];                        // of a row and of all of them
+    __shared__ double wide;                                     // the row's reference in 64 bits: it comes with the logits, since a
+                                                                // register for it all the way costs the statistics 4 %
     if (threadIdx.x < 4) sums[threadIdx.x] = 0.0;
     const int tid = threadIdx.x, rows = a.n * a.s;
     launch::wait_for_predecessor();
@@ -1258,6 +1266,9 @@ __global__ void __launch_bounds__(TPB, BLOCKS) policy_row_kernel(const AtOnceArg
         return p;
     };
     auto request = [&](const Place& p, int v) { copy_16(xs + v, reinterpret_cast<const uint4*>(p.x + p.head) + v); };
+    auto request_wide = [&](const Place& p) {
+        if (tid == 0 && a.ref_wide) copy_8(&wide, a.ref_wide + p.row);
+    };
     // this block's rows: every gridDim.x-th of the kept ones and of the others
     const int grid = gridDim.x, block = blockIdx.x;
     const int mine = block < kept ? (kept - 1 - block) / grid + 1 : 0;
@@ -1278,6 +1289,7 @@ __global__ void __launch_bounds__(TPB, BLOCKS) policy_row_kernel(const AtOnceArg
     Place now = {};
     if (mine > 0) {
         now = place(block);
+        request_wide(now);
 #pragma unroll
         for (int q = 0; q < PARTS; ++q) {
             for (int v = q * part + tid; v < min((q + 1) * part, now.vectors); v += TPB) request(now, v);
@@ -1338,7 +1350,8 @@ __global__ void __launch_bounds__(TPB, BLOCKS) policy_row_kernel(const AtOnceArg
             const double t = warp_sum(is ? (double)ps[tid].t * (double)__expf(ps[tid].m - m) : 0.0);
             if (tid == 0) {
                 const double l = label_logp(a.vocab, label, own, m, t);
-                const RowTerm r(a.kl, a.low, a.high, a.kl_beta, l, a.old_logp != nullptr, old, adv, given, 0.0);
+                const RowTerm r(a.kl, a.low, a.high, a.kl_beta, l, a.old_logp != nullptr, old, adv, a.ref_wide ? wide : (double)given,
+                                0.0);
                 const float slope = (float)(weight * r.slope), inv = __frcp_rn((float)t);
                 const float coef = slope == 0.f ? 0.f : a.expected * coef_i * slope;    // as in the second reading
                 grad = RowGrad{m, coef, -coef * inv};
@@ -1359,6 +1372,7 @@ __global__ void __launch_bounds__(TPB, BLOCKS) policy_row_kernel(const AtOnceArg
         const RowGrad r = grad;
         const int hot = where;
         if (tid < 4) sums[tid] += terms[tid];
+        request_wide(next);
         T* g = reinterpret_cast<T*>(a.g) + (long long)i * a.gn + (long long)j * a.gs;
         if ((((uintptr_t)x ^ (uintptr_t)g) & 15) != 0) {
             write_apart<T, TPB>(x, g, a.vocab, tid, r, hot);
@@ -1512,6 +1526,7 @@ struct LossCall {
     long long v0, whole;           // first word of this share of the vocabulary; words of all shares
     void* stream;
     float* terms;                  // scratch of the policy loss with its gradient: 4 doubles a block, n doubles, n * s + 2 ints
+    double* wide;                  // [n, s] or null: log-probabilities in 64 bits, left by one forward and another's reference
     double beta, smoothing, low, high;       // beta: of the preference, or the KL's weight
     double expected;               // gradient of the loss that the forward writes its gradient for
     int n, s, vocab, dtype;
@@ -1558,7 +1573,7 @@ int neox_loss_forward(const void* packed) {
     if (c.policy) {
         const PolicyArgs a = {sums, c.mask, c.advantages, c.adv_n, c.adv_s, c.old_logp, c.ref_logp, c.y != nullptr, c.n, c.s,
                               (int)pieces, c.kl, c.by_sequence, c.low, c.high, c.beta, c.row, c.slope, c.shift, c.sums, c.ticket,
-                              c.loss, c.kl_mean, c.clipped, c.logp, c.coef};
+                              c.loss, c.kl_mean, c.clipped, c.logp, c.wide, c.coef};
         return launch::overlapped(policy_kernel, grid, dim3(THREADS), 1, st, a);
     }
     const PreferenceArgs a = {sums, c.mask, c.ref_logp, c.y != nullptr, c.n, c.s, (int)pieces, c.beta, c.smoothing, c.row, c.sums,
@@ -1578,7 +1593,7 @@ int neox_policy_at_once(const void* packed) {
     if (rows >= MOST_TOKENS) return NEOX_ERR_TOO_LARGE;
     double* whole = (double*)c.terms + 4 * (rows < MOST_PARTS ? rows : MOST_PARTS);
     const AtOnceArgs a = {{c.x, c.xn, c.xs}, c.g, c.gn, c.gs, c.labels, c.mask, c.advantages, c.adv_n, c.adv_s, c.old_logp,
-                          c.ref_logp, c.n, c.s, c.vocab, c.kl, c.by_sequence, c.low, c.high, c.beta, (float)c.expected, c.row, c.slope,
+                          c.ref_logp, c.wide, c.n, c.s, c.vocab, c.kl, c.by_sequence, c.low, c.high, c.beta, (float)c.expected, c.row, c.slope,
                           (double*)c.terms, whole, (int*)(whole + c.n), c.coef, c.loss, c.kl_mean, c.clipped, c.logp};
     cudaStream_t st = (cudaStream_t)c.stream;
     policy_share_kernel<<<1, 1024, 0, st>>>(a);

@@ -38,7 +38,7 @@ native._CountingLib._NOT_LAUNCHES.update({"neox_vocab_chunks", "neox_loss_pieces
 _MOST_TOKENS = 1 << 30                  # the kernels number them, and steps past the last one, in 32 bits
 
 # The kernels' arguments in the order of LossCall (csrc/policy_losses.cu): addresses and 64-bit words, doubles, ints.
-_CALL = struct.Struct("@36q5d12i")
+_CALL = struct.Struct("@37q5d12i")
 
 
 class PreferenceLoss(NamedTuple):
@@ -160,7 +160,7 @@ def _reduced(buf, at, streams, rows, most, full, group):
 
 
 def _forward(x, y, labels, mask, width, loss, kl_mean, clipped, logp, ref, old_logp, ref_logp, adv, kl, by_sequence, beta, smoothing,
-             low, high):
+             low, high, wide=None):
     """Runs a forward into the given outputs; the buffer whose end the backward needs, and the first word of this rank's share of
     the vocabulary."""
     n, s, v = x.shape
@@ -178,7 +178,8 @@ def _forward(x, y, labels, mask, width, loss, kl_mean, clipped, logp, ref, old_l
             0 if old_logp is None else old_logp.data_ptr(), 0 if ref_logp is None else ref_logp.data_ptr(),
             *((0, 0, 0) if adv is None else (adv.data_ptr(), adv.stride(0) if adv.shape[0] > 1 else 0,
                                              adv.stride(1) if adv.shape[1] > 1 else 0)),
-            0, 0, 0, 0, 0, rank * v, tp * v, native.stream_ptr(), 0, beta, smoothing, low, high, 0.0, n, s, v, dt, kl, by_sequence)
+            0, 0, 0, 0, 0, rank * v, tp * v, native.stream_ptr(), 0, 0 if wide is None else wide.data_ptr(), beta, smoothing, low, high, 0.0,
+            n, s, v, dt, kl, by_sequence)
     run = native.lib().neox_loss_forward
     policy = width == 4
     if tp == 1:
@@ -214,7 +215,7 @@ def _backward(x, y, labels, mask, g, row, coef, slope, shift, first, g_loss, g_l
     call = _CALL.pack(x.data_ptr(), x.stride(0), x.stride(1), y_.data_ptr(), y_.stride(0), y_.stride(1), labels.data_ptr(),
                       mask.data_ptr(), 0, 0, 0, 0, 0, row, coef, slope, shift, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, g.data_ptr(), g.stride(0),
                       g.stride(1), 0 if g_loss is None else g_loss.data_ptr(), 0 if g_logp is None else g_logp.data_ptr(), first, 0,
-                      native.stream_ptr(), 0, beta, 0.0, 0.0, 0.0, expected, n, s, v, _DT[x.dtype], 0, 0, 0, 0, 0, 0, 0, done)
+                      native.stream_ptr(), 0, 0, beta, 0.0, 0.0, 0.0, expected, n, s, v, _DT[x.dtype], 0, 0, 0, 0, 0, 0, 0, done)
     native.check(native.lib().neox_loss_backward(call), "neox_loss_backward")
     return g
 
@@ -266,14 +267,14 @@ class _PreferenceFn(torch.autograd.Function):
         return once(g, x), None
 
 
-def _policy_values(x, labels, mask, adv, old_logp, ref_logits, ref_logp, low, high, kl, kl_beta, by_sequence):
+def _policy_values(x, labels, mask, adv, old_logp, ref_logits, ref_logp, low, high, kl, kl_beta, by_sequence, wide=None):
     dev = x.device
     loss = torch.empty((), dtype=torch.float32, device=dev)
     kl_mean = torch.empty((), dtype=torch.float32, device=dev)
     clipped = torch.empty((), dtype=torch.float32, device=dev)
     logp = torch.empty(x.shape[:2], dtype=torch.float32, device=dev)
     kept = _forward(x, ref_logits, labels, mask, 4, loss, kl_mean, clipped, logp, None, old_logp, ref_logp, adv, kl, by_sequence, kl_beta,
-                    0.0, low, high)
+                    0.0, low, high, wide)
     return loss, kl_mean, clipped, logp, kept
 
 
@@ -291,8 +292,9 @@ def _at_once_layout(n, s):
     return row, coef, slope, terms, at
 
 
-def _policy_at_once(x, labels, mask, adv, old_logp, ref_logp, low, high, kl, kl_beta, by_sequence, expected):
-    """The policy loss and, from the same reading of the logits, its gradient for a gradient ``expected`` of the loss."""
+def _policy_at_once(x, labels, mask, adv, old_logp, ref_logp, wide, low, high, kl, kl_beta, by_sequence, expected):
+    """The policy loss and, from the same reading of the logits, its gradient for a gradient ``expected`` of the loss.  ``wide``: the
+    reference's log-probabilities in 64 bits, in place of ``ref_logp``."""
     n, s, v = x.shape
     dev = x.device
     loss = torch.empty((), dtype=torch.float32, device=dev)
@@ -307,8 +309,8 @@ def _policy_at_once(x, labels, mask, adv, old_logp, ref_logp, low, high, kl, kl_
                       slope, 0, loss.data_ptr(), kl_mean.data_ptr(), clipped.data_ptr(), logp.data_ptr(), 0,
                       0 if old_logp is None else old_logp.data_ptr(), 0 if ref_logp is None else ref_logp.data_ptr(),
                       adv.data_ptr(), adv.stride(0) if adv.shape[0] > 1 else 0, adv.stride(1) if adv.shape[1] > 1 else 0,
-                      g.data_ptr(), g.stride(0), g.stride(1), 0, 0, 0, v, native.stream_ptr(), terms, kl_beta, 0.0, low, high,
-                      expected, n, s, v, _DT[x.dtype], kl, by_sequence, 0, 0, 1, 0, 0, 1)
+                      g.data_ptr(), g.stride(0), g.stride(1), 0, 0, 0, v, native.stream_ptr(), terms,
+                      0 if wide is None else wide.data_ptr(), kl_beta, 0.0, low, high, expected, n, s, v, _DT[x.dtype], kl, by_sequence, 0, 0, 1, 0, 0, 1)
     native.check(native.lib().neox_policy_at_once(call), "neox_policy_at_once")
     return loss, kl_mean, clipped, logp, buf, g
 
@@ -336,9 +338,11 @@ class _PolicyFn(torch.autograd.Function):
         ctx.full, ctx.kl_beta, ctx.expected, ctx.first, ctx.grad = int(kl == KL_KINDS["full"]), kl_beta, expected, 0, None
         with device_of(x):
             if at_once:
+                wide = None
                 if ref_logits is not None:
-                    ref_logp = _policy_values(ref_logits, labels, mask, adv, None, None, None, low, high, 0, 0.0, False)[3]
-                loss, kl_mean, clipped, logp, buf, ctx.grad = _policy_at_once(x, labels, mask, adv, old_logp, ref_logp, low, high, kl,
+                    wide = torch.empty(x.shape[:2], dtype=torch.float64, device=x.device)
+                    _policy_values(ref_logits, labels, mask, adv, None, None, None, low, high, 0, 0.0, False, wide)
+                loss, kl_mean, clipped, logp, buf, ctx.grad = _policy_at_once(x, labels, mask, adv, old_logp, ref_logp, wide, low, high, kl,
                                                                               kl_beta, by_sequence, expected)
                 ctx.streams, ctx.capture = 0, native.capture_id()
             else:

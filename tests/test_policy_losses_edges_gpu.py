@@ -36,6 +36,27 @@ def test_pairs_are_joined_in_64_bits():
                 assert abs(hot - (abs(float(slope)) if label else 0.0)) <= 2.0 ** -22 * abs(float(slope)), (size, sign, eps)
 
 
+def test_reference_read_first_keeps_the_digits_of_improbable_labels(monkeypatch):
+    """Labels of log-probabilities near -3000: their difference between policy and reference is as near as below the size from which
+    the reference is read first, whose log-probabilities in 32 bits would be off by up to 2^-13."""
+    n, s, v = 1, 16, 9000
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.randn(n, s, v, device=DEV, generator=g) * 2
+    y = x + 0.3 * torch.randn(n, s, v, device=DEV, generator=g)
+    labels = torch.randint(0, v, (n, s), device=DEV, generator=g)
+    x.scatter_(2, labels[..., None], -3000.0)
+    y.scatter_(2, labels[..., None], -3000.25)
+    lp = lambda t: t.double().log_softmax(-1).gather(-1, labels[..., None])[..., 0]       # noqa: E731
+    want = lp(x) - lp(y)
+    for first in (0, 1 << 62):
+        monkeypatch.setattr(PL, "_REF_FIRST", first)
+        for j in range(s):
+            mask = torch.zeros(n, s, device=DEV)
+            mask[0, j] = 1.0
+            out = PL.policy_loss(x.requires_grad_(), labels, mask, mask, ref_logits=y, kl="kl", kl_beta=0.1)
+            assert abs(float(out.kl.double() - want[0, j])) <= 2 * ROW + 2.0 ** -24 * abs(float(want[0, j])), (first, j)
+
+
 def test_clipped_tokens_leave_nothing_whatever_gradient_was_foreseen():
     """A slope of zero gives zeros, also where the gradient of the loss is infinite and was foreseen."""
     x = torch.randn(2, 6, 9000, device=DEV)
