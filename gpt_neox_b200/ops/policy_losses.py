@@ -319,6 +319,9 @@ def _policy_at_once(x, labels, mask, adv, old_logp, ref_logp, wide, low, high, k
 # are read once: forward and backward of 8 x 1024 tokens over 50304 16-bit words (824 MB) 336 us so, 361 with both read together and
 # the policy's twice; 4 x 4096 over 32064 (1 GB) 433 and 473; 4 x 512 over 50304 (206 MB) 116 and 118, but 30 us more for the host.
 _REF_FIRST = 1 << 29
+# Estimates whose references are always read together with the policy: the KL over the vocabulary, and |d|, whose slope jumps at d = 0,
+# so that a policy equal to its reference -- the first step of training -- needs both log-probabilities from sums of the same order.
+_TOGETHER = (KL_KINDS["full"], KL_KINDS["abs"])
 
 
 @functools.lru_cache(maxsize=256)
@@ -333,7 +336,7 @@ class _PolicyFn(torch.autograd.Function):
         labels, mask, adv, old_logp, ref_logits, ref_logp, low, high, kl, kl_beta, by_sequence, expected = rest
         # 16-bit floating-point numbers of five exponent bits need the loss scale before they are rounded
         at_once = ctx.needs_input_grad[0] and x.shape[1] > 0 and _tensor_parallel()[0] == 1 and (x.dtype != torch.float16 or expected != 1.0) \
-            and (ref_logits is None or (kl != KL_KINDS["full"] and x.numel() * x.element_size() >= _REF_FIRST)) \
+            and (ref_logits is None or (kl not in _TOGETHER and x.numel() * x.element_size() >= _REF_FIRST)) \
             and _one_reading_pays(x.shape[2], x.dtype)
         ctx.full, ctx.kl_beta, ctx.expected, ctx.first, ctx.grad = int(kl == KL_KINDS["full"]), kl_beta, expected, 0, None
         with device_of(x):
@@ -516,7 +519,7 @@ def policy_loss(logits, labels, loss_mask, advantages, old_logp: Optional[torch.
     ``1 / accumulation steps`` for a scaled loss.  Where the logits ask for a gradient, it is computed for that value together with
     the loss, while a row is at hand (its memory is taken then), and the backward only has to look; any other gradient of the loss
     is right as well, and costs the second reading of the logits that was to be saved.  (With the KL over the whole vocabulary, with
-    fp16 logits and ``grad_scale`` 1, with reference logits in a small batch, and for vocabularies that are short, split over ranks
+    fp16 logits and ``grad_scale`` 1, with reference logits in a small batch or for ``"abs"``, and for vocabularies that are short, split over ranks
     or too long for shared memory, logits are always read twice.)
     """
     _check(logits, labels, loss_mask, ref_logits, ref_logp)

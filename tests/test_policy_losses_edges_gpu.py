@@ -57,6 +57,29 @@ def test_reference_read_first_keeps_the_digits_of_improbable_labels(monkeypatch)
             assert abs(float(out.kl.double() - want[0, j])) <= 2 * ROW + 2.0 ** -24 * abs(float(want[0, j])), (first, j)
 
 
+@pytest.mark.parametrize("kl", ["kl", "abs", "mse", "k3"])
+@pytest.mark.parametrize("order", ["bsv", "sbv"])
+def test_reference_equal_to_the_policy_pulls_nowhere(kl, order, monkeypatch):
+    """As at the first step of training, whatever the batch's size: d is zero, and with it the slope of |d|, which is none or the whole
+    weight.  The other slopes follow d, which is off by 2 ROW at most."""
+    n, s, v = 3, 40, 9000
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = (torch.randn(*((n, s) if order == "bsv" else (s, n)), v, device=DEV, generator=g) * 2).to(torch.bfloat16)
+    x = x if order == "bsv" else x.transpose(0, 1)
+    labels = torch.randint(0, v, (n, s), device=DEV, generator=g)
+    mask = torch.ones(n, s, device=DEV)
+    for first in (0, 1 << 62):
+        monkeypatch.setattr(PL, "_REF_FIRST", first)
+        xl = x.detach().requires_grad_()
+        out = PL.policy_loss(xl, labels, mask, 0 * mask, ref_logits=x.clone(), kl=kl, kl_beta=1.0)
+        grad, = torch.autograd.grad(out.loss, xl)
+        assert abs(float(out.kl)) <= 2 * ROW
+        if kl == "kl":
+            assert float(grad.abs().max()) > 0.9 / (n * s)         # its slope is one everywhere
+        else:
+            assert float(grad.abs().max()) <= (0.0 if kl == "abs" else 2 * ROW / (n * s)), (first, float(grad.abs().max()))
+
+
 def test_clipped_tokens_leave_nothing_whatever_gradient_was_foreseen():
     """A slope of zero gives zeros, also where the gradient of the loss is infinite and was foreseen."""
     x = torch.randn(2, 6, 9000, device=DEV)
