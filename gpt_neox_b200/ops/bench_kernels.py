@@ -451,6 +451,8 @@ def moe_kernels(a, dev, bf, flush):
         ("expert_fc1_wgrad_fp32_accumulate", flops, 0.0, {"per_expert_loop": loop_wgrad, "grouped": grouped_wgrad}),
         ("router_softmax_top2", 0.0, T * E * (2 + 4) + T * k * 12.0,
          {"torch": lambda: MO.router_ref(logits, k), "kernel": lambda: MO.router(logits, k)}),
+        ("router_with_losses_top2", 0.0, T * E * 2 + T * k * 12.0,
+         {"torch": lambda: MO.balanced_router_ref(logits, k), "kernel": lambda: MO.balanced_router(logits, k)}),
         ("dispatch_rows", 0.0, T * h * 2.0 + T * k * h * 2.0 + rows * h * 2.0,
          {"torch": lambda: MO.dispatch_ref(x, row_of, rows), "kernel": lambda: MO.dispatch(x, row_of, rows)}),
         ("combine_rows", 0.0, T * k * h * 2.0 + T * h * 2.0,

@@ -90,7 +90,8 @@ class _RouterFn(torch.autograd.Function):
 
 
 def router(logits, k):
-    """``(probs [T, E] fp32, weights [T, k] fp32 (renormalised for k > 1), experts [T, k] int64, counts [E] int64)``."""
+    """``(probs [T, E] fp32, weights [T, k] fp32 (renormalised for k > 1), experts [T, k] int64, counts [E] int64)``, for callers who
+    want all probabilities; the models' layers run :func:`balanced_router`."""
     if router_kernel_ok(logits, k):
         return _RouterFn.apply(logits, k)
     return router_ref(logits, k)

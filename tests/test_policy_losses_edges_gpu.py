@@ -160,3 +160,63 @@ def test_an_eager_backward_of_a_captured_forward_has_a_gradient_of_its_own():
     want, = torch.autograd.grad(PL.policy_loss(yl, labels, mask, mask).loss, yl, one)
     assert float((second - want).abs().max()) <= 2.0 ** -18 * float(want.abs().max())
     assert not torch.equal(first, second)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("kl,ref", [("k3", "logits"), ("mse", "logits"), ("k3", "logp"), ("kl", "none")])
+def test_clipped_loss_over_a_split_vocabulary(kl, ref, dtype, monkeypatch):
+    """Two tensor-parallel shares of the vocabulary, one after the other: what either hands to the all-reduces is recorded and joined,
+    and the third round, with the joined values, gives the loss and gradient of the whole vocabulary.  Either side's rows are off by
+    ROW, their gradients rounded once."""
+    import torch.distributed as dist
+    n, s, v, cut = 3, 17, 6000, 3000
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = (torch.randn(n, s, v, device=DEV, generator=g) * 2).to(dtype)
+    labels = torch.randint(0, v, (n, s), device=DEV, generator=g)
+    labels[0, 0], labels[0, 1], labels[0, 2], labels[0, 3] = 0, cut - 1, cut, v - 1
+    mask = (torch.rand(n, s, device=DEV, generator=g) > 0.4).float()
+    mask[0, :4] = 1.0
+    adv = torch.randn(n, s, device=DEV, generator=g)
+    y = x + (0.3 * torch.randn(n, s, v, device=DEV, generator=g)).to(dtype)
+    logp = x.double().log_softmax(-1).gather(-1, labels[..., None])[..., 0]
+    old = (logp + 0.1 * torch.randn(n, s, device=DEV, generator=g)).float()
+    stored = (logp + 0.2 * torch.randn(n, s, device=DEV, generator=g)).float()
+    beta, sent, rank_now, joined = 0.3, [[], []], [0], []
+
+    def all_reduce(t, op=None, group=None):
+        i = len(sent[rank_now[0]])
+        sent[rank_now[0]].append(t.clone())
+        if i < len(joined):
+            t.copy_(joined[i])
+
+    def loss_of(x, y):
+        x = x.detach().requires_grad_()
+        given = {"logits": {"ref_logits": y}, "logp": {"ref_logp": stored}, "none": {}}[ref]
+        out = PL.policy_loss(x, labels, mask, adv, old_logp=old, kl=kl, kl_beta=beta, reduce="sequence", **given)
+        return out.loss.detach(), out.logp, out.kl, torch.autograd.grad(out.loss, x)[0]
+
+    def share(rank):
+        rank_now[0] = rank
+        sent[rank].clear()
+        at = slice(rank * cut, (rank + 1) * cut)
+        return loss_of(x[..., at], y[..., at])
+
+    with monkeypatch.context() as m:
+        m.setattr(PL, "_tensor_parallel", lambda: (2, rank_now[0], lambda: None))
+        m.setattr(dist, "all_reduce", all_reduce)
+        share(0), share(1)
+        joined.append(torch.maximum(sent[0][0], sent[1][0]))
+        share(0), share(1)
+        joined.append(sent[0][1] + sent[1][1])
+        got = [share(0), share(1)]
+    loss, lp, mean_kl, grad = loss_of(x, y)
+    d = logp - (y.double().log_softmax(-1).gather(-1, labels[..., None])[..., 0] if ref == "logits" else stored.double())
+    steep = {"k3": torch.exp(-d) + 1, "mse": d.abs() + 1, "kl": torch.ones_like(d)}[kl]      # of the estimate and of its slope
+    ratio = (logp - old.double()).exp()
+    most = float(((ratio * adv.double().abs() + beta * steep) * (mask != 0)).max())
+    for r in (0, 1):
+        assert abs(float(got[r][0] - loss)) <= 4 * ROW * most
+        assert float((got[r][1] - lp).abs().max()) <= 4 * ROW and abs(float(got[r][2] - mean_kl)) <= 4 * ROW * float(steep.max())
+        want = grad[..., r * cut:(r + 1) * cut].double()
+        off = (got[r][3].double() - want).abs()
+        assert bool((off <= torch.finfo(dtype).eps * want.abs() + 8 * ROW * most / n).all())
