@@ -8,11 +8,15 @@
 // with one a (and, for the KL over the whole vocabulary, one b) a row.
 //
 // Three kernels.  `stats_kernel` streams the kept rows once and leaves (max, sum of exponentials) of every chunk of a row;
-// `preference_kernel` / `policy_kernel` join them, eight lanes a row, in 64 bits from the sums on, and the last block to finish
-// forms the loss and what the backward multiplies; `grad_kernel` streams the rows a second time and writes the gradient, zeros
+// `preference_kernel` / `policy_kernel` join them, eight lanes a row, and the last block to finish forms the loss and what the
+// backward multiplies; `grad_kernel` streams the rows a second time and writes the gradient, zeros
 // where the coefficient is zero, without reading.  The second pass over the logits cannot be saved for a preference loss: a
 // pair's coefficient depends on all of its rows.  It can be for a policy loss, whose rows need only the sum of the mask from one
 // another: `policy_row_kernel`, further down, has a row in shared memory and writes its gradient with its loss.
+//
+// Exponentials, a lane's sums of them and gradients are in 32 bits; the lanes' sums are joined in 64, and so is everything up to the
+// loss; coefficients, 1 / sum and outputs are rounded to 32.  Of a row's log-probability that leaves an error of 1e-8 to 2e-8 in half of
+// the rows, and of at most some 2e-7 in those that one word outweighs (rows of 32000 to 50432 words).
 //
 // All of it is bound by memory traffic.  8 x 1024 tokens over 50304 bf16 words, 4506 kept, on a machine whose copies run at 6.55
 // TB/s: statistics 80 us (5.7 TB/s), joining 7, gradient 190 (6.7 TB/s); loss and gradient at once 226 (5.7 TB/s).
@@ -138,6 +142,14 @@ __device__ __forceinline__ float exp2_fast(float v) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
+// exp(d) of the gap between two maxima, d <= 0, for the few factors that whole sums are multiplied by.  Made good are the rounding of
+// the product, that of log2 e, and what ex2 is low by on average (measured: 2.2e-8 of its result for arguments above -1, 5e-8 below).
+__device__ __forceinline__ float exp_of_gap(float d) {
+    const float t = d * LOG2E, low = fmaf(d, LOG2E, -t) + d * 1.925963e-8f, e = exp2_fast(t);
+    return d < -150.f ? 0.f : fmaf(e, fmaf(low, 0.6931472f, t < -1.f ? 5e-8f : 2.2e-8f), e);
+}
+__device__ __forceinline__ f32x2 tree_sum(const f32x2 (&v)[2]) { return add(v[0], v[1]); }
+__device__ __forceinline__ f32x2 tree_sum(const f32x2 (&v)[4]) { return add(add(v[0], v[1]), add(v[2], v[3])); }
 // exp(x + shift).  The sum first: a row's largest and lowest numbers may be as large as the type has them, and the difference of
 // two 16-bit numbers near each other is exact.
 __device__ __forceinline__ f32x2 exp_of(f32x2 x, f32x2 shift) {
@@ -250,12 +262,18 @@ template <bool FULL> struct Shape {
 constexpr int MOST_ROWS = 1024;                                 // rows a block keeps at a time
 constexpr int SCAN = 8;                                         // mask words a lane has in flight
 
+// What is left of a chunk of a row.
+struct __align__(16) Part {
+    double t;                      // sum of exponentials against
+    float m;                       // the maximum
+    float w;                       // sum of p (x - y), for the KL over the vocabulary
+};
+
 struct StatsArgs {
     Rows x, y;                     // policy and reference
     const long long* labels;       // [n, s]
     const float* mask;             // [n, s]
-    float2* part;                  // [streams][rows, most]: (max, sum) of a chunk of a row
-    float* cross;                  // [rows, most]: sum of p (x - y)
+    Part* part;                    // [streams][rows, most]
     float* target;                 // [streams][rows]: the label's logit where this share of the vocabulary has it, else 0
     int* ticket;                   // zero for the next kernel, then the number of chunks
     long long v0;
@@ -274,11 +292,12 @@ __host__ __device__ __forceinline__ float cut_cost(long long rows, int vocab, in
 __host__ __device__ __forceinline__ int chunk_size(int vocab, int chunks) { return ((vocab + chunks - 1) / chunks + 7) / 8 * 8; }
 
 // (m, t): maximum and sum of exponentials against it.
-struct Sums {
-    float m, t;
+template <typename V> struct Sums {
+    float m;
+    V t;
     __device__ __forceinline__ void join_warp() {
         const float top = warp_max(m);
-        t = warp_sum(t * __expf(m - top));
+        t = warp_sum(t * (V)exp_of_gap(m - top));
         m = top;
     }
 };
@@ -370,7 +389,8 @@ template <typename T, bool FULL, int U, int STRIDE> struct Running {
         const float px = as_max<T>(p), qx = FULL ? as_max<T>(q) : n;
         if (px > m || qx > n) raise(fmaxf(m, px), fmaxf(n, qx));
         const f32x2 xs = pair(-m, -m), ys = pair(-n, -n), minus = pair(-1.f, -1.f);
-        f32x2 gap = pair(0.f, 0.f);
+        // a vector's sum first, then a step's: next to a word that outweighs the others they would lose their last bits one by one
+        f32x2 gap = pair(0.f, 0.f), step = gap, step_r = gap;
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (whole || u * STRIDE < left) {
@@ -383,14 +403,21 @@ template <typename T, bool FULL, int U, int STRIDE> struct Running {
                     for (int i = 0; i < N / 2; ++i) {
                         e[i] = exp_of(v[i], xs);
                         gap = fma(e[i], fma(q2[i], minus, v[i]), gap);
-                        r = add(r, exp_of(q2[i], ys));
+                        q2[i] = exp_of(q2[i], ys);
                     }
+                    step_r = u == 0 ? tree_sum(q2) : add(step_r, tree_sum(q2));
                 } else {
                     exps_of<T>(xr[u], m, e);
                 }
+                if constexpr (STRIDE == 32) {
+                    step = u == 0 ? tree_sum(e) : add(step, tree_sum(e));
+                } else {
 #pragma unroll
-                for (int i = 0; i < N / 2; ++i) t = add(t, e[i]);
+                    for (int i = 0; i < N / 2; ++i) step = u == 0 && i == 0 ? e[0] : add(step, e[i]);
+                }
             }
+        t = add(t, step);
+        if constexpr (FULL) r = add(r, step_r);
         if constexpr (FULL) {
             const float2 g = parts(gap);
             if (g.x + g.y != g.x + g.y) {                       // 0 times infinity somewhere: what is impossible adds nothing
@@ -571,19 +598,17 @@ __global__ void __launch_bounds__(Shape<FULL>::WARPS * 32, 1) stats_kernel(const
             }
             const int row = sm.list[now.entry].row, stream = sm.list[now.entry].stream;
             const long long cells = (long long)a.rows * a.most, at = (long long)row * a.most + now.part;
-            Sums p{run.m, parts(run.t).x + parts(run.t).y};
+            Sums<double> p{run.m, (double)parts(run.t).x + (double)parts(run.t).y};
             const float own = p.m;
             p.join_warp();
-            if (lane == 0) a.part[stream * cells + at] = make_float2(p.m, p.t);
+            float w = 0.f;
             if constexpr (FULL) {
-                Sums q{run.n, parts(run.r).x + parts(run.r).y};
-                const float w = warp_sum((parts(run.w).x + parts(run.w).y) * __expf(own - p.m));
+                Sums<double> q{run.n, (double)parts(run.r).x + (double)parts(run.r).y};
+                w = warp_sum((parts(run.w).x + parts(run.w).y) * exp_of_gap(own - p.m));
                 q.join_warp();
-                if (lane == 0) {
-                    a.part[cells + at] = make_float2(q.m, q.t);
-                    a.cross[at] = w;
-                }
+                if (lane == 0) a.part[cells + at] = Part{q.t, q.m, 0.f};
             }
+            if (lane == 0) a.part[stream * cells + at] = Part{p.t, p.m, w};
             if (now.part == 0 && lane == 0) {                   // x is the row's first element here
                 const long long label = a.labels[row] - a.v0;
                 a.target[(long long)stream * a.rows + row] = label >= 0 && label < a.vocab ? Elem<T>::get(now.x[label]) : 0.f;
@@ -606,8 +631,7 @@ constexpr int ROWS = THREADS / LANES;                           // rows of a blo
 constexpr int NEAR = 256;                                       // sequences whose sums stay in shared memory
 
 struct RowSums {
-    const float2* part;
-    const float* cross;
+    const Part* part;
     const float* target;
     const long long* labels;
     const int* ticket;             // [1]: chunks of a row, where `chunks` does not say
@@ -621,24 +645,34 @@ template <typename V> __device__ __forceinline__ V lanes_sum(V v) {
     return v;
 }
 // A lane's first chunk of a row, asked for before it is known how many there are.
-__device__ __forceinline__ float2 peek(const RowSums& r, int stream, int row, bool on) {
+__device__ __forceinline__ Part peek(const RowSums& r, int stream, int row, bool on) {
     const int lane = threadIdx.x % LANES;
-    return on && lane < r.most ? r.part[((long long)stream * r.rows + row) * r.most + lane] : make_float2(-FLT_MAX, 0.f);
+    return on && lane < r.most ? r.part[((long long)stream * r.rows + row) * r.most + lane] : Part{0.0, -FLT_MAX, 0.f};
 }
-// Joins a row's chunks: maximum and sum, in 64 bits.  All lanes of a warp come here, each with its row.
-__device__ __forceinline__ void join(const RowSums& r, int chunks, int stream, int row, bool on, float2 own, float& m, double& t) {
+// Joins a row's chunks, in 64 bits: maximum, sum and, where asked for, the sum of p (x - y).  All lanes of a warp come here, each with
+// its row.
+template <bool CROSS>
+__device__ __forceinline__ void join(const RowSums& r, int chunks, int stream, int row, bool on, Part own, float& m, double& t, double& w) {
     const int lane = threadIdx.x % LANES;
-    const float2* p = r.part + ((long long)stream * r.rows + row) * r.most;
-    if (lane >= chunks) own = make_float2(-FLT_MAX, 0.f);
-    m = own.x;
+    const Part* p = r.part + ((long long)stream * r.rows + row) * r.most;
+    if (lane >= chunks) own = Part{0.0, -FLT_MAX, 0.f};
+    m = own.m;
     if (on)
-        for (int k = lane + LANES; k < chunks; k += LANES) m = fmaxf(m, p[k].x);
+        for (int k = lane + LANES; k < chunks; k += LANES) m = fmaxf(m, p[k].m);
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    t = (double)own.y * (double)__expf(own.x - m);
+    const double scale = exp_of_gap(own.m - m);
+    t = own.t * scale;
+    if constexpr (CROSS) w = (double)own.w * scale;
     if (on)
-        for (int k = lane + LANES; k < chunks; k += LANES) t += (double)p[k].y * (double)__expf(p[k].x - m);
+        for (int k = lane + LANES; k < chunks; k += LANES) {
+            const Part next = p[k];
+            const double factor = exp_of_gap(next.m - m);
+            t += next.t * factor;
+            if constexpr (CROSS) w += (double)next.w * factor;
+        }
     t = lanes_sum(t);
+    if constexpr (CROSS) w = lanes_sum(w);
 }
 // Log-probability of a label whose logit is x.
 __device__ __forceinline__ double label_logp(long long vocab, long long label, float x, float m, double t) {
@@ -720,14 +754,14 @@ __global__ void __launch_bounds__(THREADS) preference_kernel(const PreferenceArg
     const long long label = on ? a.sums.labels[row] : 0;
     const float given = on && a.ref_logp ? a.ref_logp[row] : 0.f;
     launch::wait_for_predecessor();
-    const float2 own = peek(a.sums, 0, row, on), own_r = a.has_ref_logits ? peek(a.sums, 1, row, on) : make_float2(0.f, 0.f);
+    const Part own = peek(a.sums, 0, row, on), own_r = peek(a.sums, 1, row, on && a.has_ref_logits);
     const float x = on ? a.sums.target[row] : 0.f, y = on && a.has_ref_logits ? a.sums.target[(long long)a.sums.rows + row] : 0.f;
     const int chunks = a.sums.chunks ? a.sums.chunks : a.sums.ticket[1];
     double v[2] = {0.0, 0.0};
     float m, mr = 0.f;
-    double t, tr = 0.0;
-    join(a.sums, chunks, 0, row, on, own, m, t);
-    if (a.has_ref_logits) join(a.sums, chunks, 1, row, on, own_r, mr, tr);
+    double t, tr = 0.0, none;
+    join<false>(a.sums, chunks, 0, row, on, own, m, t, none);
+    if (a.has_ref_logits) join<false>(a.sums, chunks, 1, row, on, own_r, mr, tr, none);
     if (j < a.s && threadIdx.x % LANES == 0) {
         a.row[row] = on ? make_float2(m, __frcp_rn((float)t)) : make_float2(0.f, 0.f);
         if (on) {
@@ -844,22 +878,15 @@ __global__ void __launch_bounds__(THREADS) policy_kernel(const PolicyArgs a) {
     const double adv = on ? a.advantages[seq * a.adv_n + j * a.adv_s] : 0.f;
     const float old = on && a.old_logp ? a.old_logp[row] : 0.f, given = on && a.ref_logp ? a.ref_logp[row] : 0.f;
     launch::wait_for_predecessor();
-    const float2 own = peek(a.sums, 0, row, on), own_q = a.has_ref_logits ? peek(a.sums, 1, row, on) : make_float2(0.f, 0.f);
+    const Part own = peek(a.sums, 0, row, on), own_q = peek(a.sums, 1, row, on && a.has_ref_logits);
     const bool two = a.has_ref_logits && a.kl != KL_FULL;
     const float x = on ? a.sums.target[row] : 0.f, y = on && two ? a.sums.target[(long long)a.sums.rows + row] : 0.f;
     const int chunks = a.sums.chunks ? a.sums.chunks : a.sums.ticket[1];
     double v[4] = {0.0, 0.0, 0.0, 0.0};
     float m, mq = 0.f;
-    double t, tq = 0.0, cross = 0.0;
-    join(a.sums, chunks, 0, row, on, own, m, t);
-    if (a.has_ref_logits) join(a.sums, chunks, 1, row, on, own_q, mq, tq);
-    if (a.kl == KL_FULL) {
-        const long long at = (long long)row * a.sums.most;
-        if (on)
-            for (int k = threadIdx.x % LANES; k < chunks; k += LANES)
-                cross += (double)a.sums.cross[at + k] * (double)__expf(a.sums.part[at + k].x - m);
-        cross = lanes_sum(cross);
-    }
+    double t, tq = 0.0, cross = 0.0, none;
+    join<true>(a.sums, chunks, 0, row, on, own, m, t, cross);
+    if (a.has_ref_logits) join<false>(a.sums, chunks, 1, row, on, own_q, mq, tq, none);
     if (j < a.s && threadIdx.x % LANES == 0) {
         float2 keep = make_float2(0.f, 0.f);
         float slope = 0.f, shift = 0.f, logp = 0.f;
@@ -1239,7 +1266,7 @@ __global__ void __launch_bounds__(TPB, BLOCKS) policy_row_kernel(const AtOnceArg
     constexpr int N = Elem<T>::PER_16, U = 4, TEAM = TPB / 32, PARTS = 4;
     extern __shared__ __align__(16) unsigned char raw_smem[];
     uint4* xs = reinterpret_cast<uint4*>(raw_smem);
-    __shared__ Sums ps[TEAM];
+    __shared__ Sums<double> ps[TEAM];
     __shared__ RowGrad grad;
     __shared__ int where;
     __shared__ double terms[4], sums[4];                        // of a row and of all of them
@@ -1340,14 +1367,14 @@ __global__ void __launch_bounds__(TPB, BLOCKS) policy_row_kernel(const AtOnceArg
             }
         }
         const float2 halves = parts(run.t);
-        Sums p{run.m, halves.x + halves.y};
+        Sums<double> p{run.m, (double)halves.x + (double)halves.y};
         p.join_warp();
         if (tid % 32 == 0) ps[tid / 32] = p;
         __syncthreads();
         if (tid < 32) {
             const bool is = tid < TEAM;
             const float m = warp_max(is ? ps[tid].m : -FLT_MAX);
-            const double t = warp_sum(is ? (double)ps[tid].t * (double)__expf(ps[tid].m - m) : 0.0);
+            const double t = warp_sum(is ? ps[tid].t * (double)exp_of_gap(ps[tid].m - m) : 0.0);
             if (tid == 0) {
                 const double l = label_logp(a.vocab, label, own, m, t);
                 const RowTerm r(a.kl, a.low, a.high, a.kl_beta, l, a.old_logp != nullptr, old, adv, a.ref_wide ? wide : (double)given,
@@ -1501,8 +1528,7 @@ struct LossCall {
     long long yn, ys;
     const long long* labels;
     const float* mask;
-    float2* part;                  // scratch: [streams][n * s, most]
-    float* cross;                  // scratch: [n * s, most], for the KL over the vocabulary
+    Part* part;                    // scratch: [streams][n * s, most]
     float* target;                 // scratch: [streams][n * s]
     int* ticket;                   // scratch: 2
     double* sums;                  // scratch: [n * pieces + n, 2 or 4]
@@ -1560,7 +1586,7 @@ int neox_loss_forward(const void* packed) {
     if (c.first) {
         const StatsPlan p(rows, c.vocab, c.dtype, full);
         if (p.most != c.most) return NEOX_ERR_SHAPE;
-        const StatsArgs a = {{c.x, c.xn, c.xs}, {c.y, c.yn, c.ys}, c.labels, c.mask, c.part, c.cross, c.target, c.ticket, c.v0,
+        const StatsArgs a = {{c.x, c.xn, c.xs}, {c.y, c.yn, c.ys}, c.labels, c.mask, c.part, c.target, c.ticket, c.v0,
                              (int)rows, c.s, c.vocab, streams, p.chunks, p.most};
         const int blocks = neox_sm_count();
         if (full) FOR_TYPE(c.dtype, LAUNCH_STATS(T, true));
@@ -1568,7 +1594,7 @@ int neox_loss_forward(const void* packed) {
         if (launched() != 0) return NEOX_ERR_LAUNCH;
     }
     if (!c.second) return 0;
-    const RowSums sums = {c.part, c.cross, c.target, c.labels, c.ticket, c.whole, (int)rows, c.most, c.chunks};
+    const RowSums sums = {c.part, c.target, c.labels, c.ticket, c.whole, (int)rows, c.most, c.chunks};
     const dim3 grid((unsigned)(c.n * pieces));
     if (c.policy) {
         const PolicyArgs a = {sums, c.mask, c.advantages, c.adv_n, c.adv_s, c.old_logp, c.ref_logp, c.y != nullptr, c.n, c.s,

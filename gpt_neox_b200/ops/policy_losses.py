@@ -4,7 +4,9 @@ with a KL term.
 Both are functions of the log-probabilities that a policy gives the labels of the positions whose ``loss_mask`` is not zero.
 Positions of mask zero -- prompts, padding -- are not read: their logits may hold anything and their gradient is zero.  On a GPU
 the logits are streamed once for the loss and once for its gradient -- a policy loss writes both from one reading where it can --
-(``csrc/policy_losses.cu``), in their own type and memory order; the sums over a sequence and everything behind them are in 64 bits.
+(``csrc/policy_losses.cu``), in their own type and memory order.  Exponentials and a lane's sums of them are in 32 bits, a row's log-probability, the sums
+over a sequence, the ratios, z and the loss in 64; coefficients of the gradient and outputs are rounded to 32.  (Over a split
+vocabulary the ranks' sums are joined in 32 bits.)
 ``*_ref`` are the same losses in plain PyTorch: the CPU path and the statement the kernels are tested against.
 
 Reference counterparts: the DPO and REINFORCE objectives of ``megatron/training.py:533-939``, which form ``[b, s, V]``
@@ -38,7 +40,7 @@ native._CountingLib._NOT_LAUNCHES.update({"neox_vocab_chunks", "neox_loss_pieces
 _MOST_TOKENS = 1 << 30                  # the kernels number them, and steps past the last one, in 32 bits
 
 # The kernels' arguments in the order of LossCall (csrc/policy_losses.cu): addresses and 64-bit words, doubles, ints.
-_CALL = struct.Struct("@37q5d12i")
+_CALL = struct.Struct("@36q5d12i")
 
 
 class PreferenceLoss(NamedTuple):
@@ -119,8 +121,8 @@ def _layout(n, s, v, dtype, streams, width, full, device):
     """Chunks of a row, and where the parts of a forward's one buffer begin, in bytes, with its size in floats at the end::
 
         sums    [n * (pieces + 1), width] fp64    what the joining kernel's blocks leave
-        part    [streams, rows, most, 2]          maximum and sum of every chunk of a row, policy and reference
-        cross   [rows, most]                      sum of p (x - y), for the KL over the vocabulary
+        part    [streams, rows, most, 4]          of every chunk of a row, policy and reference: sum in 64 bits, maximum and, for the
+                                                  KL over the vocabulary, sum of p (x - y)
         target  [streams, rows]                   the labels' logits
         ticket  [2] int32
         row     [rows, 2]                         maximum and 1 / sum, from here on kept for the backward
@@ -130,7 +132,7 @@ def _layout(n, s, v, dtype, streams, width, full, device):
     """
     L, rows = native.lib(), n * s
     most = L.neox_vocab_chunks(rows, v, dtype, full)
-    sizes = (2 * width * n * (L.neox_loss_pieces(s) + 1), 2 * streams * rows * most, rows * most * full, streams * rows, 2,
+    sizes = (2 * width * n * (L.neox_loss_pieces(s) + 1), 4 * streams * rows * most, streams * rows, 2,
              2 * rows, n, rows * (width == 4), rows * full)
     at, offsets = 0, []
     for size in sizes:
@@ -143,20 +145,25 @@ def _reduced(buf, at, streams, rows, most, full, group):
     """Statistics of whole rows from those of every rank's share of the vocabulary: the chunks are joined here and two all-reduces
     follow, maxima, then sums and label logits.  What stands in rows of mask zero is never read."""
     import torch.distributed as dist
-    _, part, cross, target, ticket = (o // 4 for o in at[:5])
-    part = buf[part:part + 2 * streams * rows * most].view(streams, rows, most, 2)
+    _, part, target, ticket = (o // 4 for o in at[:4])
+    part = buf[part:part + 4 * streams * rows * most].view(streams, rows, most, 4)
     there = torch.arange(most, device=buf.device) < buf[ticket:ticket + 2].view(torch.int32)[1]
-    local = torch.where(there, part[..., 0], torch.finfo(torch.float32).min)
+    local = torch.where(there, part[..., 2], torch.finfo(torch.float32).min)
     top = local.amax(-1)
     dist.all_reduce(top, op=dist.ReduceOp.MAX, group=group)
     scale = (local - top[..., None]).exp()
-    terms = [torch.where(there, part[..., 1] * scale, 0.0).sum(-1),
+    terms = [torch.where(there, part.view(torch.float64)[..., 0] * scale, 0.0).sum(-1).float(),
              buf[target:target + (1 if full else streams) * rows].view(-1, rows)]
     if full:
-        terms.append(torch.where(there, buf[cross:cross + rows * most].view(rows, most) * scale[0], 0.0).sum(-1)[None])
+        terms.append(torch.where(there, part[0, ..., 3] * scale[0], 0.0).sum(-1)[None])
     both = torch.cat(terms)
     dist.all_reduce(both, group=group)
-    return torch.stack([top, both[:streams]], -1), both[streams:], both[-1]
+    whole = torch.empty(streams, rows, 4, dtype=torch.float32, device=buf.device)
+    whole.view(torch.float64)[..., 0] = both[:streams]
+    whole[..., 2] = top
+    if full:
+        whole[0, :, 3] = both[-1]
+    return whole, both[streams:]
 
 
 def _forward(x, y, labels, mask, width, loss, kl_mean, clipped, logp, ref, old_logp, ref_logp, adv, kl, by_sequence, beta, smoothing,
@@ -169,7 +176,7 @@ def _forward(x, y, labels, mask, width, loss, kl_mean, clipped, logp, ref, old_l
     most, *at, total = _layout(n, s, v, dt, streams, width, full, x.get_device())
     buf = torch.empty(total, dtype=torch.float32, device=x.device)
     base = buf.data_ptr()
-    sums, part, cross, target, ticket, row, coef, slope, shift = [base + o for o in at]
+    sums, part, target, ticket, row, coef, slope, shift = [base + o for o in at]
     y_ = x if y is None else y
     head = (x.data_ptr(), x.stride(0), x.stride(1), 0 if y is None else y.data_ptr(), y_.stride(0), y_.stride(1),
             labels.data_ptr(), mask.data_ptr())
@@ -183,11 +190,11 @@ def _forward(x, y, labels, mask, width, loss, kl_mean, clipped, logp, ref, old_l
     run = native.lib().neox_loss_forward
     policy = width == 4
     if tp == 1:
-        native.check(run(_CALL.pack(*head, part, cross, target, *tail, most, 0, policy, 1, 1, 0)), "neox_loss_forward")
+        native.check(run(_CALL.pack(*head, part, target, *tail, most, 0, policy, 1, 1, 0)), "neox_loss_forward")
     else:
-        native.check(run(_CALL.pack(*head, part, cross, target, *tail, most, 0, policy, 1, 0, 0)), "neox_loss_forward")
-        pairs, targets, crosses = _reduced(buf, at, streams, n * s, most, full, group())
-        native.check(run(_CALL.pack(*head, pairs.data_ptr(), crosses.data_ptr(), targets.data_ptr(), *tail, 1, 1, policy, 0, 1, 0)),
+        native.check(run(_CALL.pack(*head, part, target, *tail, most, 0, policy, 1, 0, 0)), "neox_loss_forward")
+        whole, targets = _reduced(buf, at, streams, n * s, most, full, group())
+        native.check(run(_CALL.pack(*head, whole.data_ptr(), targets.data_ptr(), *tail, 1, 1, policy, 0, 1, 0)),
                      "neox_loss_forward")
     return buf, rank * v
 
@@ -213,7 +220,7 @@ def _backward(x, y, labels, mask, g, row, coef, slope, shift, first, g_loss, g_l
     n, s, v = x.shape
     y_ = x if y is None else y
     call = _CALL.pack(x.data_ptr(), x.stride(0), x.stride(1), y_.data_ptr(), y_.stride(0), y_.stride(1), labels.data_ptr(),
-                      mask.data_ptr(), 0, 0, 0, 0, 0, row, coef, slope, shift, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, g.data_ptr(), g.stride(0),
+                      mask.data_ptr(), 0, 0, 0, 0, row, coef, slope, shift, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, g.data_ptr(), g.stride(0),
                       g.stride(1), 0 if g_loss is None else g_loss.data_ptr(), 0 if g_logp is None else g_logp.data_ptr(), first, 0,
                       native.stream_ptr(), 0, 0, beta, 0.0, 0.0, 0.0, expected, n, s, v, _DT[x.dtype], 0, 0, 0, 0, 0, 0, 0, done)
     native.check(native.lib().neox_loss_backward(call), "neox_loss_backward")
@@ -225,7 +232,7 @@ def _kept(x, buf, streams, width, full):
     n, s, v = x.shape
     at = _layout(n, s, v, _DT[x.dtype], streams, width, full, x.get_device())
     base = buf.data_ptr()
-    return base + at[6], base + at[7], base + at[8], base + at[9] if full else 0
+    return base + at[5], base + at[6], base + at[7], base + at[8] if full else 0
 
 
 def _preference_values(x, labels, mask, ref_logits, ref_logp, beta, smoothing):
@@ -305,7 +312,7 @@ def _policy_at_once(x, labels, mask, adv, old_logp, ref_logp, wide, low, high, k
     buf = torch.empty(total, dtype=torch.float32, device=dev)
     row, coef, slope, terms = [buf.data_ptr() + o for o in at]
     g = _new_grad(x)
-    call = _CALL.pack(x.data_ptr(), x.stride(0), x.stride(1), 0, 0, 0, labels.data_ptr(), mask.data_ptr(), 0, 0, 0, 0, 0, row, coef,
+    call = _CALL.pack(x.data_ptr(), x.stride(0), x.stride(1), 0, 0, 0, labels.data_ptr(), mask.data_ptr(), 0, 0, 0, 0, row, coef,
                       slope, 0, loss.data_ptr(), kl_mean.data_ptr(), clipped.data_ptr(), logp.data_ptr(), 0,
                       0 if old_logp is None else old_logp.data_ptr(), 0 if ref_logp is None else ref_logp.data_ptr(),
                       adv.data_ptr(), adv.stride(0) if adv.shape[0] > 1 else 0, adv.stride(1) if adv.shape[1] > 1 else 0,

@@ -220,3 +220,26 @@ def test_clipped_loss_over_a_split_vocabulary(kl, ref, dtype, monkeypatch):
         want = grad[..., r * cut:(r + 1) * cut].double()
         off = (got[r][3].double() - want).abs()
         assert bool((off <= torch.finfo(dtype).eps * want.abs() + 8 * ROW * most / n).all())
+
+
+@pytest.mark.parametrize("dtype,v,spread,train", [(torch.bfloat16, 50304, 2.0, True), (torch.float32, 50432, 2.0, False),
+                                                  (torch.float32, 9001, 2.0, True), (torch.bfloat16, 32000, 5.0, False)])
+def test_log_probabilities_are_not_off_on_average(dtype, v, spread, train):
+    """Half of the rows' log-probabilities, taken as the difference to their 64-bit values rounded to 32, within 3e-8: a loss of terms of
+    either sign keeps its digits.  The lanes' roundings average out over a row (2^-22 each, over hundreds of lanes: 5e-9 and less).  What
+    is left is the mean error of the exponential, from -5e-8 (of ex2) up by 1.3e-8 for every unit of the argument (log2 e in 32 bits):
+    the words that count lie 2 to 6 below their lane's largest, and the factors of whole sums are corrected."""
+    s = 96
+    g = torch.Generator(device=DEV).manual_seed(v)
+    x = torch.randn(1, s, v, device=DEV, generator=g, dtype=dtype).mul_(spread)
+    labels = torch.randint(0, v, (1, s), device=DEV, generator=g)
+    want = x.double().log_softmax(-1).gather(-1, labels[..., None])[..., 0]
+    near = want.float()
+    x.requires_grad_(train)
+    off = []
+    for j in range(s):
+        mask = torch.zeros(1, s, device=DEV)
+        mask[0, j] = 1.0
+        off.append(PL.policy_loss(x, labels, mask, mask, ref_logp=near, kl="kl", kl_beta=0.1).kl.double() - (want - near.double())[0, j])
+    off = torch.stack(off).abs()
+    assert float(off.median()) <= 3e-8 and float(off.max()) <= ROW
