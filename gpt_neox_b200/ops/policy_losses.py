@@ -4,9 +4,9 @@ with a KL term.
 Both are functions of the log-probabilities that a policy gives the labels of the positions whose ``loss_mask`` is not zero.
 Positions of mask zero -- prompts, padding -- are not read: their logits may hold anything and their gradient is zero.  On a GPU
 the logits are streamed once for the loss and once for its gradient -- a policy loss writes both from one reading where it can --
-(``csrc/policy_losses.cu``), in their own type and memory order.  Exponentials and a lane's sums of them are in 32 bits, a row's log-probability, the sums
-over a sequence, the ratios, z and the loss in 64; coefficients of the gradient and outputs are rounded to 32.  (Over a split
-vocabulary the ranks' sums are joined in 32 bits.)
+(``csrc/policy_losses.cu``), in their own type and memory order.  Exponentials and a lane's sums of them are in 32 bits; a row's
+log-probability, the sums over a sequence, the ratios, z and the loss are in 64; coefficients of the gradient and outputs are
+rounded to 32.  (Over a split vocabulary the ranks' sums are joined in 32 bits.)
 ``*_ref`` are the same losses in plain PyTorch: the CPU path and the statement the kernels are tested against.
 
 Reference counterparts: the DPO and REINFORCE objectives of ``megatron/training.py:533-939``, which form ``[b, s, V]``
