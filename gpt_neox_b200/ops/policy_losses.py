@@ -37,7 +37,7 @@ native._ARGTYPES.update({
 })
 native._CountingLib._NOT_LAUNCHES.update({"neox_vocab_chunks", "neox_loss_pieces", "neox_policy_fits"})
 
-_MOST_TOKENS = 1 << 30                  # the kernels number them, and steps past the last one, in 32 bits
+_MOST_TOKENS = _MOST_WORDS = 1 << 30    # the kernels number them, and steps past the last one, in 32 bits
 
 # The kernels' arguments in the order of LossCall (csrc/policy_losses.cu): addresses and 64-bit words, doubles, ints.
 _CALL = struct.Struct("@36q5d12i")
@@ -74,6 +74,8 @@ def _check(logits, labels, loss_mask, ref_logits, ref_logp):
         raise ValueError(f"logits are floating-point numbers, got {logits.dtype}")
     if logits.shape[0] * logits.shape[1] >= _MOST_TOKENS:
         raise ValueError(f"a batch has fewer than {_MOST_TOKENS} tokens, got {tuple(logits.shape)}")
+    if logits.shape[2] >= _MOST_WORDS:
+        raise ValueError(f"a vocabulary, or a rank's share of it, has fewer than {_MOST_WORDS} words, got {logits.shape[2]}")
     for name, t in (("labels", labels), ("loss_mask", loss_mask), ("ref_logp", ref_logp)):
         if t is not None and t.shape != logits.shape[:2]:
             raise ValueError(f"{name} is {tuple(t.shape)}, the logits' sequences are {tuple(logits.shape[:2])}")

@@ -146,3 +146,14 @@ def test_example_server_samples_from_the_policy_whose_log_probabilities_it_sends
     assert sampler.generate([3, 4], 1, 2) == [[3, 4]] and seen[0]["top_p"] == 0.95
     sampler.generate([3, 4], 1, 2, whole=True)
     assert seen[1]["top_p"] == 1.0 and seen[1]["top_k"] == 0 and seen[1]["temperature"] == 1.0 and seen[1]["do_sample"]
+
+
+# ---------------------------------------------------------------------------------------------- arguments of the losses
+def test_vocabularies_that_the_kernels_cannot_number_are_refused():
+    from gpt_neox_b200.ops import policy_losses as PL
+    many = torch.zeros(1, 1, 1).expand(2, 1, 2 ** 30)
+    labels, mask = torch.zeros(2, 1, dtype=torch.long), torch.ones(2, 1)
+    with pytest.raises(ValueError, match="words"):
+        PL.preference_loss(many, labels, mask, 0.1)
+    with pytest.raises(ValueError, match="words"):
+        PL.policy_loss(many, labels, mask, mask)
