@@ -62,7 +62,7 @@ class PolicyLoss(NamedTuple):
 
 # ---------------------------------------------------------------------------------------------- arguments
 def _constant(name, t):
-    if t is not None and t.requires_grad and torch.is_grad_enabled():
+    if isinstance(t, torch.Tensor) and t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} is a constant of this loss and gets no gradient: detach it")
     return t
 
@@ -488,10 +488,12 @@ def preference_loss(logits, labels, loss_mask, beta, ref_logits: Optional[torch.
 
     ``logits``: ``[n, s, V / tp]`` (bf16, fp16 or fp32, any strides with a contiguous vocabulary); ``labels``: ``[n, s]`` over the
     whole vocabulary, one outside makes its pair NaN; ``loss_mask``: ``[n, s]``, the weight of every position.  The reference is
-    ``ref_logits`` (shape and type of ``logits``), ``ref_logp`` (``[n, s]``) or nothing.  Reference and mask are constants.  A
+    ``ref_logits`` (shape and type of ``logits``), ``ref_logp`` (``[n, s]``) or nothing.  Reference, mask and numbers are constants.  A
     sequence without a kept position has log-probability zero.  The gradient can be taken once, not differentiated again.
     """
     _check(logits, labels, loss_mask, ref_logits, ref_logp)
+    _constant("beta", beta)
+    _constant("label_smoothing", label_smoothing)
     if logits.shape[0] % 2:
         raise ValueError(f"pairs are [chosen; rejected]: an even number of sequences, got {logits.shape[0]}")
     if not 0.0 <= label_smoothing < 1.0:
@@ -533,6 +535,8 @@ def policy_loss(logits, labels, loss_mask, advantages, old_logp: Optional[torch.
     """
     _check(logits, labels, loss_mask, ref_logits, ref_logp)
     n, s = logits.shape[:2]
+    for name, t in (("clip_low", clip_low), ("clip_high", clip_high), ("kl_beta", kl_beta)):
+        _constant(name, t)
     clip_high = clip_low if clip_high is None else clip_high
     if advantages.dim() == 1:
         advantages = advantages[:, None]

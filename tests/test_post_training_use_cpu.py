@@ -157,3 +157,16 @@ def test_vocabularies_that_the_kernels_cannot_number_are_refused():
         PL.preference_loss(many, labels, mask, 0.1)
     with pytest.raises(ValueError, match="words"):
         PL.policy_loss(many, labels, mask, mask)
+
+
+def test_numbers_that_ask_for_a_gradient_are_refused():
+    """The kernels take them as numbers: a gradient would be missing without a word."""
+    from gpt_neox_b200.ops import policy_losses as PL
+    x, labels, mask = torch.randn(2, 3, 5), torch.zeros(2, 3, dtype=torch.long), torch.ones(2, 3)
+    learnt = torch.tensor(0.1, requires_grad=True)
+    for call in (lambda t: PL.preference_loss(x, labels, mask, t), lambda t: PL.preference_loss(x, labels, mask, 0.1, label_smoothing=t),
+                 lambda t: PL.policy_loss(x, labels, mask, mask, ref_logp=mask, kl_beta=t),
+                 lambda t: PL.policy_loss(x, labels, mask, mask, clip_low=t), lambda t: PL.policy_loss(x, labels, mask, mask, clip_high=t)):
+        with pytest.raises(ValueError, match="constant"):
+            call(learnt)
+        call(learnt.detach())
