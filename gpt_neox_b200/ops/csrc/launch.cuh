@@ -5,6 +5,8 @@
 // earlier kernel may touch; it may then be sure that everything before it in the stream is done, because each kernel in
 // such a chain waits for its own predecessor before it can finish.  `let_successor_start()` allows the next one in.  Before
 // the wait only addresses may be prefetched into L2: that is coherent, so even data the predecessor writes stays right.
+// One exception: a kernel whose predecessor is always launched in the ordinary way may read before the wait what is older than that
+// predecessor, which began when all of it was done.  A kernel that does so says it, and whose launch it relies on.
 #pragma once
 #include <cuda_runtime.h>
 

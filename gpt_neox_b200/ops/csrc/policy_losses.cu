@@ -746,6 +746,9 @@ struct PreferenceArgs {
 // z = beta ((P_c - P_r) - (R_c - R_r)),
 // loss = -(1 - e) log sigma(z) - e log sigma(-z),  d loss / d P_c = -beta ((1 - e) sigma(-z) - e sigma(z)) / pairs = -d/d P_r.
 // Latency bounds it, a dozen trips to L2 one after another: some 7 us behind the statistics, whether of 96 rows or of 8192.
+// Mask, labels and stored log-probabilities are read before the wait, here and in `policy_kernel`: whatever wrote them is done, because
+// the launch in front -- the statistics, or the last of the operations that join the ranks -- is not an overlapped one and began after
+// it.  Statistics launched with overlap would have to send these reads behind the wait.
 __global__ void __launch_bounds__(THREADS) preference_kernel(const PreferenceArgs a) {
     const int seq = blockIdx.x / a.pieces, j = (blockIdx.x % a.pieces) * ROWS + threadIdx.x / LANES;
     const int row = seq * a.s + j;
@@ -1144,7 +1147,7 @@ struct AtOnceArgs {
 
 // What each sequence's slopes are multiplied by: 1 / (sum of the mask), of the whole batch or of the sequence and then shared by the
 // sequences that keep something; and the order of the rows.  One block; what it does takes as long as three trips to memory or, for
-// many rows, as two readings of the mask.
+// many rows, as three readings of the mask: sums, count, places.
 __global__ void __launch_bounds__(1024, 1) policy_share_kernel(const AtOnceArgs a) {
     __shared__ double near[32][2];
     __shared__ int kept_by[32];
